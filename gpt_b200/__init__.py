@@ -21,6 +21,8 @@ LIB_PATH = os.path.join(_HERE, "lib", "libgptb200.so")
 
 MODE_3XTF32 = 0
 MODE_TF32 = 1
+DTYPE_BF16, DTYPE_F32 = 0, 1           # gptb200_dtype
+KV_BF16, KV_F32, KV_E4M3 = 0, 1, 2     # gptb200_kv_kind
 
 # Every symbol include/gptb200.h declares (checked by the CPU test-suite against the built library).
 EXPORTED_SYMBOLS = [
@@ -38,6 +40,7 @@ EXPORTED_SYMBOLS = [
     "gptb200_softmax_cross_entropy_inplace", "gptb200_row_loss_mean", "gptb200_cross_entropy_loss_from_logits",
     "gptb200_adamw_step", "gptb200_scale_and_clip_grad", "gptb200_memory_info", "gptb200_clip_adamw_packed",
     "gptb200_embedding_decode", "gptb200_kv_cache_fill", "gptb200_attention_decode", "gptb200_advance_position",
+    "gptb200_kv_pages_write", "gptb200_kv_pages_read", "gptb200_attention_paged",
     "gptb200_loader_create", "gptb200_loader_destroy", "gptb200_loader_num_samples", "gptb200_loader_reset_epoch", "gptb200_loader_next_batch",
     "gptb200_bias_grad_noalloc",
     "gptb200_decoder_check_config", "gptb200_decoder_load", "gptb200_decoder_destroy", "gptb200_decoder_context", "gptb200_decoder_vocab",
@@ -50,6 +53,16 @@ class GptB200Error(RuntimeError):
     def __init__(self, status: int, what: str, detail: str = ""):
         self.status = status
         super().__init__(f"{what}: status {status}" + (f" ({detail})" if detail else ""))
+
+
+class _KvPages(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("scales", ctypes.c_void_p), ("kind", ctypes.c_int), ("num_pages", ctypes.c_int), ("page_tokens", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("dim", ctypes.c_int)]
+
+
+class _KvRows(ctypes.Structure):
+    _fields_ = [("row_starts", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("page_table", ctypes.c_void_p), ("sequences", ctypes.c_int),
+                ("table_pitch", ctypes.c_int), ("rows", ctypes.c_int), ("max_new", ctypes.c_int)]
 
 
 _lib = None
@@ -128,6 +141,9 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         "gptb200_kv_cache_fill": (i, [vp, fp, fp, i, i, i, i]),
         "gptb200_attention_decode": (i, [vp, fp, fp, fp, fp, i, i, i, i]),
         "gptb200_advance_position": (i, [vp, fp]),
+        "gptb200_kv_pages_write": (i, [vp, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows), fp, ctypes.c_longlong, fp, ctypes.c_longlong, i]),
+        "gptb200_kv_pages_read": (i, [vp, fp, ctypes.c_longlong, fp, ctypes.c_longlong, i, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows)]),
+        "gptb200_attention_paged": (i, [vp, fp, ctypes.c_longlong, fp, fp, ctypes.c_longlong, i, i, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows), f32, f32, i, i]),
         "gptb200_loader_create": (i, [ctypes.POINTER(vp), ctypes.c_char_p, i]),
         "gptb200_loader_destroy": (i, [vp]),
         "gptb200_loader_num_samples": (ctypes.c_longlong, [vp]),
@@ -230,6 +246,24 @@ def _ptr(t: Any) -> int | None:
     if isinstance(t, int):
         return t
     return int(t.data_ptr())
+
+
+class KvPages:
+    """A layer's pool of a paged cache of keys and values (gptb200_kv_pages in include/gptb200.h): data [num_pages][2][kv_heads][page_tokens][dim], for
+    KV_E4M3 scales [num_pages][2][kv_heads][page_tokens].  Keeps what it is given alive; calls take it as often as they like."""
+
+    def __init__(self, data, scales, kind: int, num_pages: int, page_tokens: int, kv_heads: int, dim: int):
+        self._tensors = (data, scales)
+        self.struct = _KvPages(_ptr(data), _ptr(scales), kind, num_pages, page_tokens, kv_heads, dim)
+
+
+class KvRows:
+    """The new rows of a call on a paged cache (gptb200_kv_rows in include/gptb200.h): int32 device arrays row_starts [sequences + 1], lengths [sequences] and
+    page_table [sequences][table_pitch], the tensors' rows and the most new rows of a sequence.  Keeps the arrays alive; their contents may change between calls."""
+
+    def __init__(self, row_starts, lengths, page_table, sequences: int, table_pitch: int, rows: int, max_new: int):
+        self._tensors = (row_starts, lengths, page_table)
+        self.struct = _KvRows(_ptr(row_starts), _ptr(lengths), _ptr(page_table), sequences, table_pitch, rows, max_new)
 
 
 class Backend:
@@ -342,6 +376,21 @@ class Backend:
         self._check(self._lib.gptb200_unembed_backward(self._ctx, _ptr(grad_x), _ptr(grad_wte), _ptr(grad_y), _ptr(x),
                                                        _ptr(wte), batch_size * seq_len, hidden_size, vocab_size_padded),
                     "gptb200_unembed_backward")
+
+    # ---- a paged cache of keys and values (include/gptb200.h: gptb200_kv_pages_*, gptb200_attention_paged); pitches in elements
+    def kv_pages_write(self, pages: KvPages, rows: KvRows, k, k_pitch: int, v, v_pitch: int, dtype: int) -> None:
+        """The rows' keys and values [rows x kv_heads * dim] go into their sequences' pages."""
+        self._check(self._lib.gptb200_kv_pages_write(self._ctx, pages.struct, rows.struct, _ptr(k), k_pitch, _ptr(v), v_pitch, dtype), "gptb200_kv_pages_write")
+
+    def kv_pages_read(self, k, k_pitch: int, v, v_pitch: int, dtype: int, pages: KvPages, rows: KvRows) -> None:
+        """The rows' keys and values come back out of the pages."""
+        self._check(self._lib.gptb200_kv_pages_read(self._ctx, _ptr(k), k_pitch, _ptr(v), v_pitch, dtype, pages.struct, rows.struct), "gptb200_kv_pages_read")
+
+    def attention_paged(self, out, out_pitch: int, lse, q, q_pitch: int, dtype: int, heads: int, pages: KvPages, rows: KvRows, scale: float, cap: float = 0.0,
+                        window: int = 0, sinks: int = 0) -> None:
+        """Attention of the new rows over their sequences' pages: all keys up to a row's own, or the last `window` and the first `sinks`; scores capped where cap > 0."""
+        self._check(self._lib.gptb200_attention_paged(self._ctx, _ptr(out), out_pitch, _ptr(lse), _ptr(q), q_pitch, dtype, heads, pages.struct, rows.struct, scale, cap, window,
+                                                      sinks), "gptb200_attention_paged")
 
     # ---- memory operators (device_malloc / device_free / device_memset / device_memcpy_*)
     def device_malloc(self, nbytes: int) -> int:

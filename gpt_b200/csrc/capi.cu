@@ -1359,6 +1359,7 @@ int gptb200_ctx_synchronize(gptb200_ctx *ctx)
         cudaMemset(ctx->d_status, 0, sizeof(int));
         // a kernel that gave up may have left tickets half counted: they must be zero between launches
         cudaMemset(ctx->d_pair_flags + size_t(ctx->num_sms) * 8 + 2, 0, (kSkinnyMaxTickets + kDbiasTickets) * sizeof(unsigned int));
+        if (st == DEV_BAD_PAGES) return fail(ctx, GPTB200_ERR_INVALID_ARG, "device status %d: a page table, a length or a row start of a paged cache is out of range", st);
         return fail(ctx, GPTB200_ERR_DEVICE_TIMEOUT, "device status %d: a bounded wait inside a kernel ran out", st);
     }
     return GPTB200_OK;

@@ -1,0 +1,154 @@
+// Entry points of the paged cache of keys and values (include/gptb200.h: gptb200_kv_pages_*, gptb200_attention_paged): checks, choice of kernel, launches.
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+#include "ctx_internal.h"
+#include "kv_pages.cuh"
+
+using namespace gptb200;
+
+namespace {
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// The device that is current at the call stays so.
+struct OnDevice {
+    int before = -1;
+    bool changed = false;
+    cudaError_t enter(int device)
+    {
+        cudaError_t e = cudaGetDevice(&before);
+        if (e == cudaSuccess && before != device) {
+            e = cudaSetDevice(device);
+            changed = e == cudaSuccess;
+        }
+        return e;
+    }
+    ~OnDevice()
+    {
+        if (changed) cudaSetDevice(before);
+    }
+};
+
+int check_pages(gptb200_ctx *ctx, const gptb200_kv_pages *p, const gptb200_kv_rows *b, kvp::Pages *pages, kvp::Batch *batch)
+{
+    if (!p || !b) return fail(ctx, GPTB200_ERR_INVALID_ARG, "no pages or no rows given");
+    if (p->kind < GPTB200_KV_BF16 || p->kind > GPTB200_KV_E4M3) return fail(ctx, GPTB200_ERR_INVALID_ARG, "kind %d of pages is unknown", p->kind);
+    if (p->num_pages < 0 || p->kv_heads <= 0 || p->dim < 8 || p->dim > 128 || p->dim % 8 || p->page_tokens < 8 || p->page_tokens > 4096 || (p->page_tokens & (p->page_tokens - 1)))
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "pages: %d of %d tokens (a power of two from 8 to 4096), %d heads of %d (a multiple of 8, at most 128)", p->num_pages, p->page_tokens, p->kv_heads,
+                    p->dim);
+    if (b->sequences < 0 || b->rows < 0 || b->max_new < 0 || b->table_pitch < 0)
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "rows: %d sequences, %d rows, %d new at most, %d pages each", b->sequences, b->rows, b->max_new, b->table_pitch);
+    if (b->sequences == INT_MAX) return fail(ctx, GPTB200_ERR_TOO_LARGE, "too many sequences");
+    if (b->sequences > 0 && b->rows > 0) {
+        if (!p->data || !aligned16(p->data) || (p->kind == GPTB200_KV_E4M3 && (!p->scales || !aligned16(p->scales))))
+            return fail(ctx, GPTB200_ERR_INVALID_ARG, "pages: no memory, or not aligned to 16 bytes");
+        if (!b->row_starts || !b->lengths || (!b->page_table && b->table_pitch > 0)) return fail(ctx, GPTB200_ERR_INVALID_ARG, "rows: no starts, lengths or page table");
+    }
+    int shift = 0;
+    while ((1 << shift) < p->page_tokens) ++shift;
+    *pages = {p->data, p->kind == GPTB200_KV_E4M3 ? p->scales : nullptr, p->num_pages, shift, p->kv_heads, p->dim};
+    const long long capacity = std::min<long long>(static_cast<long long>(b->table_pitch) << shift, 1 << 30);
+    *batch = {b->row_starts, b->lengths, b->page_table, b->sequences, b->table_pitch, b->rows, static_cast<int>(capacity), ctx->d_status};
+    return GPTB200_OK;
+}
+
+// rows of `width` elements with a pitch: 16-byte pieces everywhere
+int check_rows(gptb200_ctx *ctx, const char *what, const void *p, long long pitch, long long width, int dtype)
+{
+    const int per16 = dtype == GPTB200_DTYPE_F32 ? 4 : 8;
+    if (!p || !aligned16(p) || pitch < width || pitch % per16)
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "%s: no memory, not aligned to 16 bytes, or a pitch of %lld for rows of %lld (a multiple of %d)", what, pitch, width, per16);
+    return GPTB200_OK;
+}
+
+template <bool WRITE>
+int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_pitch, int dtype, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows)
+{
+    if (!ctx) return GPTB200_ERR_INVALID_ARG;
+    if (dtype != GPTB200_DTYPE_BF16 && dtype != GPTB200_DTYPE_F32) return fail(ctx, GPTB200_ERR_INVALID_ARG, "dtype %d is unknown", dtype);
+    kvp::RowsArgs a{};
+    int rc = check_pages(ctx, pages, rows, &a.pages, &a.batch);
+    if (rc != GPTB200_OK) return rc;
+    if (rows->sequences == 0 || rows->rows == 0) return GPTB200_OK;
+    const long long width = 1LL * pages->kv_heads * pages->dim;
+    if ((rc = check_rows(ctx, "keys", k, k_pitch, width, dtype)) != GPTB200_OK || (rc = check_rows(ctx, "values", v, v_pitch, width, dtype)) != GPTB200_OK) return rc;
+    if (width > INT_MAX / 64) return fail(ctx, GPTB200_ERR_TOO_LARGE, "rows of %lld elements", width);
+    OnDevice device;
+    CUDA_TRY(ctx, device.enter(ctx->device));
+    a.k = k; a.v = v; a.k_pitch = k_pitch; a.v_pitch = v_pitch;
+    while ((1 << a.lanes_log2) < pages->dim / 8) ++a.lanes_log2;
+    // about four pieces per thread while that fills the GPU, one row per block at least
+    const int per_row = 2 * pages->kv_heads << a.lanes_log2;
+    const int most = std::min(kvp::kRowMax, std::max(1, 4 * kvp::kRowThreads / per_row));
+    a.rows_per_block = std::max(1, std::min(most, rows->rows / (2 * ctx->num_sms)));
+    const int blocks = (rows->rows + a.rows_per_block - 1) / a.rows_per_block;
+    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(blocks), dim3(kvp::kRowThreads), 0, a); };
+    cudaError_t e;
+    if (dtype == GPTB200_DTYPE_F32)
+        e = pages->kind == GPTB200_KV_E4M3 ? launch(kvp::kv_rows_kernel<float, kvp::KIND_E4M3, WRITE>)
+            : pages->kind == GPTB200_KV_F32 ? launch(kvp::kv_rows_kernel<float, kvp::KIND_F32, WRITE>)
+                                            : launch(kvp::kv_rows_kernel<float, kvp::KIND_BF16, WRITE>);
+    else
+        e = pages->kind == GPTB200_KV_E4M3 ? launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_E4M3, WRITE>)
+            : pages->kind == GPTB200_KV_F32 ? launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_F32, WRITE>)
+                                            : launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_BF16, WRITE>);
+    CUDA_TRY(ctx, e);
+    ctx->launches++;
+    return GPTB200_OK;
+}
+
+template <typename T>
+int attention_rows(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
+{
+    const long long warps = 1LL * a.batch.rows * a.heads, blocks = (warps + kvp::kRowWarps - 1) / kvp::kRowWarps;
+    if (blocks > INT_MAX) return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %d heads", a.batch.rows, a.heads);
+    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(static_cast<unsigned>(blocks)), dim3(kvp::kRowWarps * 32), 0, a); };
+    CUDA_TRY(ctx, kind == GPTB200_KV_E4M3 ? launch(kvp::attention_rows_kernel<T, kvp::KIND_E4M3>)
+                  : kind == GPTB200_KV_F32 ? launch(kvp::attention_rows_kernel<T, kvp::KIND_F32>)
+                                           : launch(kvp::attention_rows_kernel<T, kvp::KIND_BF16>));
+    ctx->launches++;
+    return GPTB200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int gptb200_kv_pages_write(gptb200_ctx *ctx, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, const void *k, long long k_pitch, const void *v, long long v_pitch, int dtype)
+{
+    return run_rows<true>(ctx, const_cast<void *>(k), k_pitch, const_cast<void *>(v), v_pitch, dtype, pages, rows);
+}
+
+int gptb200_kv_pages_read(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_pitch, int dtype, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows)
+{
+    return run_rows<false>(ctx, k, k_pitch, v, v_pitch, dtype, pages, rows);
+}
+
+int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, float *lse, const void *q, long long q_pitch, int dtype, int heads, const gptb200_kv_pages *pages,
+                            const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks)
+{
+    if (!ctx) return GPTB200_ERR_INVALID_ARG;
+    if (dtype != GPTB200_DTYPE_BF16 && dtype != GPTB200_DTYPE_F32) return fail(ctx, GPTB200_ERR_INVALID_ARG, "dtype %d is unknown", dtype);
+    kvp::Attention a{};
+    int rc = check_pages(ctx, pages, rows, &a.pages, &a.batch);
+    if (rc != GPTB200_OK) return rc;
+    if (heads <= 0 || heads % pages->kv_heads) return fail(ctx, GPTB200_ERR_INVALID_ARG, "%d heads are not a multiple of the cache's %d", heads, pages->kv_heads);
+    if (!(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap) || window < 0 || sinks < 0)
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "scale %g, cap %g, window %d, first tokens %d", scale, cap, window, sinks);
+    if (rows->sequences == 0 || rows->rows == 0) return GPTB200_OK;
+    const long long width = 1LL * heads * pages->dim;
+    if ((rc = check_rows(ctx, "q", q, q_pitch, width, dtype)) != GPTB200_OK || (rc = check_rows(ctx, "out", out, out_pitch, width, dtype)) != GPTB200_OK) return rc;
+    if (width > INT_MAX / 64 || 1LL * rows->rows * heads > INT_MAX - 256) return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %lld elements", rows->rows, width);
+    OnDevice device;
+    CUDA_TRY(ctx, device.enter(ctx->device));
+    a.q = q; a.out = out; a.lse = lse; a.q_pitch = q_pitch; a.out_pitch = out_pitch;
+    a.heads = heads; a.share = heads / pages->kv_heads;
+    a.scale = scale; a.cap = cap;
+    a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
+    a.sinks = a.window ? sinks : 0;
+    return dtype == GPTB200_DTYPE_F32 ? attention_rows<float>(ctx, a, pages->kind) : attention_rows<__nv_bfloat16>(ctx, a, pages->kind);
+}
+
+}  // extern "C"

@@ -1,0 +1,514 @@
+// A cache of keys and values in pages: what its operators share, rows into pages and back, and attention of one row at a time.
+//
+// Pool of a layer: [page][keys, values][key / value head][token of the page][dimension], so that a page's tokens of one head lie one behind the other
+// (attention reads them as one run).  A sequence's pages are in its row of a table of page numbers.  Elements are bf16, fp32, or e4m3 codes with one
+// power of two per token and head (exponent + 127, a byte, [page][keys, values][head][token]).
+//
+// Why a power of two: e4m3 has the same relative precision over fourteen powers of two, so a finer scale buys nothing, and with this one every
+// division, product and stored value is exact in fp32 and in bf16: a code read back is one value, whoever reads it.  One byte instead of four per head
+// and token is 3 % of a cache of heads of 64.
+#pragma once
+
+#include <cfloat>
+#include <cuda_bf16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "gemm_sm100.cuh"
+
+namespace gptb200 {
+namespace kvp {
+
+enum Kind : int { KIND_BF16 = GPTB200_KV_BF16, KIND_F32 = GPTB200_KV_F32, KIND_E4M3 = GPTB200_KV_E4M3 };
+
+// The smallest power of two whose 448 multiples reach a row's largest value lies in this range; beyond it codes saturate or vanish.  Every code times
+// every such power is zero or a normal number of fp32 and of bf16.
+constexpr int kMinExponent = -117, kMaxExponent = 119;
+
+struct Pages {
+    void *data;
+    uint8_t *scales;   // e4m3 only
+    int num_pages, page_shift, kv_heads, dim;
+
+    // element (page, which, head, token, 0), in elements; without the last factor the place in `scales`
+    __device__ __forceinline__ long long place(int page, int which, int head, int token) const
+    {
+        return ((((static_cast<long long>(page) * 2 + which) * kv_heads + head) << page_shift) + token);
+    }
+};
+
+struct Batch {
+    const int *row_starts, *lengths, *table;
+    int sequences, table_pitch, rows;
+    int capacity;      // tokens that a row of the table can hold, at most 2^30
+    int *status;
+};
+
+// A sequence's new rows: row0 .. row0 + count - 1 at positions pos0, pos0 + 1, ...; positions below zero hold nothing and see nothing.
+struct Sequence {
+    int row0, count, pos0;
+};
+
+__host__ __device__ inline void report_bad(int *status)
+{
+#ifdef __CUDA_ARCH__
+    atomicCAS(status, 0, DEV_BAD_PAGES);
+#else
+    if (*status == 0) *status = DEV_BAD_PAGES;
+#endif
+}
+
+__host__ __device__ inline int smaller(int a, int b) { return a < b ? a : b; }
+__host__ __device__ inline int larger(int a, int b) { return a > b ? a : b; }
+
+// Whatever the three arrays hold, the rows lie inside the tensors and the positions inside the table.
+__host__ __device__ inline Sequence sequence_of(const Batch &b, int s)
+{
+    const int first = b.row_starts[s], end = b.row_starts[s + 1], length = b.lengths[s];
+    Sequence q;
+    q.row0 = smaller(larger(first, 0), b.rows);
+    q.count = smaller(larger(end, q.row0), b.rows) - q.row0;
+    const int n = smaller(larger(length, 0), b.capacity);
+    q.pos0 = n - q.count;
+    if (q.row0 != first || q.row0 + q.count != end || n != length) report_bad(b.status);
+    return q;
+}
+
+// Page of a sequence's token at a position within [0, capacity); -1 (and a report) when the table holds no page's number.
+__host__ __device__ inline int page_of(const Batch &b, const Pages &p, int s, int position)
+{
+    const int page = b.table[static_cast<long long>(s) * b.table_pitch + (position >> p.page_shift)];
+    if (page >= 0 && page < p.num_pages) return page;
+    report_bad(b.status);
+    return -1;
+}
+
+// The sequence that a row belongs to, by a whole warp (32 starts compared at once), or -1: a row behind the last sequence.
+__device__ __forceinline__ int sequence_of_row(const Batch &b, int row, int lane)
+{
+    int low = 0, high = b.sequences;   // the last s in [low, high) with row_starts[s] <= row
+    while (high - low > 1) {
+        const int step = (high - low + 31) / 32, at = low + lane * step;
+        const unsigned mask = __ballot_sync(0xffffffffu, at < high && b.row_starts[at] <= row);
+        const int last = mask ? 31 - __clz(mask) : 0;
+        high = min(high, low + (last + 1) * step);
+        low += last * step;
+    }
+    return b.row_starts[low] <= row && row < b.row_starts[low + 1] ? low : -1;
+}
+
+// ---- eight elements of one row
+
+__device__ __forceinline__ void load8(float (&v)[8], const float *src)
+{
+    const float4 a = *reinterpret_cast<const float4 *>(src), b = *reinterpret_cast<const float4 *>(src + 4);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+__device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ void load8(float (&v)[8], const __nv_bfloat16 *src)
+{
+    const uint4 w = *reinterpret_cast<const uint4 *>(src);
+    const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = bf16_low(x[i]);
+        v[2 * i + 1] = bf16_high(x[i]);
+    }
+}
+__device__ __forceinline__ void store8(float *dst, const float (&v)[8])
+{
+    *reinterpret_cast<float4 *>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    *reinterpret_cast<float4 *>(dst + 4) = make_float4(v[4], v[5], v[6], v[7]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *dst, const float (&v)[8])
+{
+    *reinterpret_cast<uint4 *>(dst) = make_uint4(ptx::pack_bf16x2(v[0], v[1]), ptx::pack_bf16x2(v[2], v[3]), ptx::pack_bf16x2(v[4], v[5]), ptx::pack_bf16x2(v[6], v[7]));
+}
+
+// Two codes (the low sixteen bits) as fp32 values, exactly.
+__device__ __forceinline__ float2 codes2(uint32_t pair)
+{
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(pair), __NV_E4M3);
+    return __half22float2(__half2(h));
+}
+// Rounded to nearest even, beyond 448 the largest code; neither infinities nor NaN come here
+__device__ __forceinline__ uint32_t to_codes2(float a, float b)
+{
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
+__device__ __forceinline__ float scale_of(uint32_t stored) { return __uint_as_float(stored << 23); }
+
+__device__ __forceinline__ void load8_codes(float (&v)[8], const uint8_t *src, float scale)
+{
+    const uint2 w = *reinterpret_cast<const uint2 *>(src);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 c = codes2((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
+        v[2 * i] = c.x * scale;
+        v[2 * i + 1] = c.y * scale;
+    }
+}
+
+// The smallest e with most <= 448 * 2^e, from most's exponent and mantissa (448 = 1.75 * 2^8).
+__device__ __forceinline__ int exponent_for(float most)
+{
+    const uint32_t bits = __float_as_uint(most);
+    const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u);
+    return min(max(e, kMinExponent), kMaxExponent);
+}
+
+// Rows of keys and values <-> pages.  A piece of eight elements per lane: as many lanes as a head has pieces (a power of two of them, so that the row's
+// largest value is a few shuffles) take one (row, keys or values, head) at a time.  Bound by DRAM: nothing is read or written twice.
+constexpr int kRowThreads = 256;
+constexpr int kRowMax = 32;   // rows per block, at most
+
+struct RowsArgs {
+    Pages pages;
+    Batch batch;
+    void *k, *v;
+    long long k_pitch, v_pitch;
+    int lanes_log2;      // lanes per head
+    int rows_per_block;
+};
+
+// WRITE: rows of T into pages of KIND, else the other way.
+template <typename T, int KIND, bool WRITE>
+__global__ void __launch_bounds__(kRowThreads)
+kv_rows_kernel(const RowsArgs a)
+{
+    __shared__ int where[kRowMax][2];   // page (-1: none) and token within it
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int first = blockIdx.x * a.rows_per_block, rows = min(a.rows_per_block, a.batch.rows - first);
+    for (int r = warp; r < rows; r += kRowThreads / 32) {
+        const int s = sequence_of_row(a.batch, first + r, lane);
+        if (lane == 0) {
+            int page = -1, token = 0;
+            if (s >= 0) {
+                const Sequence q = sequence_of(a.batch, s);
+                const int nth = first + r - q.row0, position = q.pos0 + nth;
+                if (nth >= 0 && nth < q.count && position >= 0) {
+                    page = page_of(a.batch, a.pages, s, position);
+                    token = position & ((1 << a.pages.page_shift) - 1);
+                }
+            }
+            where[r][0] = page;
+            where[r][1] = token;
+        }
+    }
+    __syncthreads();
+    const int pieces = a.pages.dim / 8, per = 1 << a.lanes_log2, piece = threadIdx.x & (per - 1), heads = a.pages.kv_heads;
+    const int units = rows * 2 * heads, stride = kRowThreads >> a.lanes_log2, rounds = (units + stride - 1) / stride;
+    const bool active = piece < pieces;
+#pragma unroll 4
+    for (int round = 0; round < rounds; ++round) {
+        const int u = round * stride + (threadIdx.x >> a.lanes_log2);
+        const int r = u / (2 * heads), which = u / heads % 2, h = u % heads;
+        const bool in = u < units && active;
+        const int page = in ? where[r][0] : -1;
+        const bool on = page >= 0;
+        T *row = nullptr;
+        long long at = 0;
+        if (on) {
+            row = static_cast<T *>(which ? a.v : a.k) + static_cast<long long>(first + r) * (which ? a.v_pitch : a.k_pitch) + h * a.pages.dim + piece * 8;
+            at = a.pages.place(page, which, h, where[r][1]);
+        }
+        float v[8] = {};
+        if constexpr (WRITE) {
+            if (on) load8(v, row);
+            if constexpr (KIND == KIND_E4M3) {
+                float most = 0.0f;
+                uint32_t bad = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool finite = fabsf(v[i]) <= FLT_MAX;
+                    bad |= static_cast<uint32_t>(!finite) << i;
+                    if (!finite) v[i] = 0.0f;
+                    most = fmaxf(most, fabsf(v[i]));
+                }
+                for (int o = per >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int e = exponent_for(most);
+                const float by = power_of_two(-e);
+                uint32_t c[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    c[i] = to_codes2(v[2 * i] * by, v[2 * i + 1] * by);
+                    // the format has no infinity: both kinds become its NaN
+                    if (bad >> (2 * i) & 1) c[i] = (c[i] & 0xff00u) | 0x7fu;
+                    if (bad >> (2 * i + 1) & 1) c[i] = (c[i] & 0x00ffu) | 0x7f00u;
+                }
+                if (on) {
+                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.pages.data) + at * a.pages.dim + piece * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
+                    if (piece == 0) a.pages.scales[at] = static_cast<uint8_t>(e + 127);
+                }
+            } else if constexpr (KIND == KIND_BF16) {
+                if (on) store8(static_cast<__nv_bfloat16 *>(a.pages.data) + at * a.pages.dim + piece * 8, v);
+            } else {
+                if (on) store8(static_cast<float *>(a.pages.data) + at * a.pages.dim + piece * 8, v);
+            }
+        } else if (on) {
+            if constexpr (KIND == KIND_E4M3)
+                load8_codes(v, static_cast<const uint8_t *>(a.pages.data) + at * a.pages.dim + piece * 8, scale_of(a.pages.scales[at]));
+            else if constexpr (KIND == KIND_BF16)
+                load8(v, static_cast<const __nv_bfloat16 *>(a.pages.data) + at * a.pages.dim + piece * 8);
+            else
+                load8(v, static_cast<const float *>(a.pages.data) + at * a.pages.dim + piece * 8);
+            store8(row, v);
+        }
+    }
+}
+
+// ---- attention
+
+struct Attention {
+    Pages pages;
+    Batch batch;
+    const void *q;
+    void *out;
+    float *lse;                // [rows][heads] or null
+    long long q_pitch, out_pitch;
+    int heads, share;          // share: query heads per key / value head
+    float scale, cap;          // cap 0: none
+    int window, sinks;         // window 0: all earlier tokens
+};
+
+__host__ __device__ inline bool visible(const Attention &a, int key, int position)
+{
+    return key <= position && (a.window == 0 || key > position - a.window || key < a.sinks);
+}
+
+// ---- the line of work that the tiled kernels share
+//
+// A tile is a number of packed query rows of one sequence and key / value head: row i of the tile is head i % share of token i / share, so that a group's
+// query heads meet keys and values once.  A tile's work is the blocks of keys that any of its rows sees; all tiles' blocks form one line (sequence, key / value
+// head, tile, block), which is cut into equal ranges, one per block of the grid: whatever the lengths, all blocks do the same work.  A range may begin and
+// end inside a tile; such parts go to scratch as (maximum, sum, weighted values), and the block that arrives last at a tile adds them up in the order of
+// the line, so that results do not depend on who that is.
+
+struct KeyBlocks {
+    int first_ones;   // blocks 0 .. first_ones - 1 (the first tokens that stay visible) ...
+    int from;         // ... then from, from + 1, ...
+    int count;        // in all, at least 1: a tile that sees nothing has its output to write
+};
+
+// Blocks of `keys` keys for rows at positions p0 .. p1.
+__host__ __device__ inline KeyBlocks key_blocks(int p0, int p1, int window, int sinks, int keys)
+{
+    if (p1 < 0) return {0, 0, 1};
+    const int from = window > 0 ? larger(0, p0 - window + 1) / keys : 0;
+    const int ones = window > 0 ? smaller((smaller(sinks, p1 + 1) + keys - 1) / keys, from) : 0;
+    return {ones, from, ones + p1 / keys - from + 1};
+}
+__host__ __device__ inline int block_key(const KeyBlocks &b, int i, int keys) { return (i < b.first_ones ? i : b.from + i - b.first_ones) * keys; }
+
+// Tile t of a sequence's rows of one key / value head.
+__host__ __device__ inline KeyBlocks tile_blocks(const Attention &a, const Sequence &q, int t, int tile_rows, int keys)
+{
+    const int first = t * tile_rows / a.share, last = smaller((t + 1) * tile_rows, q.count * a.share) - 1;
+    return key_blocks(q.pos0 + first, q.pos0 + last / a.share, a.window, a.sinks, keys);
+}
+__host__ __device__ inline int tiles_of(const Attention &a, const Sequence &q, int tile_rows) { return (q.count * a.share + tile_rows - 1) / tile_rows; }
+__host__ __device__ inline long long blocks_of(const Attention &a, const Sequence &q, int tile_rows, int keys)
+{
+    long long n = 0;
+    const int tiles = tiles_of(a, q, tile_rows);
+    for (int t = 0; t < tiles; ++t) n += tile_blocks(a, q, t, tile_rows, keys).count;
+    return n;
+}
+
+// Where a block of the grid stands on the line.
+struct Place {
+    Sequence q;
+    KeyBlocks blocks;
+    int s, g, tile, tiles;
+    int off;              // block within the tile
+};
+
+// Next tile that has rows; false behind the last one.
+__host__ __device__ inline bool next_tile(const Attention &a, Place &p, int tile_rows, int keys)
+{
+    p.off = 0;
+    if (++p.tile >= p.tiles) {
+        p.tile = 0;
+        if (++p.g >= a.pages.kv_heads) {
+            p.g = 0;
+            do {
+                if (++p.s >= a.batch.sequences) return false;
+                p.q = sequence_of(a.batch, p.s);
+            } while (p.q.count == 0);
+            p.tiles = tiles_of(a, p.q, tile_rows);
+        }
+    }
+    p.blocks = tile_blocks(a, p.q, p.tile, tile_rows, keys);
+    return true;
+}
+
+// The place `rest` blocks into sequence s, whose head's tiles have `per_head` blocks in all.
+__host__ __device__ inline Place place_in(const Attention &a, int s, long long rest, long long per_head, int tile_rows, int keys)
+{
+    Place p;
+    p.s = s;
+    p.q = sequence_of(a.batch, s);
+    p.tiles = tiles_of(a, p.q, tile_rows);
+    p.g = static_cast<int>(rest / per_head);
+    rest -= p.g * per_head;
+    for (p.tile = 0;; ++p.tile) {
+        p.blocks = tile_blocks(a, p.q, p.tile, tile_rows, keys);
+        if (rest < p.blocks.count || p.tile + 1 >= p.tiles) break;
+        rest -= p.blocks.count;
+    }
+    p.off = static_cast<int>(rest);
+    return p;
+}
+
+struct Range {
+    long long begin, end;   // this block's blocks of the line
+    long long per;          // of every block of the grid
+};
+
+// The block's range of the line and the place where it begins; an empty range: nothing to do.  All threads of the block take part; a block has THREADS of them.
+template <int THREADS>
+__device__ inline Range range_of_block(const Attention &a, int tile_rows, int keys, int least, Place &place)
+{
+    __shared__ long long sums[THREADS / 32];
+    __shared__ long long found_rest, found_per_head;
+    __shared__ int found_s;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int chunk = (a.batch.sequences + THREADS - 1) / THREADS, s0 = threadIdx.x * chunk, s1 = min(s0 + chunk, a.batch.sequences);
+    long long mine = 0;
+    for (int s = s0; s < s1; ++s) mine += blocks_of(a, sequence_of(a.batch, s), tile_rows, keys) * a.pages.kv_heads;
+    long long upto = mine;   // inclusive prefix
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+    }
+    if (lane == 31) sums[warp] = upto;
+    __syncthreads();
+    long long total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) upto += sums[w];
+        total += sums[w];
+    }
+    Range r;
+    r.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+    r.begin = min(r.per * blockIdx.x, total);
+    r.end = min(r.begin + r.per, total);
+    if (r.begin < r.end) {
+        if (upto - mine <= r.begin && r.begin < upto) {
+            long long rest = r.begin - (upto - mine);
+            for (int s = s0; s < s1; ++s) {
+                const long long per_head = blocks_of(a, sequence_of(a.batch, s), tile_rows, keys), n = per_head * a.pages.kv_heads;
+                if (rest < n) {
+                    found_s = s;
+                    found_rest = rest;
+                    found_per_head = per_head;
+                    break;
+                }
+                rest -= n;
+            }
+        }
+        __syncthreads();
+        place = place_in(a, found_s, found_rest, found_per_head, tile_rows, keys);
+    }
+    return r;
+}
+
+// A part of a tile in scratch: block b of the grid has two, for a tile that began before its range and for one that goes on behind it.
+struct Parts {
+    float *base;              // [grid][2][floats]
+    unsigned int *tickets;    // [grid]: parts arrived of the tile that begins in a block's range and goes on behind it; zero between launches
+    int floats;
+};
+
+template <int KIND>
+__device__ __forceinline__ void load8_held(float (&v)[8], const Pages &p, int page, int which, int head, int token, int piece)
+{
+    const long long at = p.place(page, which, head, token);
+    if constexpr (KIND == KIND_E4M3)
+        load8_codes(v, static_cast<const uint8_t *>(p.data) + at * p.dim + piece * 8, scale_of(p.scales[at]));
+    else if constexpr (KIND == KIND_BF16)
+        load8(v, static_cast<const __nv_bfloat16 *>(p.data) + at * p.dim + piece * 8);
+    else
+        load8(v, static_cast<const float *>(p.data) + at * p.dim + piece * 8);
+}
+
+// One query row of one head, by a whole warp, from the definition: only keys that the row sees are read.  Sixteen lanes hold a head (eight elements each), so that
+// the warp's halves take every second key; a running maximum and sum per half, put together at the end.
+template <typename T, int KIND>
+__device__ void attention_row(const Attention &a, int s, int position, int row, int head, int lane)
+{
+    const int piece = lane & 15, half = lane >> 4, pieces = a.pages.dim / 8, g = head / a.share;
+    const bool active = piece < pieces;
+    float q[8] = {}, acc[8] = {}, m = -INFINITY, l = 0.0f;
+    if (active) load8(q, static_cast<const T *>(a.q) + row * a.q_pitch + head * a.pages.dim + piece * 8);
+    const int from = a.window ? max(0, position - a.window + 1) : 0, sinks = a.window ? min(a.sinks, from) : 0;
+    const int keys = position < 0 ? 0 : sinks + position - from + 1;
+    for (int i = 0; i < keys; i += 2) {   // the halves stay together: shuffles are the whole warp's
+        const int n = i + half, key = n < sinks ? n : from + n - sinks;
+        const bool on = n < keys;
+        float k[8] = {}, v[8] = {};
+        bool there = false;
+        if (on) {
+            const int page = page_of(a.batch, a.pages, s, key), token = key & ((1 << a.pages.page_shift) - 1);
+            there = page >= 0;
+            if (there && active) {
+                load8_held<KIND>(k, a.pages, page, 0, g, token, piece);
+                load8_held<KIND>(v, a.pages, page, 1, g, token, piece);
+            }
+        }
+        float x = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x = fmaf(q[e], k[e], x);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        if (on && there) {
+            x *= a.scale;
+            if (a.cap > 0.0f) x = a.cap * tanhf(x / a.cap);
+            const float now = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - now), w = expf(x - now);
+            m = now;
+            l = fmaf(l, keep, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], keep, w * v[e]);
+        }
+    }
+    const float other = __shfl_xor_sync(0xffffffffu, m, 16), top = fmaxf(m, other), f = m == -INFINITY ? 0.0f : expf(m - top);
+    l *= f;
+    l += __shfl_xor_sync(0xffffffffu, l, 16);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        acc[e] *= f;
+        acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+        acc[e] = keys > 0 ? acc[e] / l : 0.0f;
+    }
+    if (active && half == 0) store8(static_cast<T *>(a.out) + row * a.out_pitch + head * a.pages.dim + piece * 8, acc);
+    if (a.lse && lane == 0) a.lse[static_cast<long long>(row) * a.heads + head] = keys > 0 ? top + logf(l) : -INFINITY;
+}
+
+constexpr int kRowWarps = 4;
+
+// A warp per (row, head).
+template <typename T, int KIND>
+__global__ void __launch_bounds__(kRowWarps * 32)
+attention_rows_kernel(const Attention a)
+{
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const long long w = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    if (w >= static_cast<long long>(a.batch.rows) * a.heads) return;
+    const int row = static_cast<int>(w / a.heads), head = static_cast<int>(w % a.heads);
+    const int s = sequence_of_row(a.batch, row, lane);
+    if (s < 0) return;
+    const Sequence q = sequence_of(a.batch, s);
+    const int nth = row - q.row0;
+    if (nth < 0 || nth >= q.count) return;
+    attention_row<T, KIND>(a, s, q.pos0 + nth, row, head, lane);
+}
+
+}  // namespace kvp
+}  // namespace gptb200

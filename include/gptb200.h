@@ -274,6 +274,47 @@ int gptb200_kv_cache_fill(gptb200_ctx *ctx, float *cache, const float *qkv, int 
 int gptb200_attention_decode(gptb200_ctx *ctx, float *y, float *cache, const float *qkv_new, const int *pos_dev, int batch, int max_len, int d,
                              int heads);
 int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
+/* ---- a cache of keys and values in pages (no counterpart in the reference): sequences of any length share one pool per layer, as the requests that a
+ *      server holds do.  gptb200_kv_pages describes a layer's pool, gptb200_kv_rows the new rows of a call: the same two describe the writing of a step's keys and
+ *      values, the attention of its queries right after it, and the way back.
+ *   pages   data: [num_pages][keys, values][kv_heads][page_tokens][dim], contiguous, bf16, fp32 or e4m3 codes (gptb200_kv_kind), 16-byte aligned; e4m3:
+ *           scales [num_pages][keys, values][kv_heads][page_tokens], one byte each (1 .. 254), 16-byte aligned: a code c stands for c * 2^(byte - 127).
+ *           page_tokens: a power of two from 8 to 4096; dim: a multiple of 8, at most 128.
+ *   rows    the new rows of all sequences, one behind the other: sequence s has rows row_starts[s] .. row_starts[s + 1] - 1 (row_starts: sequences + 1
+ *           numbers) of tensors with `rows` rows; lengths[s] counts its tokens with the new ones, so that its last new row is its token at position
+ *           lengths[s] - 1; page_table[s * table_pitch + i] is the page of tokens i * page_tokens to (i + 1) * page_tokens - 1.  The three arrays are int32 in
+ *           device memory (a captured call reads them when it is replayed).  max_new: the most new rows of a sequence, which chooses the kernel; results
+ *           hold whatever it says.  Rows behind the last sequence's are left as they are; so is a row at a position below zero by a write or a read, while
+ *           attention sees nothing from there and gives zeros (lse: minus infinity).  Entries of the table that no row of the call needs are not read.
+ *           Numbers that do not fit (a page the pool does not have, a length beyond the table, starts out of order or beyond `rows`) touch no foreign
+ *           memory: that part of the results is undefined and the next gptb200_ctx_synchronize returns GPTB200_ERR_INVALID_ARG.
+ *   kv_pages_write   k and v [rows][kv_heads * dim] in dtype (gptb200_dtype), pitches in elements, into their places.  e4m3: the power of two of a token's head is the
+ *           smallest whose 448-fold reaches its largest finite value (between 2^-117 and 2^119: beyond, values saturate or vanish), codes are
+ *           rounded to nearest even; infinities and NaN become NaN.  A place that two rows of a call share holds either.
+ *   kv_pages_read    the same rows' values out of the pages: k and v are written.  With row counts equal to the lengths, whole sequences.
+ *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
+ *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
+ *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they may be the same
+ *           tensor only with the same pitch.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.
+ *   All addresses are 16-byte aligned, pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
+ *   other. */
+typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;
+typedef enum gptb200_kv_kind { GPTB200_KV_BF16 = 0, GPTB200_KV_F32 = 1, GPTB200_KV_E4M3 = 2 } gptb200_kv_kind;
+typedef struct gptb200_kv_pages {
+    void *data;
+    unsigned char *scales;   /* e4m3 only */
+    int kind, num_pages, page_tokens, kv_heads, dim;
+} gptb200_kv_pages;
+typedef struct gptb200_kv_rows {
+    const int *row_starts, *lengths, *page_table;
+    int sequences, table_pitch, rows, max_new;
+} gptb200_kv_rows;
+int gptb200_kv_pages_write(gptb200_ctx *ctx, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, const void *k, long long k_pitch, const void *v,
+                           long long v_pitch, int dtype);
+int gptb200_kv_pages_read(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_pitch, int dtype, const gptb200_kv_pages *pages,
+                          const gptb200_kv_rows *rows);
+int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, float *lse, const void *q, long long q_pitch, int dtype, int heads,
+                            const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks);
 /* Gradient scaling, norm clipping and AdamW over one packed buffer of `segments` tensors in two launches: what the reference
  * does with device_scale_and_clip_grad followed by one device_adamw_step per tensor (src/model/gpt.cpp:644-677,
  * cuda/kernels/gradient_clip.cu:35-59, adamw.cu:71-97).  Tensor t covers elements [segment_ends[t-1], segment_ends[t]);
@@ -391,7 +432,6 @@ int gptb200_model_step_count(gptb200_model *m);
  *                   segments that run side by side; unless set 1024, or down to 256 where the requests of a step would leave the GPU idle: the last bits of a long
  *                   prompt then depend on how many requests share its step and on the longest of them; set, on the longest only), "wkv_segment_tokens" (the same for wkv, a multiple of 16, default 0:
  *                   automatic) and those of gptb200_ctx_set_option */
-typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;
 typedef struct gptb200_decoder gptb200_decoder;
 int gptb200_decoder_check_config(const char *config_json, char *message, size_t capacity);   /* host only */
 int gptb200_decoder_load(gptb200_decoder **out, const char *folder, int dtype, int device, void *cuda_stream, char *message, size_t capacity);
