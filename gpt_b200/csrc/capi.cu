@@ -1151,14 +1151,15 @@ int gptb200_ctx_create(gptb200_ctx **out, int device, void *cuda_stream, int mod
     }
     ctx->encode = reinterpret_cast<EncodeTiledFn>(fn);
     // [pair][CTA][epilogue warp] + launch number, CTA count; then one ticket per column block of the decode kernel; then the
-    // tickets of the bias gradient inside the grad_w GEMM (per tile column, CTA and epilogue warp)
-    const size_t flag_bytes = (size_t(ctx->num_sms) * 8 + 2 + kSkinnyMaxTickets + kDbiasTickets) * sizeof(unsigned int);
+    // tickets of the bias gradient inside the grad_w GEMM (per tile column, CTA and epilogue warp); then those of attention over a paged cache
+    const size_t flag_bytes = (size_t(ctx->num_sms) * 8 + 2 + kSkinnyMaxTickets + kDbiasTickets + kPagedTickets) * sizeof(unsigned int);
     if (cudaMalloc(&ctx->d_status, sizeof(int)) != cudaSuccess || cudaMemset(ctx->d_status, 0, sizeof(int)) != cudaSuccess ||
         cudaMalloc(&ctx->d_pair_flags, flag_bytes) != cudaSuccess || cudaMemset(ctx->d_pair_flags, 0, flag_bytes) != cudaSuccess) {
         if (ctx->d_status) cudaFree(ctx->d_status);
         delete ctx;
         return GPTB200_ERR_CUDA;
     }
+    ctx->d_paged_tickets = ctx->d_pair_flags + size_t(ctx->num_sms) * 8 + 2 + kSkinnyMaxTickets + kDbiasTickets;
     *out = ctx;
     return GPTB200_OK;
 }
@@ -1358,7 +1359,7 @@ int gptb200_ctx_synchronize(gptb200_ctx *ctx)
     if (st != 0) {
         cudaMemset(ctx->d_status, 0, sizeof(int));
         // a kernel that gave up may have left tickets half counted: they must be zero between launches
-        cudaMemset(ctx->d_pair_flags + size_t(ctx->num_sms) * 8 + 2, 0, (kSkinnyMaxTickets + kDbiasTickets) * sizeof(unsigned int));
+        cudaMemset(ctx->d_pair_flags + size_t(ctx->num_sms) * 8 + 2, 0, (kSkinnyMaxTickets + kDbiasTickets + kPagedTickets) * sizeof(unsigned int));
         if (st == DEV_BAD_PAGES) return fail(ctx, GPTB200_ERR_INVALID_ARG, "device status %d: a page table, a length or a row start of a paged cache is out of range", st);
         return fail(ctx, GPTB200_ERR_DEVICE_TIMEOUT, "device status %d: a bounded wait inside a kernel ran out", st);
     }

@@ -80,6 +80,7 @@ struct gptb200_ctx {
     unsigned int *d_pair_flags = nullptr;  // per CTA pair, CTA and epilogue warp: number of the launch whose partial tile is complete;
                                            // then the number of completed launches and a CTA counter (both kept by the kernel);
                                            // then the decode kernel's tickets (one per column block, zero between launches)
+    unsigned int *d_paged_tickets = nullptr;   // a part of them: attention over a paged cache, one per block of its grids, zero between launches
     float *ws = nullptr;  // scratch: split-K partial tiles, partial rows of column reductions
     size_t ws_bytes = 0;
     bool ws_captured = false;   // a graph that was captured holds its address ...
@@ -106,6 +107,7 @@ struct gptb200_ctx {
 namespace gptb200 {
 
 constexpr size_t kTmapCacheMax = 4096;
+constexpr int kPagedTickets = 1024;   // most blocks of a grid that shares tiles of paged attention
 
 inline int fail(gptb200_ctx *ctx, int code, const char *fmt, ...)
 {

@@ -4,7 +4,7 @@
 #include <cmath>
 
 #include "ctx_internal.h"
-#include "kv_pages.cuh"
+#include "paged_tokens.cuh"
 
 using namespace gptb200;
 
@@ -112,6 +112,43 @@ int attention_rows(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
     return GPTB200_OK;
 }
 
+// A kernel that cuts the line of work into equal ranges: `per_sm` blocks on every SM, a part of a tile in scratch for either end of a range.
+template <typename Args>
+int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, int smem, int per_sm, int part_floats)
+{
+    const void *key = reinterpret_cast<const void *>(kernel);
+    if (!ctx->configured.count(key)) {
+        CUDA_TRY(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        ctx->configured.insert(key);
+    }
+    const int sms = ctx->max_sms > 0 ? std::min(ctx->max_sms, ctx->num_sms) : ctx->num_sms;
+    const int blocks = std::min(sms * per_sm, kPagedTickets);
+    const int rc = ensure_workspace(ctx, size_t(2) * blocks * part_floats * sizeof(float));
+    if (rc != GPTB200_OK) return rc;
+    args.parts = {ctx->ws, ctx->d_paged_tickets, part_floats};
+    CUDA_TRY(ctx, launch_chained(ctx, kernel, dim3(blocks), dim3(threads), smem, args));
+    ctx->launches++;
+    return GPTB200_OK;
+}
+
+template <int D16, bool CODES>
+int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args)
+{
+    return run_line(ctx, kvp::paged_tokens_kernel<D16, CODES>, args, kvp::kTokensThreads, kvp::TokensShape<D16, CODES>::kSmem, CODES ? 3 : 2, kvp::kTokensPart);
+}
+
+int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
+{
+    kvp::TokensArgs args{a, {}, 4};
+    const bool codes = kind == GPTB200_KV_E4M3;
+    switch ((a.pages.dim + 31) / 32) {
+        case 1: return codes ? run_tokens<2, true>(ctx, args) : run_tokens<2, false>(ctx, args);
+        case 2: return codes ? run_tokens<4, true>(ctx, args) : run_tokens<4, false>(ctx, args);
+        case 3: return codes ? run_tokens<6, true>(ctx, args) : run_tokens<6, false>(ctx, args);
+        default: return codes ? run_tokens<8, true>(ctx, args) : run_tokens<8, false>(ctx, args);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -148,6 +185,7 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     a.scale = scale; a.cap = cap;
     a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
     a.sinks = a.window ? sinks : 0;
+    if (dtype == GPTB200_DTYPE_BF16 && pages->kind != GPTB200_KV_F32) return attention_tokens(ctx, a, pages->kind);
     return dtype == GPTB200_DTYPE_F32 ? attention_rows<float>(ctx, a, pages->kind) : attention_rows<__nv_bfloat16>(ctx, a, pages->kind);
 }
 

@@ -469,14 +469,14 @@ __device__ void attention_row(const Attention &a, int s, int position, int row, 
         if (on && there) {
             x *= a.scale;
             if (a.cap > 0.0f) x = a.cap * tanhf(x / a.cap);
-            const float now = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - now), w = expf(x - now);
+            const float now = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - now), w = x == -INFINITY ? 0.0f : expf(x - now);
             m = now;
             l = fmaf(l, keep, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], keep, w * v[e]);
         }
     }
-    const float other = __shfl_xor_sync(0xffffffffu, m, 16), top = fmaxf(m, other), f = m == -INFINITY ? 0.0f : expf(m - top);
+    const float other = __shfl_xor_sync(0xffffffffu, m, 16), top = fmaxf(m, other), f = m == -INFINITY ? 1.0f : expf(m - top);   // a half that saw nothing holds zeros
     l *= f;
     l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll

@@ -1,0 +1,514 @@
+// Attention of a few new rows per sequence (single tokens above all) over a paged cache, in bf16.
+//
+// A tile is sixteen packed query rows of one sequence and key / value head (kv_pages.cuh: the line of work).  Each warp of a block takes sixteen keys of every
+// block of 64 in turn: asynchronous copies bring them, and their values, into a ring of its own; scores and weighted values are mma.sync products of 16 x 8 x 16, the
+// weights going from one to the other in registers; maximum and sum run along in fp32.  The warps meet once per tile.
+//
+// Bound by the cache's bytes: 16 query rows against 4 * dim bytes of a bf16 key and value are 16 flops a byte, a tenth of what mma.sync sustains, so the legacy
+// instructions do here; what counts is bytes in flight, hence the rings (50 to 100 KB per block, two or three blocks per SM) and no barrier inside the loop.
+//
+// Codes (e4m3) go through registers once, to fp16, which holds every code exactly; their powers of two never touch the products:
+//   scores   q of a row is divided by a power of two (its largest value's), so that fp16 holds it as bf16 did; the row's and the key's powers multiply the score
+//   values   weight j enters the second product as 2^(x_j + e_j - R), x_j the score in base 2, e_j the value's exponent, R their running maximum: at most 1, rounded
+//            to eleven bits where bf16 weights have eight.  The sum of weights runs against the scores' own maximum, in fp32.
+// The products' inner dimension may be permuted on both sides, and so may the output's columns: a lane takes neighbouring codes with one load, pairs two keys'
+// codes with a byte permutation, and no transposition is needed.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include "kv_pages.cuh"
+
+namespace gptb200 {
+namespace kvp {
+
+constexpr int kTokensWarps = 4, kTokensThreads = kTokensWarps * 32;
+constexpr int kTokensRows = 16, kTokensKeys = 64;
+constexpr int kTokensPart = kTokensRows * 128 + 2 * kTokensRows;   // floats of a part in scratch
+
+// D16: dimensions in steps of 16 (zeros behind the head's own)
+template <int D16, bool CODES>
+struct TokensShape {
+    static constexpr int kDim = 16 * D16;
+    // pitches that spread what the lanes of one load touch over all banks
+    static constexpr int kKeyPitch = CODES ? (D16 == 8 ? 144 : 16 * D16) : 2 * kDim + 16;
+    static constexpr int kValuePitch = CODES ? (D16 == 8 ? 144 : D16 == 6 ? 112 : D16 == 4 ? 80 : 48) : 2 * kDim + 16;
+    static constexpr int kStage = 16 * (kKeyPitch + kValuePitch) + (CODES ? 32 : 0);
+    static constexpr int kStages = 3;
+    static constexpr int kQPitch = 2 * kDim + 16;
+    static constexpr int kRing = kTokensWarps * kStages * kStage;
+    static constexpr int kMergePitch = kDim + 4;
+    static constexpr int kMerge = kTokensWarps * kTokensRows * kMergePitch * 4;
+    static constexpr int kSmem = kTokensRows * kQPitch + (kRing > kMerge ? kRing : kMerge);
+};
+
+namespace tok {
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr)
+{
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <bool HALF>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1)
+{
+    if constexpr (HALF)
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                     : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x)
+{
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Factor that brings what stands against maximum m to maximum `top`.  A part that saw nothing holds zeros (or NaN, which stay) and counts as it is.
+__device__ __forceinline__ float share_of(float m, float top) { return m == -INFINITY ? 1.0f : exp2_fast(m - top); }
+// bytes of shared memory, from nothing where `from` is not to be read
+template <int BYTES>
+__device__ __forceinline__ void copy(uint32_t dst, const void *from, bool there)
+{
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(there ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+// two codes as two halves
+__device__ __forceinline__ uint32_t halves(uint32_t pair)
+{
+    uint32_t h;
+    asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(pair));
+    return h;
+}
+__device__ __forceinline__ uint32_t pack_half2(float a, float b)
+{
+    uint32_t h;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
+    return h;
+}
+template <int WORDS>
+__device__ __forceinline__ void lds_words(uint32_t (&v)[WORDS], uint32_t addr)
+{
+    static_assert(WORDS == 1 || WORDS == 2 || WORDS == 3 || WORDS == 4);
+    if constexpr (WORDS == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr));
+    else if constexpr (WORDS == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v[0]), "=r"(v[1]) : "r"(addr));
+    else
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v[i]) : "r"(addr + 4 * i));
+}
+
+}  // namespace tok
+
+struct TokensArgs {
+    Attention a;
+    Parts parts;
+    int least;        // blocks of the line per block of the grid, at least
+};
+
+template <int D16, bool CODES>
+__global__ void __launch_bounds__(kTokensThreads, CODES ? 3 : 2)
+paged_tokens_kernel(const __grid_constant__ TokensArgs args)
+{
+    using namespace tok;
+    using S = TokensShape<D16, CODES>;
+    constexpr int kind = CODES ? KIND_E4M3 : KIND_BF16;
+    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+    extern __shared__ __align__(16) uint8_t tokens_smem[];
+    __shared__ float merge_ml[kTokensWarps][kTokensRows][2], total_ml[kTokensRows][2], row_power[kTokensRows];
+    __shared__ int bad_rows, arrived_last;
+    const Attention &a = args.a;
+    grid_dependency_wait();
+    grid_dependency_launch();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
+    Place place;
+    Range range = range_of_block<kTokensThreads>(a, kTokensRows, kTokensKeys, args.least, place);
+    const uint32_t q_tile = ptx::smem_u32(tokens_smem), ring = q_tile + kTokensRows * S::kQPitch + warp * S::kStages * S::kStage;
+    const int dim = a.pages.dim, pieces = dim / 8;
+    // a head narrower than the padded width: its tail columns stay zero
+    auto clear_tail = [&] {
+        if (dim == S::kDim) return;
+        for (int i = lane; i < S::kStages * S::kStage / 16; i += 32) ptx::sts128(ring + 16 * i, 0u, 0u, 0u, 0u);
+        __syncwarp();
+    };
+
+    for (long long at = range.begin; at < range.end;) {
+        const int n_blocks = static_cast<int>(min(static_cast<long long>(place.blocks.count - place.off), range.end - at));
+        const bool whole = place.off == 0 && n_blocks == place.blocks.count;
+        const int packed0 = place.tile * kTokensRows, rows = min(kTokensRows, place.q.count * a.share - packed0);
+        const int p0 = place.q.pos0 + packed0 / a.share, p1 = place.q.pos0 + (packed0 + rows - 1) / a.share;
+        const int low = a.window ? p0 - a.window + 1 : 0;   // keys below it are visible only among the first ones
+        auto tile_key = [&](int i) { return block_key(place.blocks, place.off + i, kTokensKeys) + warp * 16; };
+        auto wanted = [&](int key) { return key <= p1 && (key >= low || key < a.sinks); };   // by any row of the tile
+
+        // ---- the ring
+        // lanes with an even number look up the page of the tile's first eight keys, the others that of the last eight
+        auto page_for = [&](int i) {
+            if (i >= n_blocks) return -1;
+            const int key = tile_key(i) + 8 * (lane & 1);
+            return key <= p1 && (key + 7 >= low || key < a.sinks) ? page_of(a.batch, a.pages, place.s, key) : -1;
+        };
+        int next_page = page_for(0);
+        auto fetch = [&](int i) {
+            const int stage = i % S::kStages;
+            const uint32_t dst = ring + stage * S::kStage;
+            const int page[2] = {__shfl_sync(0xffffffffu, next_page, 0), __shfl_sync(0xffffffffu, next_page, 1)};
+            next_page = page_for(i + 1);
+            if (i < n_blocks) {
+                const int t = tile_key(i), mask = (1 << a.pages.page_shift) - 1;
+                if constexpr (CODES) {
+                    const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
+                    if (dim % 16 == 0) {
+#pragma unroll
+                        for (int j = 0; j < D16 / 2; ++j) {
+                            const int idx = j * 32 + lane, r = idx / D16, c = idx % D16, key = t + r, pg = page[r >> 3];
+                            const bool on = c * 16 < dim && pg >= 0 && wanted(key);
+#pragma unroll
+                            for (int which = 0; which < 2; ++which) {
+                                const uint8_t *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 16 : data;
+                                const uint32_t to = dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 16;
+                                if (c * 16 < dim) copy<16>(to, src, on);
+                            }
+                        }
+                    } else {
+                        for (int idx = lane; idx < 16 * pieces; idx += 32) {
+                            const int r = idx / pieces, c = idx % pieces, key = t + r, pg = page[r >> 3];
+                            const bool on = pg >= 0 && wanted(key);
+#pragma unroll
+                            for (int which = 0; which < 2; ++which) {
+                                const uint8_t *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 8 : data;
+                                copy<8>(dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 8, src, on);
+                            }
+                        }
+                    }
+                    if (lane < 4) {   // powers of two: eight keys a copy, keys' then values'
+                        const int half = lane & 1, which = lane >> 1, pg = page[half];
+                        const uint8_t *src = pg >= 0 ? a.pages.scales + a.pages.place(pg, which, place.g, (t + 8 * half) & mask) : a.pages.scales;
+                        copy<8>(dst + 16 * (S::kKeyPitch + S::kValuePitch) + 16 * which + 8 * half, src, pg >= 0);
+                    }
+                } else {
+                    const __nv_bfloat16 *data = static_cast<const __nv_bfloat16 *>(a.pages.data);
+#pragma unroll
+                    for (int j = 0; j < D16; ++j) {
+                        const int idx = j * 32 + lane, r = idx / (2 * D16), c = idx % (2 * D16), key = t + r, pg = page[r >> 3];
+                        const bool on = c < pieces && pg >= 0 && wanted(key);
+#pragma unroll
+                        for (int which = 0; which < 2; ++which) {
+                            const __nv_bfloat16 *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 8 : data;
+                            if (c < pieces) copy<16>(dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 16, src, on);
+                        }
+                    }
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        clear_tail();
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) fetch(i);
+
+        // ---- the queries: a row's eight dimensions per lane, sixteen lanes a row
+        for (int r = threadIdx.x >> 4; r < kTokensRows; r += kTokensThreads / 16) {
+            const int c = threadIdx.x & 15;
+            float v[8] = {};
+            if (r < rows && c < pieces) {
+                const int packed = packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
+                load8(v, static_cast<const __nv_bfloat16 *>(a.q) + row * a.q_pitch + head * dim + c * 8);
+            }
+            uint32_t w[4];
+            if constexpr (CODES) {
+                float most = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+                const int e2 = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 100);
+                const float by = power_of_two(-e2);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = pack_half2(v[2 * i] * by, v[2 * i + 1] * by);
+                if (c == 0) row_power[r] = power_of_two(e2);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = ptx::pack_bf16x2(v[2 * i], v[2 * i + 1]);
+            }
+            if (c < 2 * D16) ptx::sts128(q_tile + r * S::kQPitch + c * 16, w[0], w[1], w[2], w[3]);
+        }
+        if (threadIdx.x == 0) bad_rows = 0;
+        __syncthreads();
+        uint32_t qf[D16][4];
+#pragma unroll
+        for (int k = 0; k < D16; ++k) {
+            if constexpr (CODES) {
+                uint32_t u[2], v[2];
+                lds_words<2>(u, q_tile + g8 * S::kQPitch + (t4 * 4 * D16 + 4 * k) * 2);
+                lds_words<2>(v, q_tile + (g8 + 8) * S::kQPitch + (t4 * 4 * D16 + 4 * k) * 2);
+                qf[k][0] = u[0]; qf[k][1] = v[0]; qf[k][2] = u[1]; qf[k][3] = v[1];
+            } else {
+                ldsm4(qf[k], q_tile + (lane & 15) * S::kQPitch + (k * 16 + ((lane >> 4) << 3)) * 2);
+            }
+        }
+        const bool second = rows > 8;   // rows 8 .. 15 are there
+        int pos[2];
+        float to_score[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = g8 + 8 * i;
+            pos[i] = r < rows ? place.q.pos0 + (packed0 + r) / a.share : -1;
+            to_score[i] = a.scale * (CODES ? row_power[r] : 1.0f);
+        }
+
+        float m[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // ref: against which the weighted values stand (codes only)
+        float O[2 * D16][4] = {};
+        for (int it = 0; it < n_blocks; ++it) {
+            fetch(it + S::kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+            __syncwarp();
+            const int t = tile_key(it);
+            const uint32_t kt = ring + it % S::kStages * S::kStage, vt = kt + 16 * S::kKeyPitch, et = vt + 16 * S::kValuePitch;
+            float x[2][4] = {};
+            float value_e[2][2];   // exponents of the values of the lane's keys
+            if constexpr (CODES) {
+                // keys g8 and g8 + 8: the lane's 4 * D16 codes of each
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const uint32_t from = kt + (g8 + 8 * j) * S::kKeyPitch + t4 * 4 * D16;
+                    constexpr int kWords = D16 % 4 == 0 ? 4 : 2;
+#pragma unroll
+                    for (int k = 0; k < D16; k += kWords) {
+                        uint32_t w[kWords];
+                        lds_words<kWords>(w, from + 4 * k);
+#pragma unroll
+                        for (int i = 0; i < kWords; ++i) mma<true>(x[j], qf[k + i], halves(w[i]), halves(w[i] >> 16));
+                    }
+                    uint16_t ke, ve;
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(ke) : "r"(et + 8 * j + 2 * t4));
+                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(ve) : "r"(et + 16 + 8 * j + 2 * t4));
+                    const float k0 = scale_of(ke & 255u), k1 = scale_of(ke >> 8);
+                    x[j][0] *= k0; x[j][1] *= k1; x[j][2] *= k0; x[j][3] *= k1;
+                    value_e[j][0] = static_cast<float>(static_cast<int>(ve & 255u) - 127);
+                    value_e[j][1] = static_cast<float>(static_cast<int>(ve >> 8) - 127);
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < D16; ++k) {
+                    uint32_t f[4];
+                    ldsm4(f, kt + ((lane & 7) + ((lane >> 4) << 3)) * S::kKeyPitch + (k * 16 + (((lane >> 3) & 1) << 3)) * 2);
+                    mma<false>(x[0], qf[k], f[0], f[1]);
+                    mma<false>(x[1], qf[k], f[2], f[3]);
+                }
+            }
+            const bool all_seen = t + 15 <= p0 && (a.window == 0 || t > p1 - a.window || t + 15 < a.sinks) && p0 >= 0;
+            uint32_t weights[4];
+            float turn[2] = {1.0f, 1.0f};
+            float w[2][4] = {};
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (i == 1 && !second) break;
+                float top = -INFINITY, top_ref = -INFINITY;
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float v = x[j][2 * i + e] * to_score[i];
+                        if (a.cap > 0.0f) v = a.cap * tanhf(v / a.cap);
+                        v *= kLog2e;
+                        if (!all_seen && !visible(a, t + 8 * j + 2 * t4 + e, pos[i])) v = -INFINITY;
+                        x[j][2 * i + e] = v;
+                        top = fmaxf(top, v);
+                        if (CODES) top_ref = fmaxf(top_ref, v + value_e[j][e]);
+                    }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float now = fmaxf(m[i], top), use = now == -INFINITY ? 0.0f : now;   // nothing seen yet: every weight is 2^-inf = 0
+                const float f = exp2_fast(m[i] - use);
+                m[i] = now;
+                l[i] *= f;
+                float use_ref = use;
+                if constexpr (CODES) {
+                    top_ref = fmaxf(top_ref, __shfl_xor_sync(0xffffffffu, top_ref, 1));
+                    top_ref = fmaxf(top_ref, __shfl_xor_sync(0xffffffffu, top_ref, 2));
+                    const float now_ref = fmaxf(ref[i], top_ref);
+                    use_ref = now_ref == -INFINITY ? 0.0f : now_ref;
+                    turn[i] = exp2_fast(ref[i] - use_ref);
+                    ref[i] = now_ref;
+                } else {
+                    turn[i] = f;
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float p = exp2_fast(x[j][2 * i + e] - use);
+                        l[i] += p;
+                        w[j][2 * i + e] = CODES ? exp2_fast(x[j][2 * i + e] + value_e[j][e] - use_ref) : p;
+                    }
+            }
+            // weights as the second product's A operand: rows g8 / g8 + 8, keys 2 t4 and 2 t4 + 8
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) weights[2 * j + i] = CODES ? pack_half2(w[j][2 * i], w[j][2 * i + 1]) : ptx::pack_bf16x2(w[j][2 * i], w[j][2 * i + 1]);
+            if (__any_sync(0xffffffffu, turn[0] != 1.0f || turn[1] != 1.0f)) {
+#pragma unroll
+                for (int u = 0; u < 2 * D16; ++u) {
+                    O[u][0] *= turn[0];
+                    O[u][1] *= turn[0];
+                    O[u][2] *= turn[1];
+                    O[u][3] *= turn[1];
+                }
+            }
+            if constexpr (CODES) {
+                // dimensions g8 * 2 D16 + u of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: column g8 of tile u
+                constexpr int kWords = D16 / 2;
+                uint32_t c[4][kWords];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) lds_words<kWords>(c[r], vt + (2 * t4 + (r & 1) + 8 * (r >> 1)) * S::kValuePitch + g8 * 2 * D16);
+#pragma unroll
+                for (int i = 0; i < kWords; ++i) {
+                    const uint32_t lo0 = __byte_perm(c[0][i], c[1][i], 0x5140), lo1 = __byte_perm(c[0][i], c[1][i], 0x7362);
+                    const uint32_t hi0 = __byte_perm(c[2][i], c[3][i], 0x5140), hi1 = __byte_perm(c[2][i], c[3][i], 0x7362);
+                    mma<true>(O[4 * i], weights, halves(lo0), halves(hi0));
+                    mma<true>(O[4 * i + 1], weights, halves(lo0 >> 16), halves(hi0 >> 16));
+                    mma<true>(O[4 * i + 2], weights, halves(lo1), halves(hi1));
+                    mma<true>(O[4 * i + 3], weights, halves(lo1 >> 16), halves(hi1 >> 16));
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 2 * D16; u += 2) {
+                    uint32_t f[4];
+                    ldsm4t(f, vt + (lane & 15) * S::kValuePitch + (u * 8 + ((lane >> 4) << 3)) * 2);
+                    mma<false>(O[u], weights, f[0], f[1]);
+                    mma<false>(O[u + 1], weights, f[2], f[3]);
+                }
+            }
+            __syncwarp();   // this stage may be filled again
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+        // ---- the warps' parts
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (t4 == 0) {
+                merge_ml[warp][g8 + 8 * i][0] = m[i];
+                merge_ml[warp][g8 + 8 * i][1] = l[i];
+            }
+        }
+        __syncthreads();   // every warp is done with its ring: the sums take its place
+        float *merge = reinterpret_cast<float *>(tokens_smem + kTokensRows * S::kQPitch);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int r = g8 + 8 * i;
+            float top = merge_ml[0][r][0];
+#pragma unroll
+            for (int w = 1; w < kTokensWarps; ++w) top = fmaxf(top, merge_ml[w][r][0]);
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kTokensWarps; ++w)
+                sum += merge_ml[w][r][1] * share_of(merge_ml[w][r][0], top);
+            if (warp == 0 && t4 == 0) {
+                total_ml[r][0] = top;
+                total_ml[r][1] = sum;
+            }
+            const float f = share_of(CODES ? ref[i] : m[i], top);
+#pragma unroll
+            for (int u = 0; u < 2 * D16; ++u) {
+                float *to = merge + (warp * kTokensRows + r) * S::kMergePitch;
+                if constexpr (CODES) {
+                    to[(2 * t4) * 2 * D16 + u] = O[u][2 * i] * f;
+                    to[(2 * t4 + 1) * 2 * D16 + u] = O[u][2 * i + 1] * f;
+                } else {
+                    *reinterpret_cast<float2 *>(to + u * 8 + 2 * t4) = make_float2(O[u][2 * i] * f, O[u][2 * i + 1] * f);
+                }
+            }
+        }
+        __syncthreads();
+        auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
+            const int packed = packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
+            const bool sees = place.q.pos0 + packed / a.share >= 0;   // itself at least
+            const float inv = sees ? 1.0f / sum : 0.0f;
+            bool fine = true;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                v[e] *= inv;
+                fine = fine && fabsf(v[e]) <= FLT_MAX;
+            }
+            if (!fine) atomicOr(&bad_rows, 1 << r);
+            store8(static_cast<__nv_bfloat16 *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
+            if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
+        };
+        const long long first = at - place.off, last = first + place.blocks.count - 1;   // the tile's blocks on the line
+        float *part = args.parts.base + (2LL * blockIdx.x + (first >= range.begin)) * args.parts.floats;
+        for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
+            const int r = i / pieces, c = i % pieces;
+            float v[8] = {};
+#pragma unroll
+            for (int w = 0; w < kTokensWarps; ++w) {
+                float u[8];
+                load8(u, merge + (w * kTokensRows + r) * S::kMergePitch + c * 8);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += u[e];
+            }
+            if (whole) {
+                finish(r, c, v, total_ml[r][0], total_ml[r][1]);
+            } else {
+                store8(part + r * dim + c * 8, v);
+                if (c == 0) *reinterpret_cast<float2 *>(part + kTokensRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
+            }
+        }
+        if (!whole) {
+            const int b0 = static_cast<int>(first / range.per), b1 = static_cast<int>(last / range.per);
+            __threadfence();
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const unsigned int before = atomicAdd(args.parts.tickets + b0, 1u);
+                arrived_last = before == static_cast<unsigned int>(b1 - b0);
+                if (arrived_last) args.parts.tickets[b0] = 0u;
+                __threadfence();
+            }
+            __syncthreads();
+            if (arrived_last) {
+                for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
+                    const int r = i / pieces, c = i % pieces;
+                    auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats; };
+                    float top = -INFINITY, sum = 0.0f, v[8] = {};
+                    for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(slot(b) + kTokensRows * 128 + 2 * r));
+#pragma unroll 4
+                    for (int b = b0; b <= b1; ++b) {
+                        const float *from = slot(b);
+                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + kTokensRows * 128 + 2 * r));
+                        const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from + r * dim + c * 8)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + r * dim + c * 8 + 4));
+                        const float f = share_of(ml.x, top);
+                        sum = fmaf(ml.y, f, sum);
+                        v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
+                        v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
+                    }
+                    finish(r, c, v, top, sum);
+                }
+            }
+        }
+        __syncthreads();
+        // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is
+        // formed once more from its own keys alone.
+        for (int rest = bad_rows, n = 0; rest; rest &= rest - 1, ++n) {
+            if (n % kTokensWarps != warp) continue;
+            const int packed = packed0 + __ffs(rest) - 1;
+            attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + packed / a.share, place.q.row0 + packed / a.share, place.g * a.share + packed % a.share, lane);
+        }
+        __syncthreads();   // what the next tile writes again has been read
+        at += n_blocks;
+        if (at < range.end && !next_tile(a, place, kTokensRows, kTokensKeys)) break;
+    }
+}
+
+}  // namespace kvp
+}  // namespace gptb200
