@@ -4,7 +4,7 @@
 #include <cmath>
 
 #include "ctx_internal.h"
-#include "paged_tokens.cuh"
+#include "paged_prompt_sm100.cuh"
 
 using namespace gptb200;
 
@@ -149,6 +149,22 @@ int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
     }
 }
 
+template <int NB, bool CODES>
+int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args)
+{
+    return run_line(ctx, args.a.cap > 0.0f ? kvp::paged_prompt_kernel<NB, CODES, true> : kvp::paged_prompt_kernel<NB, CODES, false>, args, kvp::kPromptThreads,
+                    kvp::PromptShape<NB>::kSmem, 1, kvp::kPromptPart);
+}
+
+int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
+{
+    constexpr float kLog2e = 1.4426950408889634f;
+    kvp::PromptArgs args{a, {}, 2, a.scale * kLog2e, a.cap * kLog2e, a.cap > 0.0f ? a.scale / a.cap : 0.0f};
+    const bool codes = kind == GPTB200_KV_E4M3;
+    if (a.pages.dim <= 64) return codes ? run_prompt<1, true>(ctx, args) : run_prompt<1, false>(ctx, args);
+    return codes ? run_prompt<2, true>(ctx, args) : run_prompt<2, false>(ctx, args);
+}
+
 }  // namespace
 
 extern "C" {
@@ -185,7 +201,8 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     a.scale = scale; a.cap = cap;
     a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
     a.sinks = a.window ? sinks : 0;
-    if (dtype == GPTB200_DTYPE_BF16 && pages->kind != GPTB200_KV_F32) return attention_tokens(ctx, a, pages->kind);
+    if (dtype == GPTB200_DTYPE_BF16 && pages->kind != GPTB200_KV_F32)
+        return 1LL * rows->max_new * a.share > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind);
     return dtype == GPTB200_DTYPE_F32 ? attention_rows<float>(ctx, a, pages->kind) : attention_rows<__nv_bfloat16>(ctx, a, pages->kind);
 }
 

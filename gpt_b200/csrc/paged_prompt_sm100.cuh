@@ -1,0 +1,610 @@
+// Attention of prompts and portions of prompts over a paged cache on the tensor cores, in bf16.
+//
+// A tile is 256 packed query rows of one sequence and key / value head (kv_pages.cuh: the line of work), worked on as two halves of 128; per block of 128 keys
+//   S = Q K^T   tcgen05.mma from shared memory, S in TMEM
+//   softmax     a thread per row: the row's scores in registers, running reference and sum in fp32; weights go back to TMEM over S, rounded to bf16 (eight bits:
+//               the output has no more; the sum is that of the unrounded weights, as the logarithm of the sum needs it)
+//   O += P V    tcgen05.mma with P from TMEM and V from shared memory as stored (MN-major)
+// The halves take turns on the tensor pipe: while one is in softmax the other's products run.  O is scaled only when a row's maximum has grown by more than 2^8
+// since the last time.  The grid is one block per SM, each with an equal range of the line; queries of the next tile are fetched while the last one is stored.
+//
+//   warps 0-1, 2-3   keys, values (named barriers 2 and 3): pages are looked up per key, rows come by asynchronous 16-byte copies into the swizzled layout that the tensor core reads (a
+//                    page is as small as eight tokens; an e4m3 row goes through registers and becomes bf16 there, exactly); all four fetch queries
+//   warp 4           issues the products, one elected lane
+//   warps 8-11       softmax and output of half 0;  warps 12-15: half 1
+// Keys and values that no row of the tile sees are zeros in shared memory, whatever the pages hold there.  Every wait is bounded.
+#pragma once
+
+#include "paged_tokens.cuh"
+
+namespace gptb200 {
+namespace kvp {
+
+constexpr int kPromptThreads = 512, kPromptRows = 256, kPromptKeys = 128;
+constexpr int kPromptBlock = 128 * 128;   // bytes of [128 rows x 64 bf16]
+constexpr int kPromptMaxStages = 3;
+constexpr int kPromptPart = kPromptRows * 128 + 2 * kPromptRows;   // floats of a part in scratch
+
+template <int NB>   // 64-column blocks of a head
+struct PromptShape {
+    static constexpr int kStages = NB == 1 ? 3 : 2;
+    static constexpr int kTile = NB * kPromptBlock;
+    static constexpr int kSmem = (2 + 2 * kStages) * kTile + 1024 + 256;
+};
+
+struct PromptArgs {
+    Attention a;
+    Parts parts;
+    int least;
+    float scale_log2;          // scale * log2(e)
+    float cap_log2, cap_arg;   // cap * log2(e), scale / cap
+};
+
+namespace pro {
+
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate)
+{
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "setp.ne.b32 P, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, P;\n\t}"
+        :
+        : "r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x16(uint32_t taddr, const uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        :
+        : "r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]),
+          "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&v)[16])
+{
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]),
+          "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// All threads of a named barrier learn whether all of them bring true.
+__device__ __forceinline__ bool all_of(int barrier, int threads, bool mine)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(ok)
+        : "r"(static_cast<uint32_t>(mine)), "r"(barrier), "r"(threads)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ float rcp_fast(float x)
+{
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ unsigned long long pair(float a, float b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+
+// cap * tanh(x), x the score over the cap: cap - 2 cap / (1 + exp(2 x))
+__device__ __forceinline__ float capped(float x, float cap) { return fmaf(-2.0f * cap, rcp_fast(1.0f + tok::exp2_fast(x * 2.8853900817779268f)), cap); }
+// tanh of two values within [-1, 1]: x times a polynomial in x^2, the Chebyshev fit of degree 7 of tanh(x) / x (largest error 5e-9, with fp32 rounding 7e-8)
+__device__ __forceinline__ unsigned long long tanh_inner2(unsigned long long x)
+{
+    constexpr float c[8] = {1.0f, -0.33333307504653931f, 0.13332527875900269f, -0.053887963294982910f, 0.021501919254660606f, -0.0079579148441553116f, 0.0023032133467495441f,
+                            -0.00035729847149923444f};
+    const unsigned long long u = ptx::mul2(x, x);
+    unsigned long long p = ptx::both(c[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = ptx::fma2(p, u, ptx::both(c[i]));
+    return ptx::mul2(p, x);
+}
+
+// Four codes as four bf16 values times a power of two.  A code's bits in a bf16's place (exponent and mantissa side by side) stand for code * 2^-120, subnormal
+// ones among them; one product by 2^(120 + e) puts them right, exactly (e up to 7; the rest, for values beyond 57344, in a second one).
+__device__ __forceinline__ uint32_t bf16_mul(uint32_t a, uint32_t b)
+{
+    uint32_t d;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w, uint32_t power, uint32_t power_rest)
+{
+    uint32_t even = ((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u), odd = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);   // codes 0, 2 and 1, 3
+    even = bf16_mul(even, power);
+    odd = bf16_mul(odd, power);
+    if (power_rest) {
+        even = bf16_mul(even, power_rest);
+        odd = bf16_mul(odd, power_rest);
+    }
+    // the format's NaN: all bits but the sign set
+    const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u;
+    if (nan & 0x80808080u) {
+        if (nan & 0x00000080u) even |= 0x00007fffu;
+        if (nan & 0x00008000u) odd |= 0x00007fffu;
+        if (nan & 0x00800000u) even |= 0x7fff0000u;
+        if (nan & 0x80000000u) odd |= 0x7fff0000u;
+    }
+    return make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+}
+
+}  // namespace pro
+
+template <int NB, bool CODES, bool CAPPED>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+paged_prompt_kernel(const __grid_constant__ PromptArgs args)
+{
+    using S = PromptShape<NB>;
+    constexpr int kind = CODES ? KIND_E4M3 : KIND_BF16;
+    constexpr float kLn2 = 0.69314718055994531f;
+    extern __shared__ uint8_t prompt_smem[];
+    __shared__ long long row_at[2][2][kPromptKeys];   // keys / values, in turn: element of a key's row, -1: zeros
+    __shared__ int row_e[2][2][kPromptKeys];          // codes: exponent
+    __shared__ int arrived_last[2];
+    const Attention &a = args.a;
+    const uint32_t base = (ptx::smem_u32(prompt_smem) + 1023u) & ~1023u;
+    uint8_t *gen = prompt_smem + (base - ptx::smem_u32(prompt_smem));
+    const uint32_t q_base = base, k_base = q_base + 2 * S::kTile, v_base = k_base + S::kStages * S::kTile, bar = v_base + S::kStages * S::kTile;
+    auto k_full = [&](int s) { return bar + 8u * s; };
+    auto k_empty = [&](int s) { return bar + 8u * (3 + s); };
+    auto v_full = [&](int s) { return bar + 8u * (6 + s); };
+    auto v_empty = [&](int s) { return bar + 8u * (9 + s); };
+    auto s_full = [&](int h) { return bar + 8u * (12 + h); };
+    auto p_full = [&](int h) { return bar + 8u * (14 + h); };
+    auto o_full = [&](int h) { return bar + 8u * (16 + h); };
+    const uint32_t q_full = bar + 8u * 18, q_empty = bar + 8u * 19, drain = bar + 8u * 20;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + (bar - base) + 8 * 21);
+    volatile uint32_t *abort_flag = tmem_slot + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *status = a.batch.status;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kPromptMaxStages; ++s) {
+            ptx::mbar_init(k_full(s), 64);
+            ptx::mbar_init(k_empty(s), 1);
+            ptx::mbar_init(v_full(s), 64);
+            ptx::mbar_init(v_empty(s), 1);
+        }
+        for (int h = 0; h < 2; ++h) {
+            ptx::mbar_init(s_full(h), 1);
+            ptx::mbar_init(p_full(h), 128);
+            ptx::mbar_init(o_full(h), 1);
+        }
+        ptx::mbar_init(q_full, 128);
+        ptx::mbar_init(q_empty, 1);
+        ptx::mbar_init(drain, 1);
+        *abort_flag = 0u;
+        ptx::fence_mbar_init();
+    }
+    if (warp == 4) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_slot), 512);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before();
+    __syncthreads();
+    ptx::tc_fence_after();
+    const uint32_t tmem = *tmem_slot;   // columns: S / P of half h at 128 h, O at 256 + 128 h
+    grid_dependency_wait();
+    grid_dependency_launch();
+    Place place;
+    const Range range = range_of_block<kPromptThreads>(a, kPromptRows, kPromptKeys, args.least, place);
+    const int dim = a.pages.dim, steps = (dim + 15) / 16;
+
+    // A tile's part of this block's range, the same for all roles.
+    struct Segment {
+        int blocks, packed0, rows;
+        int first[2], last[2], low[2];   // positions of each half's first and last row; keys below `low` are visible only among the first ones
+    };
+    auto segment_of = [&](const Place &p, long long at) {
+        Segment s;
+        s.blocks = static_cast<int>(min(static_cast<long long>(p.blocks.count - p.off), range.end - at));
+        s.packed0 = p.tile * kPromptRows;
+        s.rows = min(kPromptRows, p.q.count * a.share - s.packed0);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const bool there = h * 128 < s.rows;
+            s.first[h] = there ? p.q.pos0 + (s.packed0 + h * 128) / a.share : -1;
+            s.last[h] = there ? p.q.pos0 + (s.packed0 + min(s.rows, h * 128 + 128) - 1) / a.share : -1;
+            s.low[h] = a.window ? s.first[h] - a.window + 1 : 0;
+        }
+        return s;
+    };
+    auto needs = [&](const Segment &s, int h, int key) { return key <= s.last[h] && (key + kPromptKeys - 1 >= s.low[h] || key < a.sinks); };   // any row of the half, of a block of keys
+
+    if (warp < 4) {
+        ptx::reg_dec<104>();
+        const int which = warp >> 1, t = threadIdx.x & 63;
+        const uint32_t ring = which ? v_base : k_base;
+        const int pieces = dim / 8, mask = (1 << a.pages.page_shift) - 1;
+        bool ok = true;
+        int n = 0, tile = 0;   // blocks and tiles so far
+        for (long long at = range.begin; at < range.end; ++tile) {
+            const Segment seg = segment_of(place, at);
+            // queries: all four warps, a row's pieces of eight side by side
+            ok = bounded_wait(q_empty, (tile & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);   // run out: the warps leave together, below
+            for (int i = threadIdx.x; ok && i < kPromptRows * 8 * NB; i += 128) {
+                const int r = i / (8 * NB), c = i % (8 * NB);
+                if (c >= 2 * steps) continue;
+                uint4 w = make_uint4(0u, 0u, 0u, 0u);
+                if (r < seg.rows && c < pieces) {
+                    const int packed = seg.packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
+                    w = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + row * a.q_pitch + head * dim + c * 8);
+                }
+                ptx::sts128(q_base + (r >> 7) * S::kTile + (c >> 3) * kPromptBlock + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
+            }
+            ptx::fence_proxy_async_smem();
+            ptx::mbar_arrive(q_full);
+            const int low = a.window ? seg.first[0] - a.window + 1 : 0, p1 = max(seg.last[0], seg.last[1]);
+            for (int b = 0; b < seg.blocks; ++b, ++n) {
+                const int key0 = block_key(place.blocks, place.off + b, kPromptKeys), stage = n % S::kStages, turn = n & 1;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int key = key0 + t + 64 * i;
+                    const bool wanted = key <= p1 && (key >= low || key < a.sinks);
+                    const int page = wanted ? page_of(a.batch, a.pages, place.s, key) : -1;
+                    const long long row = page >= 0 ? a.pages.place(page, which, place.g, key & mask) : -1;
+                    row_at[which][turn][t + 64 * i] = row >= 0 ? row * dim : -1;
+                    if (CODES) row_e[which][turn][t + 64 * i] = row >= 0 ? static_cast<int>(a.pages.scales[row]) - 127 : 0;
+                }
+                ok = ok && bounded_wait(which ? v_empty(stage) : k_empty(stage), ((n / S::kStages) & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);
+                if (!pro::all_of(2 + which, 64, ok)) {
+                    ok = false;
+                    break;
+                }
+                const uint32_t dst = ring + stage * S::kTile;
+                if constexpr (CODES) {
+                    const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
+                    constexpr int kPer = 8;
+                    // pieces of eight codes, kPer of them under way per thread
+                    for (int i0 = 0; i0 < kPromptKeys * 8 * NB / 64; i0 += kPer) {
+                        uint2 w[kPer];
+#pragma unroll
+                        for (int u = 0; u < kPer; ++u) {
+                            const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
+                            const long long row = row_at[which][turn][r];
+                            w[u] = row >= 0 && c < pieces ? *reinterpret_cast<const uint2 *>(data + row + c * 8) : make_uint2(0u, 0u);
+                        }
+#pragma unroll
+                        for (int u = 0; u < kPer; ++u) {
+                            const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
+                            const int e = row_e[which][turn][r];
+                            const uint32_t power = (120 + min(e, 7) + 127) << 7, rest = e > 7 ? (e - 7 + 127) << 7 : 0;
+                            const uint2 x = pro::codes_to_bf16(w[u].x, power * 0x10001u, rest * 0x10001u), y = pro::codes_to_bf16(w[u].y, power * 0x10001u, rest * 0x10001u);
+                            if (c < 2 * steps) ptx::sts128(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                        }
+                    }
+                } else {
+                    const __nv_bfloat16 *data = static_cast<const __nv_bfloat16 *>(a.pages.data);
+#pragma unroll 8
+                    for (int i = 0; i < kPromptKeys * 8 * NB / 64; ++i) {
+                        const int idx = i * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
+                        const long long row = row_at[which][turn][r];
+                        const bool on = row >= 0 && c < pieces;
+                        if (c < 2 * steps) tok::copy<16>(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? data + row + c * 8 : data, on);
+                    }
+                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                }
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(which ? v_full(stage) : k_full(stage));
+            }
+            if (!ok) break;
+            at += seg.blocks;
+            if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+        }
+    } else if (warp < 8) {
+        ptx::reg_dec<40>();
+        if (warp == 4) {
+            const bool issuer = ptx::elect_one();
+            constexpr uint32_t idesc_s = ptx::make_idesc_bf16(128, 128, false, false);
+            const uint32_t idesc_o = ptx::make_idesc_bf16(128, 16 * steps, false, true);
+            const ptx::SmemDesc dq = ptx::smem_desc_words(q_base, 16, 1024, ptx::kLayoutSw128), dk = ptx::smem_desc_words(k_base, 16, 1024, ptx::kLayoutSw128),
+                                dv = ptx::smem_desc_words(v_base, kPromptBlock, 1024, ptx::kLayoutSw128);
+            auto wait = [&](uint32_t b, uint32_t parity, int code) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, code)); };
+            bool ok = true;
+            int n = 0, tile = 0, turns[2] = {0, 0};
+            for (long long at = range.begin; ok && at < range.end; ++tile) {
+                const Segment seg = segment_of(place, at);
+                bool begun[2] = {false, false}, wanted[2] = {false, false};
+                ok = wait(q_full, tile & 1, DEV_TIMEOUT_MMA_FULL);
+                for (int b = -1; ok && b < seg.blocks; ++b) {
+                    const int vs = (n + b) % S::kStages, ks = (n + b + 1) % S::kStages;
+                    const bool more = b + 1 < seg.blocks;
+                    const int next_key = more ? block_key(place.blocks, place.off + b + 1, kPromptKeys) : 0;
+                    if (b >= 0) ok = wait(v_full(vs), ((n + b) / S::kStages) & 1, DEV_TIMEOUT_MMA_FULL);
+                    bool have_k = false;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (ok && b >= 0 && wanted[h]) {
+                            ok = wait(p_full(h), turns[h] & 1, DEV_TIMEOUT_MMA_TMEM);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            if (issuer) {
+                                uint32_t acc = begun[h];
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    pro::mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 8 * k, dv.at(vs * S::kTile + k * 2048), idesc_o, acc);
+                                    acc = 1;
+                                }
+                            }
+                            __syncwarp();
+                            begun[h] = true;
+                            turns[h]++;
+                        }
+                        if (!ok) break;
+                        wanted[h] = more && needs(seg, h, next_key);
+                        if (more && !have_k) {
+                            ok = wait(k_full(ks), ((n + b + 1) / S::kStages) & 1, DEV_TIMEOUT_MMA_FULL);
+                            if (!ok) break;
+                            ptx::tc_fence_after();
+                            have_k = true;
+                        }
+                        if (wanted[h]) {
+                            if (issuer) {
+                                uint32_t acc = 0;
+                                for (int k = 0; k < steps; ++k) {
+                                    const uint32_t off = (k >> 2) * kPromptBlock + (k & 3) * 32;
+                                    ptx::mma_f16_ss(tmem + 128 * h, dq.at(h * S::kTile + off), dk.at(ks * S::kTile + off), idesc_s, acc);
+                                    acc = 1;
+                                }
+                                ptx::mma_commit(s_full(h));
+                            }
+                            __syncwarp();
+                        }
+                    }
+                    if (!ok) break;
+                    if (issuer) {
+                        if (b >= 0) ptx::mma_commit(v_empty(vs));
+                        if (more) ptx::mma_commit(k_empty(ks));
+                        if (b + 2 == seg.blocks) ptx::mma_commit(q_empty);   // the last scores
+                        if (!more) {
+                            ptx::mma_commit(o_full(0));
+                            ptx::mma_commit(o_full(1));
+                        }
+                    }
+                    __syncwarp();
+                }
+                if (!ok) break;
+                n += seg.blocks;
+                at += seg.blocks;
+                if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+            }
+            if (issuer) ptx::mma_commit(drain);
+            __syncwarp();
+            bounded_wait(drain, 0u, abort_flag, status, DEV_TIMEOUT_DRAIN);
+        }
+        __syncwarp();
+    } else {
+        ptx::reg_inc<184>();
+        const int h = warp >= 12, quarter = warp & 3;
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t s_addr = tmem + lanes + 128 * h, o_addr = tmem + lanes + 256 + 128 * h;
+        const int r = quarter * 32 + lane;   // row within the half
+        auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, DEV_TIMEOUT_EPILOGUE)); };
+        bool ok = true;
+        int turns = 0, tile = 0;
+        for (long long at = range.begin; at < range.end; ++tile) {
+            const Segment seg = segment_of(place, at);
+            const int packed = seg.packed0 + h * 128 + r;
+            const bool there = h * 128 + r < seg.rows;
+            const int token = packed / a.share, position = there ? place.q.pos0 + token : -1;
+            float ref = -INFINITY, sum = 0.0f;   // what the weights stand against (base 2), their sum
+            bool begun = false;
+            for (int b = 0; b < seg.blocks; ++b) {
+                const int key0 = block_key(place.blocks, place.off + b, kPromptKeys);
+                if (!needs(seg, h, key0)) continue;
+                ok = wait(s_full(h), turns & 1);
+                if (!ok) break;
+                ptx::tc_fence_after();
+                turns++;
+                const bool whole = key0 + kPromptKeys - 1 <= seg.first[h] && (a.window == 0 || key0 > seg.last[h] - a.window || key0 + kPromptKeys - 1 < a.sinks);
+                uint32_t x[4][32];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(s_addr + 32 * c, x[c]);
+                ptx::tmem_ld_wait();
+                if (!whole) {
+                    const int high = position - key0, low = a.window ? high - a.window : -1, first = a.sinks - key0;
+#pragma unroll
+                    for (int i = 0; i < kPromptKeys; ++i)
+                        if (i > high || (i <= low && i >= first)) x[i >> 5][i & 31] = 0xff800000u;   // minus infinity
+                }
+                bool near_zero = true;   // no score of the warp's rows beyond the cap: tanh is a polynomial
+                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, least[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+#pragma unroll
+                for (int i = 0; i < kPromptKeys; ++i) {
+                    const float v = __uint_as_float(x[i >> 5][i & 31]);
+                    most[i & 3] = fmaxf(most[i & 3], v);
+                    if (CAPPED) least[i & 3] = fminf(least[i & 3], v == -INFINITY ? 0.0f : v);
+                }
+                float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                if (CAPPED) {
+                    const float down = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
+                    near_zero = __all_sync(0xffffffffu, fmaxf(top, -down) * args.cap_arg <= 1.0f);
+                    if (top > -INFINITY) top = pro::capped(top * args.cap_arg, args.cap_log2);
+                } else {
+                    top *= args.scale_log2;
+                }
+                const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
+                if (!begun) {
+                    ref = top;
+                } else if (__any_sync(0xffffffffu, grow)) {
+                    // earlier weights stand against the old maximum: scale O (complete: this block's scores come after it) and the sum
+                    const float f = grow ? tok::exp2_fast(ref - top) : 1.0f;
+                    if (grow) ref = top;
+                    sum *= f;
+                    for (int c = 0; c < 16 * steps; c += 16) {
+                        uint32_t o[16];
+                        pro::tmem_ld_32x16(o_addr + c, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        pro::tmem_st_32x16(o_addr + c, o);
+                    }
+                }
+                begun = true;
+                const float use = ref == -INFINITY ? 0.0f : ref;   // nothing seen yet: every weight is 2^-inf = 0
+                const unsigned long long scale2 = ptx::both(CAPPED ? args.cap_arg : args.scale_log2), minus_ref = ptx::both(-use);
+                unsigned long long sums[2] = {0, 0};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float s0 = __uint_as_float(x[c][2 * i]), s1 = __uint_as_float(x[c][2 * i + 1]);
+                        float e0, e1;
+                        if (!CAPPED) {
+                            pro::unpair(ptx::fma2(pro::pair(s0, s1), scale2, minus_ref), e0, e1);
+                        } else if (near_zero) {
+                            // the polynomial of a hidden score (minus infinity) is NaN: hidden again below
+                            pro::unpair(ptx::fma2(pro::tanh_inner2(ptx::mul2(pro::pair(s0, s1), scale2)), ptx::both(args.cap_log2), minus_ref), e0, e1);
+                            if (!whole) {
+                                if (s0 == -INFINITY) e0 = -INFINITY;
+                                if (s1 == -INFINITY) e1 = -INFINITY;
+                            }
+                        } else {
+                            e0 = pro::capped(s0 * args.cap_arg, args.cap_log2) - use;
+                            e1 = pro::capped(s1 * args.cap_arg, args.cap_log2) - use;
+                            if (!whole) {
+                                if (s0 == -INFINITY) e0 = -INFINITY;
+                                if (s1 == -INFINITY) e1 = -INFINITY;
+                            }
+                        }
+                        e0 = tok::exp2_fast(e0);
+                        e1 = tok::exp2_fast(e1);
+                        sums[i & 1] = ptx::add2(sums[i & 1], pro::pair(e0, e1));
+                        w[i] = ptx::pack_bf16x2(e0, e1);
+                    }
+                    pro::tmem_st_32x16(s_addr + 16 * c, w);
+                }
+                {
+                    float e0, e1;
+                    pro::unpair(ptx::add2(sums[0], sums[1]), e0, e1);
+                    sum += e0 + e1;
+                }
+                pro::tmem_st_wait();
+                ptx::tc_fence_before();
+                ptx::mbar_arrive(p_full(h));
+            }
+            if (ok) ok = wait(o_full(h), tile & 1);
+            ptx::tc_fence_after();
+            if (!pro::all_of(4 + h, 128, ok)) break;
+            if (h * 128 < seg.rows) {
+                const long long first = at - place.off, last = first + place.blocks.count - 1;   // the tile's blocks on the line
+                const bool whole = place.off == 0 && seg.blocks == place.blocks.count;
+                const bool sees = position >= 0;
+                const int head = place.g * a.share + packed % a.share;
+                const long long row = place.q.row0 + token;
+                __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + row * a.out_pitch + head * dim;
+                bool fine = true;
+                auto store = [&](int c, const uint32_t (&o)[16], float by) {   // columns c .. c + 15
+                    uint32_t w[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float u = __uint_as_float(o[2 * i]) * by, v = __uint_as_float(o[2 * i + 1]) * by;
+                        fine = fine && (c + 2 * i >= dim || (fabsf(u) <= FLT_MAX && fabsf(v) <= FLT_MAX));
+                        w[i] = sees ? ptx::pack_bf16x2(u, v) : 0u;
+                    }
+                    if (there && c < dim) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
+                    if (there && c + 8 < dim) *reinterpret_cast<uint4 *>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+                };
+                auto store_sum = [&](float top, float total) {
+                    if (a.lse && there) a.lse[row * a.heads + head] = sees ? top * kLn2 + logf(total) : -INFINITY;
+                };
+                bool done = whole;
+                if (whole) {
+                    const float by = 1.0f / sum;
+                    for (int c = 0; c < 16 * steps; c += 16) {
+                        uint32_t o[16];
+                        pro::tmem_ld_32x16(o_addr + c, o);
+                        ptx::tmem_ld_wait();
+                        store(c, o, by);
+                    }
+                    store_sum(ref, sum);
+                } else {
+                    // four columns of all rows side by side, so that the rows' threads write and read runs
+                    float *part = args.parts.base + (2LL * blockIdx.x + (first >= range.begin)) * args.parts.floats + h * (128 * 128 + 256);
+                    for (int c = 0; c < 16 * steps; c += 16) {
+                        uint32_t o[16];
+                        pro::tmem_ld_32x16(o_addr + c, o);
+                        ptx::tmem_ld_wait();
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            *reinterpret_cast<uint4 *>(part + ((c / 4 + i) * 128 + r) * 4) = begun ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+                    *reinterpret_cast<float2 *>(part + 128 * 128 + 2 * r) = make_float2(ref, sum);
+                    const int b0 = static_cast<int>(first / range.per), b1 = static_cast<int>(last / range.per);
+                    __threadfence();
+                    pro::all_of(4 + h, 128, true);
+                    if (r == 0) {
+                        const unsigned int before = atomicAdd(args.parts.tickets + 2 * b0 + h, 1u);
+                        arrived_last[h] = before == static_cast<unsigned int>(b1 - b0);
+                        if (arrived_last[h]) args.parts.tickets[2 * b0 + h] = 0u;
+                        __threadfence();
+                    }
+                    pro::all_of(4 + h, 128, true);
+                    done = arrived_last[h];
+                    if (done) {
+                        auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats + h * (128 * 128 + 256); };
+                        float top = -INFINITY, total = 0.0f;
+                        for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(slot(b) + 128 * 128 + 2 * r));
+                        for (int b = b0; b <= b1; ++b) {
+                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(b) + 128 * 128 + 2 * r));
+                            total = fmaf(ml.y, tok::share_of(ml.x, top), total);
+                        }
+                        const float by = 1.0f / total;
+                        for (int c = 0; c < 16 * steps; c += 16) {
+                            float v[16] = {};
+                            for (int b = b0; b <= b1; ++b) {
+                                const float *from = slot(b);
+                                const float f = tok::share_of(__ldcg(from + 128 * 128 + 2 * r), top);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    const float4 u = __ldcg(reinterpret_cast<const float4 *>(from + ((c / 4 + i) * 128 + r) * 4));
+                                    v[4 * i] = fmaf(u.x, f, v[4 * i]); v[4 * i + 1] = fmaf(u.y, f, v[4 * i + 1]);
+                                    v[4 * i + 2] = fmaf(u.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(u.w, f, v[4 * i + 3]);
+                                }
+                            }
+                            uint32_t o[16];
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(v[i]);
+                            store(c, o, by);
+                        }
+                        store_sum(top, total);
+                    }
+                }
+                // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is
+                // formed once more from its own keys alone.
+                __syncwarp();
+                for (uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && !fine); bad; bad &= bad - 1) {
+                    const int p = seg.packed0 + h * 128 + quarter * 32 + __ffs(bad) - 1;
+                    attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + p / a.share, place.q.row0 + p / a.share, place.g * a.share + p % a.share, lane);
+                }
+            }
+            ptx::tc_fence_before();   // the accumulator has been read: the next tile's products may write it (they wait for its weights)
+            at += seg.blocks;
+            if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+        }
+    }
+
+    ptx::tc_fence_before();
+    __syncthreads();
+    if (warp == 4) {
+        ptx::tc_fence_after();
+        ptx::tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace kvp
+}  // namespace gptb200
