@@ -139,7 +139,7 @@ int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args)
 
 int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
 {
-    kvp::TokensArgs args{a, {}, 4};
+    kvp::TokensArgs args{a, {}, {kvp::kTokensRows, kvp::kTokensKeys, 1, 5}};
     const bool codes = kind == GPTB200_KV_E4M3;
     switch ((a.pages.dim + 31) / 32) {
         case 1: return codes ? run_tokens<2, true>(ctx, args) : run_tokens<2, false>(ctx, args);
@@ -159,8 +159,19 @@ int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args)
 int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
 {
     constexpr float kLog2e = 1.4426950408889634f;
-    kvp::PromptArgs args{a, {}, 2, a.scale * kLog2e, a.cap * kLog2e, a.cap > 0.0f ? a.scale / a.cap : 0.0f};
     const bool codes = kind == GPTB200_KV_E4M3;
+    kvp::PromptArgs args{};
+    args.a = a;
+    args.cut = {kvp::kPromptRows, kvp::kPromptKeys, 2, 4};
+    args.scale_log2 = a.scale * kLog2e;
+    args.cap_log2 = a.cap * kLog2e;
+    args.cap_arg = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
+    const long long rows = (2LL * a.pages.num_pages * a.pages.kv_heads) << a.pages.page_shift;
+    if (!codes && rows > 0 && rows <= INT_MAX) {
+        args.box_rows = std::min(1 << a.pages.page_shift, kvp::kPromptKeys);
+        const int rc = bf16_operand_map(ctx, &args.map, a.pages.data, rows, a.pages.dim, a.pages.dim, args.box_rows);
+        if (rc != GPTB200_OK) return rc;
+    }
     if (a.pages.dim <= 64) return codes ? run_prompt<1, true>(ctx, args) : run_prompt<1, false>(ctx, args);
     return codes ? run_prompt<2, true>(ctx, args) : run_prompt<2, false>(ctx, args);
 }
@@ -198,6 +209,7 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     CUDA_TRY(ctx, device.enter(ctx->device));
     a.q = q; a.out = out; a.lse = lse; a.q_pitch = q_pitch; a.out_pitch = out_pitch;
     a.heads = heads; a.share = heads / pages->kv_heads;
+    a.shares = kvp::divisor(a.share);
     a.scale = scale; a.cap = cap;
     a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
     a.sinks = a.window ? sinks : 0;

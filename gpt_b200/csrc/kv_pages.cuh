@@ -263,6 +263,29 @@ kv_rows_kernel(const RowsArgs a)
 
 // ---- attention
 
+// Division of numbers below 2^31 by a number known on the host, as a product and a shift (Granlund and Montgomery, Division by invariant integers using
+// multiplication, 1994): a tile's positions take half a dozen divisions by the group's size, which were 3 000 cycles between two tiles.
+struct Divisor {
+    uint32_t by = 1, factor = 0;
+    int shift = 0;
+    __host__ __device__ inline int divide(int n) const
+    {
+#ifdef __CUDA_ARCH__
+        return static_cast<int>((__umulhi(static_cast<uint32_t>(n), factor) + static_cast<uint32_t>(n)) >> shift);
+#else
+        return static_cast<int>((static_cast<uint32_t>((static_cast<uint64_t>(n) * factor) >> 32) + static_cast<uint32_t>(n)) >> shift);
+#endif
+    }
+};
+inline Divisor divisor(uint32_t by)
+{
+    Divisor d;
+    d.by = by;
+    while ((1ull << d.shift) < by) ++d.shift;
+    d.factor = static_cast<uint32_t>((((1ull << d.shift) - by) << 32) / by + 1);
+    return d;
+}
+
 struct Attention {
     Pages pages;
     Batch batch;
@@ -271,6 +294,7 @@ struct Attention {
     float *lse;                // [rows][heads] or null
     long long q_pitch, out_pitch;
     int heads, share;          // share: query heads per key / value head
+    Divisor shares;
     float scale, cap;          // cap 0: none
     int window, sinks;         // window 0: all earlier tokens
 };
@@ -298,24 +322,31 @@ struct KeyBlocks {
 __host__ __device__ inline KeyBlocks key_blocks(int p0, int p1, int window, int sinks, int keys)
 {
     if (p1 < 0) return {0, 0, 1};
-    const int from = window > 0 ? larger(0, p0 - window + 1) / keys : 0;
-    const int ones = window > 0 ? smaller((smaller(sinks, p1 + 1) + keys - 1) / keys, from) : 0;
-    return {ones, from, ones + p1 / keys - from + 1};
+    const unsigned n = keys;
+    const int from = window > 0 ? static_cast<int>(larger(0, p0 - window + 1) / n) : 0;
+    const int ones = window > 0 ? smaller(static_cast<int>((smaller(sinks, p1 + 1) + n - 1) / n), from) : 0;
+    return {ones, from, ones + static_cast<int>(p1 / n) - from + 1};
 }
 __host__ __device__ inline int block_key(const KeyBlocks &b, int i, int keys) { return (i < b.first_ones ? i : b.from + i - b.first_ones) * keys; }
 
 // Tile t of a sequence's rows of one key / value head.
 __host__ __device__ inline KeyBlocks tile_blocks(const Attention &a, const Sequence &q, int t, int tile_rows, int keys)
 {
-    const int first = t * tile_rows / a.share, last = smaller((t + 1) * tile_rows, q.count * a.share) - 1;
-    return key_blocks(q.pos0 + first, q.pos0 + last / a.share, a.window, a.sinks, keys);
+    const int first = t * tile_rows, last = smaller((t + 1) * tile_rows, q.count * a.share) - 1;
+    return key_blocks(q.pos0 + a.shares.divide(first), q.pos0 + a.shares.divide(last), a.window, a.sinks, keys);
 }
 __host__ __device__ inline int tiles_of(const Attention &a, const Sequence &q, int tile_rows) { return (q.count * a.share + tile_rows - 1) / tile_rows; }
-__host__ __device__ inline long long blocks_of(const Attention &a, const Sequence &q, int tile_rows, int keys)
+
+// How a kernel cuts the line: rows of a tile, keys of a block, blocks that a tile's own costs stand for, blocks per range at least.
+struct Cut {
+    int tile_rows, keys, lead, least;
+};
+
+__host__ __device__ inline long long blocks_of(const Attention &a, const Sequence &q, const Cut &cut)
 {
-    long long n = 0;
-    const int tiles = tiles_of(a, q, tile_rows);
-    for (int t = 0; t < tiles; ++t) n += tile_blocks(a, q, t, tile_rows, keys).count;
+    const int tiles = tiles_of(a, q, cut.tile_rows);
+    long long n = 1LL * tiles * cut.lead;
+    for (int t = 0; t < tiles; ++t) n += tile_blocks(a, q, t, cut.tile_rows, cut.keys).count;
     return n;
 }
 
@@ -324,11 +355,11 @@ struct Place {
     Sequence q;
     KeyBlocks blocks;
     int s, g, tile, tiles;
-    int off;              // block within the tile
+    int off;              // place within the tile: `lead` ones without a block of keys, then its blocks
 };
 
 // Next tile that has rows; false behind the last one.
-__host__ __device__ inline bool next_tile(const Attention &a, Place &p, int tile_rows, int keys)
+__host__ __device__ inline bool next_tile(const Attention &a, Place &p, const Cut &cut)
 {
     p.off = 0;
     if (++p.tile >= p.tiles) {
@@ -339,82 +370,139 @@ __host__ __device__ inline bool next_tile(const Attention &a, Place &p, int tile
                 if (++p.s >= a.batch.sequences) return false;
                 p.q = sequence_of(a.batch, p.s);
             } while (p.q.count == 0);
-            p.tiles = tiles_of(a, p.q, tile_rows);
+            p.tiles = tiles_of(a, p.q, cut.tile_rows);
         }
     }
-    p.blocks = tile_blocks(a, p.q, p.tile, tile_rows, keys);
+    p.blocks = tile_blocks(a, p.q, p.tile, cut.tile_rows, cut.keys);
     return true;
 }
 
-// The place `rest` blocks into sequence s, whose head's tiles have `per_head` blocks in all.
-__host__ __device__ inline Place place_in(const Attention &a, int s, long long rest, long long per_head, int tile_rows, int keys)
-{
-    Place p;
-    p.s = s;
-    p.q = sequence_of(a.batch, s);
-    p.tiles = tiles_of(a, p.q, tile_rows);
-    p.g = static_cast<int>(rest / per_head);
-    rest -= p.g * per_head;
-    for (p.tile = 0;; ++p.tile) {
-        p.blocks = tile_blocks(a, p.q, p.tile, tile_rows, keys);
-        if (rest < p.blocks.count || p.tile + 1 >= p.tiles) break;
-        rest -= p.blocks.count;
-    }
-    p.off = static_cast<int>(rest);
-    return p;
-}
-
 struct Range {
-    long long begin, end;   // this block's blocks of the line
+    long long begin, end;   // this block's part of the line
     long long per;          // of every block of the grid
 };
 
-// The block's range of the line and the place where it begins; an empty range: nothing to do.  All threads of the block take part; a block has THREADS of them.
-template <int THREADS>
-__device__ inline Range range_of_block(const Attention &a, int tile_rows, int keys, int least, Place &place)
+// What of the tile at `at` lies in a range: places of the line, and blocks of keys among them.
+struct Part {
+    int places, from, blocks;
+    bool whole;             // all of the tile's blocks
+    long long first_block, last_block;   // of the tile, on the line
+};
+__host__ __device__ inline Part part_of(const Place &p, const Range &r, long long at, const Cut &cut)
 {
-    __shared__ long long sums[THREADS / 32];
-    __shared__ long long found_rest, found_per_head;
-    __shared__ int found_s;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int chunk = (a.batch.sequences + THREADS - 1) / THREADS, s0 = threadIdx.x * chunk, s1 = min(s0 + chunk, a.batch.sequences);
-    long long mine = 0;
-    for (int s = s0; s < s1; ++s) mine += blocks_of(a, sequence_of(a.batch, s), tile_rows, keys) * a.pages.kv_heads;
-    long long upto = mine;   // inclusive prefix
+    Part t;
+    const int rest = cut.lead + p.blocks.count - p.off;
+    t.places = r.end - at < rest ? static_cast<int>(r.end - at) : rest;
+    t.from = larger(p.off - cut.lead, 0);
+    t.blocks = larger(p.off + t.places - cut.lead - t.from, 0);
+    t.whole = t.blocks == p.blocks.count;
+    t.first_block = at - p.off + cut.lead;
+    t.last_block = t.first_block + p.blocks.count - 1;
+    return t;
+}
+
+// blocks_of of 32 sequences, one per lane (count 0: none): a lane adds up a few tiles itself, many are added up by the whole warp.
+__device__ inline long long blocks_of_lanes(const Attention &a, const Sequence &q, const Cut &cut, int lane)
+{
+    constexpr int kFew = 4;
+    const int tiles = tiles_of(a, q, cut.tile_rows);
+    long long n = tiles <= kFew ? blocks_of(a, q, cut) : 0;
+    for (unsigned many = __ballot_sync(0xffffffffu, tiles > kFew); many; many &= many - 1) {
+        const int from = __ffs(many) - 1;
+        const Sequence other = {0, __shfl_sync(0xffffffffu, q.count, from), __shfl_sync(0xffffffffu, q.pos0, from)};
+        long long sum = 0;
+        for (int t = lane; t < tiles_of(a, other, cut.tile_rows); t += 32) sum += cut.lead + tile_blocks(a, other, t, cut.tile_rows, cut.keys).count;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == from) n = sum;
+    }
+    return n;
+}
+
+__device__ inline long long inclusive_sum(long long v, int lane)
+{
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
     }
-    if (lane == 31) sums[warp] = upto;
-    __syncthreads();
-    long long total = 0;
+    return v;
+}
+
+// The block's range of the line and the place where it begins; an empty range: nothing to do.  All threads of the block take part; a block has THREADS of them.
+// Every warp adds up its share of the sequences; the one whose share holds the range's beginning finds the place.
+template <int THREADS>
+__device__ inline Range range_of_block(const Attention &a, const Cut &cut, Place &place)
+{
+    constexpr int kWarps = THREADS / 32;
+    __shared__ long long sums[kWarps];
+    __shared__ Place found;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = (a.batch.sequences + kWarps - 1) / kWarps, s0 = warp * share, s1 = min(s0 + share, a.batch.sequences);
+    auto of_lane = [&](int s, Sequence &q) {
+        q = s < s1 ? sequence_of(a.batch, s) : Sequence{0, 0, 0};
+        return blocks_of_lanes(a, q, cut, lane);
+    };
+    long long mine = 0;
+    Sequence q;
+    for (int s = s0; s < s1; s += 32) mine += of_lane(s + lane, q) * a.pages.kv_heads;
 #pragma unroll
-    for (int w = 0; w < THREADS / 32; ++w) {
-        if (w < warp) upto += sums[w];
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) sums[warp] = mine;
+    __syncthreads();
+    long long total = 0, before = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += sums[w];
         total += sums[w];
     }
     Range r;
-    r.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(least));
+    r.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(cut.least));
     r.begin = min(r.per * blockIdx.x, total);
     r.end = min(r.begin + r.per, total);
-    if (r.begin < r.end) {
-        if (upto - mine <= r.begin && r.begin < upto) {
-            long long rest = r.begin - (upto - mine);
-            for (int s = s0; s < s1; ++s) {
-                const long long per_head = blocks_of(a, sequence_of(a.batch, s), tile_rows, keys), n = per_head * a.pages.kv_heads;
-                if (rest < n) {
-                    found_s = s;
-                    found_rest = rest;
-                    found_per_head = per_head;
-                    break;
-                }
-                rest -= n;
+    if (r.begin >= r.end) return r;
+    if (before <= r.begin && r.begin < before + mine) {   // one warp of the block
+        long long rest = r.begin - before;
+        for (int s = s0; s < s1; s += 32) {
+            const long long per_head = of_lane(s + lane, q), n = per_head * a.pages.kv_heads, upto = inclusive_sum(n, lane);
+            const unsigned behind = __ballot_sync(0xffffffffu, rest < upto);
+            if (behind == 0) {
+                rest -= __shfl_sync(0xffffffffu, upto, 31);
+                continue;
             }
+            const int at = __ffs(behind) - 1;
+            const long long head_blocks = __shfl_sync(0xffffffffu, per_head, at);
+            Place p;
+            p.s = s + at;
+            p.q = {__shfl_sync(0xffffffffu, q.row0, at), __shfl_sync(0xffffffffu, q.count, at), __shfl_sync(0xffffffffu, q.pos0, at)};
+            p.tiles = tiles_of(a, p.q, cut.tile_rows);
+            rest -= __shfl_sync(0xffffffffu, upto - n, at);
+            p.g = static_cast<int>(rest / head_blocks);
+            rest -= p.g * head_blocks;
+            for (int t = 0; t < p.tiles; t += 32) {
+                const bool in = t + lane < p.tiles;
+                KeyBlocks blocks = {0, 0, 0};
+                if (in) blocks = tile_blocks(a, p.q, t + lane, cut.tile_rows, cut.keys);
+                const int places = in ? cut.lead + blocks.count : 0;
+                const long long end = inclusive_sum(places, lane);
+                const unsigned past = __ballot_sync(0xffffffffu, in && rest < end);
+                if (past == 0) {
+                    rest -= __shfl_sync(0xffffffffu, end, 31);
+                    continue;
+                }
+                if (lane == __ffs(past) - 1) {
+                    p.tile = t + lane;
+                    p.blocks = blocks;
+                    p.off = static_cast<int>(rest - (end - places));
+                    found = p;
+                }
+                break;
+            }
+            break;
         }
-        __syncthreads();
-        place = place_in(a, found_s, found_rest, found_per_head, tile_rows, keys);
     }
+    __syncthreads();
+    place = found;
     return r;
 }
 

@@ -11,6 +11,7 @@
 //   warps 0-1, 2-3   keys, values (named barriers 2 and 3): pages are looked up per key, rows come by asynchronous 16-byte copies into the swizzled layout that the tensor core reads (a
 //                    page is as small as eight tokens; an e4m3 row goes through registers and becomes bf16 there, exactly); all four fetch queries
 //   warp 4           issues the products, one elected lane
+//   warp 5           walks along the line and hands the others each tile's part of the range through a ring in shared memory
 //   warps 8-11       softmax and output of half 0;  warps 12-15: half 1
 // Keys and values that no row of the tile sees are zeros in shared memory, whatever the pages hold there.  Every wait is bounded.
 #pragma once
@@ -29,13 +30,16 @@ template <int NB>   // 64-column blocks of a head
 struct PromptShape {
     static constexpr int kStages = NB == 1 ? 3 : 2;
     static constexpr int kTile = NB * kPromptBlock;
-    static constexpr int kSmem = (2 + 2 * kStages) * kTile + 1024 + 256;
+    static constexpr int kStaging = 8 * 2048;   // per softmax warp 64 bytes of 32 output rows
+    static constexpr int kSmem = (2 + 2 * kStages) * kTile + kStaging + 1024 + 256;
 };
 
-struct PromptArgs {
+struct alignas(64) PromptArgs {
+    CUtensorMap map;           // bf16 pools: [page, keys / values, head, token][dimension in words], boxes of box_rows x 64 elements
+    int box_rows;              // tokens of a page, at most 128; 0: no map (codes, or more rows than a map has)
     Attention a;
     Parts parts;
-    int least;
+    Cut cut;
     float scale_log2;          // scale * log2(e)
     float cap_log2, cap_arg;   // cap * log2(e), scale / cap
 };
@@ -84,6 +88,9 @@ __device__ __forceinline__ bool all_of(int barrier, int threads, bool mine)
         : "memory");
     return ok != 0;
 }
+
+// Bits 0 .. n - 1 of a word.
+__device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
 __device__ __forceinline__ float rcp_fast(float x)
 {
@@ -143,6 +150,18 @@ __device__ __forceinline__ uint2 codes_to_bf16(uint32_t w, uint32_t power, uint3
 
 }  // namespace pro
 
+// A tile's part of a range, as the roles need it.
+struct Segment {
+    int blocks;               // 0: the range is done
+    int s, g, row0, pos0, packed0, rows;
+    int from;                 // first block among the tile's
+    KeyBlocks keys;
+    int first[2], last[2], low[2];   // positions of each half's first and last row; keys below `low` are visible only among the first ones
+    bool whole, tail;         // all of the tile's blocks; the tile begins in this range
+    int b0, b1;               // blocks of the grid that share the tile
+};
+constexpr int kPromptSegments = 4, kPromptSegmentWarps = 13;   // ring; warps that read it
+
 template <int NB, bool CODES, bool CAPPED>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 paged_prompt_kernel(const __grid_constant__ PromptArgs args)
@@ -154,10 +173,11 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
     __shared__ long long row_at[2][2][kPromptKeys];   // keys / values, in turn: element of a key's row, -1: zeros
     __shared__ int row_e[2][2][kPromptKeys];          // codes: exponent
     __shared__ int arrived_last[2];
+    __shared__ Segment segments[kPromptSegments];
     const Attention &a = args.a;
     const uint32_t base = (ptx::smem_u32(prompt_smem) + 1023u) & ~1023u;
     uint8_t *gen = prompt_smem + (base - ptx::smem_u32(prompt_smem));
-    const uint32_t q_base = base, k_base = q_base + 2 * S::kTile, v_base = k_base + S::kStages * S::kTile, bar = v_base + S::kStages * S::kTile;
+    const uint32_t q_base = base, k_base = q_base + 2 * S::kTile, v_base = k_base + S::kStages * S::kTile, staging = v_base + S::kStages * S::kTile, bar = staging + S::kStaging;
     auto k_full = [&](int s) { return bar + 8u * s; };
     auto k_empty = [&](int s) { return bar + 8u * (3 + s); };
     auto v_full = [&](int s) { return bar + 8u * (6 + s); };
@@ -166,7 +186,9 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
     auto p_full = [&](int h) { return bar + 8u * (14 + h); };
     auto o_full = [&](int h) { return bar + 8u * (16 + h); };
     const uint32_t q_full = bar + 8u * 18, q_empty = bar + 8u * 19, drain = bar + 8u * 20;
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + (bar - base) + 8 * 21);
+    auto seg_full = [&](int i) { return bar + 8u * (21 + i % kPromptSegments); };
+    auto seg_empty = [&](int i) { return bar + 8u * (21 + kPromptSegments + i % kPromptSegments); };
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + (bar - base) + 8 * (21 + 2 * kPromptSegments));
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *status = a.batch.status;
@@ -182,6 +204,11 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             ptx::mbar_init(s_full(h), 1);
             ptx::mbar_init(p_full(h), 128);
             ptx::mbar_init(o_full(h), 1);
+        }
+        if (!CODES && args.box_rows) ptx::prefetch_tensormap(&args.map);
+        for (int i = 0; i < kPromptSegments; ++i) {
+            ptx::mbar_init(seg_full(i), 1);
+            ptx::mbar_init(seg_empty(i), kPromptSegmentWarps);
         }
         ptx::mbar_init(q_full, 128);
         ptx::mbar_init(q_empty, 1);
@@ -200,27 +227,14 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
     grid_dependency_wait();
     grid_dependency_launch();
     Place place;
-    const Range range = range_of_block<kPromptThreads>(a, kPromptRows, kPromptKeys, args.least, place);
+    const Range range = range_of_block<kPromptThreads>(a, args.cut, place);
     const int dim = a.pages.dim, steps = (dim + 15) / 16;
 
-    // A tile's part of this block's range, the same for all roles.
-    struct Segment {
-        int blocks, packed0, rows;
-        int first[2], last[2], low[2];   // positions of each half's first and last row; keys below `low` are visible only among the first ones
-    };
-    auto segment_of = [&](const Place &p, long long at) {
-        Segment s;
-        s.blocks = static_cast<int>(min(static_cast<long long>(p.blocks.count - p.off), range.end - at));
-        s.packed0 = p.tile * kPromptRows;
-        s.rows = min(kPromptRows, p.q.count * a.share - s.packed0);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const bool there = h * 128 < s.rows;
-            s.first[h] = there ? p.q.pos0 + (s.packed0 + h * 128) / a.share : -1;
-            s.last[h] = there ? p.q.pos0 + (s.packed0 + min(s.rows, h * 128 + 128) - 1) / a.share : -1;
-            s.low[h] = a.window ? s.first[h] - a.window + 1 : 0;
-        }
-        return s;
+    auto segment = [&](int i) -> const Segment & { return segments[i % kPromptSegments]; };
+    auto segment_phase = [&](int i) { return (i / kPromptSegments) & 1; };
+    auto release = [&](int i) {   // by every warp that reads segments
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(seg_empty(i));
     };
     auto needs = [&](const Segment &s, int h, int key) { return key <= s.last[h] && (key + kPromptKeys - 1 >= s.low[h] || key < a.sinks); };   // any row of the half, of a block of keys
 
@@ -229,62 +243,54 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         const int which = warp >> 1, t = threadIdx.x & 63;
         const uint32_t ring = which ? v_base : k_base;
         const int pieces = dim / 8, mask = (1 << a.pages.page_shift) - 1;
-        bool ok = true;
-        int n = 0, tile = 0;   // blocks and tiles so far
-        for (long long at = range.begin; at < range.end; ++tile) {
-            const Segment seg = segment_of(place, at);
-            // queries: all four warps, a row's pieces of eight side by side
-            ok = bounded_wait(q_empty, (tile & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);   // run out: the warps leave together, below
-            for (int i = threadIdx.x; ok && i < kPromptRows * 8 * NB; i += 128) {
-                const int r = i / (8 * NB), c = i % (8 * NB);
-                if (c >= 2 * steps) continue;
-                uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                if (r < seg.rows && c < pieces) {
-                    const int packed = seg.packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
-                    w = *reinterpret_cast<const uint4 *>(static_cast<const __nv_bfloat16 *>(a.q) + row * a.q_pitch + head * dim + c * 8);
-                }
-                ptx::sts128(q_base + (r >> 7) * S::kTile + (c >> 3) * kPromptBlock + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4), w.x, w.y, w.z, w.w);
-            }
-            ptx::fence_proxy_async_smem();
-            ptx::mbar_arrive(q_full);
+        int n = 0, tile = 0, b = 0;   // blocks and tiles so far, block of the tile's part
+        bool boxes = false;
+        // the rows that this block of keys comes from, two keys per thread
+        auto look_up = [&] {
+            const Segment &seg = segment(tile);
+            const int key0 = block_key(seg.keys, seg.from + b, kPromptKeys), turn = n & 1;
             const int low = a.window ? seg.first[0] - a.window + 1 : 0, p1 = max(seg.last[0], seg.last[1]);
-            for (int b = 0; b < seg.blocks; ++b, ++n) {
-                const int key0 = block_key(place.blocks, place.off + b, kPromptKeys), stage = n % S::kStages, turn = n & 1;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const int key = key0 + t + 64 * i;
-                    const bool wanted = key <= p1 && (key >= low || key < a.sinks);
-                    const int page = wanted ? page_of(a.batch, a.pages, place.s, key) : -1;
-                    const long long row = page >= 0 ? a.pages.place(page, which, place.g, key & mask) : -1;
-                    row_at[which][turn][t + 64 * i] = row >= 0 ? row * dim : -1;
-                    if (CODES) row_e[which][turn][t + 64 * i] = row >= 0 ? static_cast<int>(a.pages.scales[row]) - 127 : 0;
+            // wanted as a whole: whole boxes out of the pages, a thread each
+            boxes = !CODES && args.box_rows > 0 && key0 + kPromptKeys - 1 <= p1 && (key0 >= low || key0 + kPromptKeys <= a.sinks);
+            if (boxes) {
+                if (t * args.box_rows < kPromptKeys) {
+                    const int key = key0 + t * args.box_rows, page = page_of(a.batch, a.pages, seg.s, key);
+                    row_at[which][turn][t * args.box_rows] = a.pages.place(max(page, 0), which, seg.g, key & mask);
                 }
-                ok = ok && bounded_wait(which ? v_empty(stage) : k_empty(stage), ((n / S::kStages) & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);
-                if (!pro::all_of(2 + which, 64, ok)) {
-                    ok = false;
-                    break;
-                }
-                const uint32_t dst = ring + stage * S::kTile;
-                if constexpr (CODES) {
-                    const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
-                    constexpr int kPer = 8;
-                    // pieces of eight codes, kPer of them under way per thread
-                    for (int i0 = 0; i0 < kPromptKeys * 8 * NB / 64; i0 += kPer) {
-                        uint2 w[kPer];
+                return;
+            }
 #pragma unroll
-                        for (int u = 0; u < kPer; ++u) {
-                            const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
-                            const long long row = row_at[which][turn][r];
-                            w[u] = row >= 0 && c < pieces ? *reinterpret_cast<const uint2 *>(data + row + c * 8) : make_uint2(0u, 0u);
-                        }
+            for (int i = 0; i < 2; ++i) {
+                const int key = key0 + t + 64 * i;
+                const bool wanted = key <= p1 && (key >= low || key < a.sinks);
+                const int page = wanted ? page_of(a.batch, a.pages, seg.s, key) : -1;
+                const long long row = page >= 0 ? a.pages.place(page, which, seg.g, key & mask) : -1;
+                row_at[which][turn][t + 64 * i] = row;
+                if (CODES) row_e[which][turn][t + 64 * i] = row >= 0 ? static_cast<int>(a.pages.scales[row]) - 127 : 0;
+            }
+        };
+        // the two warps learn together whether there is another tile
+        auto another = [&] {
+            const bool ok = bounded_wait(seg_full(tile), segment_phase(tile), abort_flag, status, DEV_TIMEOUT_PRODUCER);
+            return pro::all_of(2 + which, 64, ok) && segment(tile).blocks > 0;
+        };
+        bool more = another();
+        if (more) look_up();
+        while (more) {
+            const int stage = n % S::kStages, turn = n & 1;
+            const bool first = b == 0, by_box = boxes;
+            const int packed0 = segment(tile).packed0, rows = segment(tile).rows, q_turn = tile & 1;
+            const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + segment(tile).row0 * a.q_pitch + segment(tile).g * a.share * dim;
+            const uint32_t full = which ? v_full(stage) : k_full(stage);
+            bool ok = bounded_wait(which ? v_empty(stage) : k_empty(stage), ((n / S::kStages) & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);
+            if (!pro::all_of(2 + which, 64, ok)) break;
+            const uint32_t dst = ring + stage * S::kTile;
+            if constexpr (!CODES) {
+                if (by_box) {
+                    if (t * args.box_rows < kPromptKeys) {
+                        const int page_row = static_cast<int>(row_at[which][turn][t * args.box_rows]);
 #pragma unroll
-                        for (int u = 0; u < kPer; ++u) {
-                            const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
-                            const int e = row_e[which][turn][r];
-                            const uint32_t power = (120 + min(e, 7) + 127) << 7, rest = e > 7 ? (e - 7 + 127) << 7 : 0;
-                            const uint2 x = pro::codes_to_bf16(w[u].x, power * 0x10001u, rest * 0x10001u), y = pro::codes_to_bf16(w[u].y, power * 0x10001u, rest * 0x10001u);
-                            if (c < 2 * steps) ptx::sts128(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
-                        }
+                        for (int c = 0; c < NB; ++c) ptx::tma_load_2d(dst + c * kPromptBlock + t * args.box_rows * 128, &args.map, 32 * c, page_row, full);
                     }
                 } else {
                     const __nv_bfloat16 *data = static_cast<const __nv_bfloat16 *>(a.pages.data);
@@ -293,16 +299,65 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         const int idx = i * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
                         const long long row = row_at[which][turn][r];
                         const bool on = row >= 0 && c < pieces;
-                        if (c < 2 * steps) tok::copy<16>(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? data + row + c * 8 : data, on);
+                        if (c < 2 * steps) tok::copy<16>(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? data + row * dim + c * 8 : data, on);
                     }
-                    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
                 }
-                ptx::fence_proxy_async_smem();
-                ptx::mbar_arrive(which ? v_full(stage) : k_full(stage));
             }
-            if (!ok) break;
-            at += seg.blocks;
-            if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            // on to the next block: its pages are looked up while this one's rows are on their way
+            ++n;
+            if (++b == segment(tile).blocks) {
+                b = 0;
+                release(tile++);
+                more = another();
+            }
+            if (more) look_up();
+            if constexpr (CODES) {
+                const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
+                constexpr int kPer = 8;
+                // pieces of eight codes, kPer of them under way per thread
+                for (int i0 = 0; i0 < kPromptKeys * 8 * NB / 64; i0 += kPer) {
+                    uint2 w[kPer];
+#pragma unroll
+                    for (int u = 0; u < kPer; ++u) {
+                        const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
+                        const long long row = row_at[which][turn][r];
+                        w[u] = row >= 0 && c < pieces ? *reinterpret_cast<const uint2 *>(data + row * dim + c * 8) : make_uint2(0u, 0u);
+                    }
+#pragma unroll
+                    for (int u = 0; u < kPer; ++u) {
+                        const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
+                        const int e = row_e[which][turn][r];
+                        const uint32_t power = (120 + min(e, 7) + 127) << 7, rest = e > 7 ? (e - 7 + 127) << 7 : 0;
+                        const uint2 x = pro::codes_to_bf16(w[u].x, power * 0x10001u, rest * 0x10001u), y = pro::codes_to_bf16(w[u].y, power * 0x10001u, rest * 0x10001u);
+                        if (c < 2 * steps) ptx::sts128(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                    }
+                }
+            }
+            if (by_box) {
+                if (t == 0)
+                    ptx::mbar_arrive_expect_tx(full, S::kTile);
+                else
+                    ptx::mbar_arrive(full);
+            } else {
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(full);
+            }
+            if (first) {   // queries, when the tile before has no more use for its own: all four warps, a row's pieces of eight side by side
+                ok = bounded_wait(q_empty, q_turn ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);   // run out: the warps leave together at the next block
+#pragma unroll 4
+                for (int i = threadIdx.x; ok && i < kPromptRows * 8 * NB; i += 128) {
+                    const int r = i / (8 * NB), c = i % (8 * NB), packed = packed0 + r, token = a.shares.divide(packed);
+                    const bool on = r < rows && c < pieces;
+                    if (c < 2 * steps)
+                        tok::copy<16>(q_base + (r >> 7) * S::kTile + (c >> 3) * kPromptBlock + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                                      on ? q + token * a.q_pitch + (packed - token * a.share) * dim + c * 8 : q, on);
+                }
+                asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+                ptx::fence_proxy_async_smem();
+                ptx::mbar_arrive(q_full);
+            }
         }
     } else if (warp < 8) {
         ptx::reg_dec<40>();
@@ -314,15 +369,18 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                                 dv = ptx::smem_desc_words(v_base, kPromptBlock, 1024, ptx::kLayoutSw128);
             auto wait = [&](uint32_t b, uint32_t parity, int code) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, code)); };
             bool ok = true;
-            int n = 0, tile = 0, turns[2] = {0, 0};
-            for (long long at = range.begin; ok && at < range.end; ++tile) {
-                const Segment seg = segment_of(place, at);
+            int n = 0, turns[2] = {0, 0};
+            for (int tile = 0; ok; ++tile) {
+                ok = wait(seg_full(tile), segment_phase(tile), DEV_TIMEOUT_MMA_FULL);
+                if (!ok) break;
+                const Segment &seg = segment(tile);
+                if (seg.blocks == 0) break;
                 bool begun[2] = {false, false}, wanted[2] = {false, false};
                 ok = wait(q_full, tile & 1, DEV_TIMEOUT_MMA_FULL);
                 for (int b = -1; ok && b < seg.blocks; ++b) {
                     const int vs = (n + b) % S::kStages, ks = (n + b + 1) % S::kStages;
                     const bool more = b + 1 < seg.blocks;
-                    const int next_key = more ? block_key(place.blocks, place.off + b + 1, kPromptKeys) : 0;
+                    const int next_key = more ? block_key(seg.keys, seg.from + b + 1, kPromptKeys) : 0;
                     if (b >= 0) ok = wait(v_full(vs), ((n + b) / S::kStages) & 1, DEV_TIMEOUT_MMA_FULL);
                     bool have_k = false;
 #pragma unroll
@@ -378,12 +436,52 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 }
                 if (!ok) break;
                 n += seg.blocks;
-                at += seg.blocks;
-                if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+                release(tile);
             }
             if (issuer) ptx::mma_commit(drain);
             __syncwarp();
             bounded_wait(drain, 0u, abort_flag, status, DEV_TIMEOUT_DRAIN);
+        } else if (warp == 5) {
+            int n = 0;
+            for (long long at = range.begin; at <= range.end;) {
+                Segment seg{};
+                if (at < range.end) {
+                    const Part part = part_of(place, range, at, args.cut);
+                    seg.blocks = part.blocks;
+                    seg.s = place.s;
+                    seg.g = place.g;
+                    seg.row0 = place.q.row0;
+                    seg.pos0 = place.q.pos0;
+                    seg.packed0 = place.tile * kPromptRows;
+                    seg.rows = min(kPromptRows, place.q.count * a.share - seg.packed0);
+                    seg.from = part.from;
+                    seg.keys = place.blocks;
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const bool there = h * 128 < seg.rows;
+                        seg.first[h] = there ? seg.pos0 + a.shares.divide(seg.packed0 + h * 128) : -1;
+                        seg.last[h] = there ? seg.pos0 + a.shares.divide(seg.packed0 + min(seg.rows, h * 128 + 128) - 1) : -1;
+                        seg.low[h] = a.window ? seg.first[h] - a.window + 1 : 0;
+                    }
+                    seg.whole = part.whole;
+                    seg.tail = part.first_block >= range.begin;
+                    if (!part.whole) {
+                        seg.b0 = static_cast<int>(part.first_block / range.per);
+                        seg.b1 = static_cast<int>(part.last_block / range.per);
+                    }
+                    at += part.places;
+                    if (at < range.end) next_tile(a, place, args.cut);
+                    if (seg.blocks == 0) continue;   // only the tile's own costs fell into this range
+                } else {
+                    ++at;   // behind the end: the last entry
+                }
+                if (!__all_sync(0xffffffffu, bounded_wait(seg_empty(n), segment_phase(n) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER))) break;
+                if (lane == 0) {
+                    segments[n % kPromptSegments] = seg;
+                    ptx::mbar_arrive(seg_full(n));
+                }
+                ++n;
+            }
         }
         __syncwarp();
     } else {
@@ -394,16 +492,18 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         const int r = quarter * 32 + lane;   // row within the half
         auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, DEV_TIMEOUT_EPILOGUE)); };
         bool ok = true;
-        int turns = 0, tile = 0;
-        for (long long at = range.begin; at < range.end; ++tile) {
-            const Segment seg = segment_of(place, at);
+        int turns = 0;
+        for (int tile = 0;; ++tile) {
+            if (!pro::all_of(4 + h, 128, wait(seg_full(tile), segment_phase(tile)))) break;
+            const Segment &seg = segment(tile);
+            if (seg.blocks == 0) break;
             const int packed = seg.packed0 + h * 128 + r;
             const bool there = h * 128 + r < seg.rows;
-            const int token = packed / a.share, position = there ? place.q.pos0 + token : -1;
+            const int token = a.shares.divide(packed), position = there ? seg.pos0 + token : -1;
             float ref = -INFINITY, sum = 0.0f;   // what the weights stand against (base 2), their sum
             bool begun = false;
             for (int b = 0; b < seg.blocks; ++b) {
-                const int key0 = block_key(place.blocks, place.off + b, kPromptKeys);
+                const int key0 = block_key(seg.keys, seg.from + b, kPromptKeys);
                 if (!needs(seg, h, key0)) continue;
                 ok = wait(s_full(h), turns & 1);
                 if (!ok) break;
@@ -415,10 +515,14 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(s_addr + 32 * c, x[c]);
                 ptx::tmem_ld_wait();
                 if (!whole) {
-                    const int high = position - key0, low = a.window ? high - a.window : -1, first = a.sinks - key0;
+                    // keys up to `high`, but only those from `low` on or before `first`: a bit per key
+                    const int high = position - key0, low = a.window ? high - a.window + 1 : 0, first = a.sinks - key0;
 #pragma unroll
-                    for (int i = 0; i < kPromptKeys; ++i)
-                        if (i > high || (i <= low && i >= first)) x[i >> 5][i & 31] = 0xff800000u;   // minus infinity
+                    for (int c = 0; c < 4; ++c) {
+                        const uint32_t seen = pro::bits_below(high + 1 - 32 * c) & (~pro::bits_below(low - 32 * c) | pro::bits_below(first - 32 * c));
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) x[c][i] = seen & (1u << i) ? x[c][i] : 0xff800000u;   // minus infinity
+                    }
                 }
                 bool near_zero = true;   // no score of the warp's rows beyond the cap: tanh is a polynomial
                 float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, least[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
@@ -501,50 +605,67 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             ptx::tc_fence_after();
             if (!pro::all_of(4 + h, 128, ok)) break;
             if (h * 128 < seg.rows) {
-                const long long first = at - place.off, last = first + place.blocks.count - 1;   // the tile's blocks on the line
-                const bool whole = place.off == 0 && seg.blocks == place.blocks.count;
                 const bool sees = position >= 0;
-                const int head = place.g * a.share + packed % a.share;
-                const long long row = place.q.row0 + token;
-                __nv_bfloat16 *dst = static_cast<__nv_bfloat16 *>(a.out) + row * a.out_pitch + head * dim;
-                bool fine = true;
-                auto store = [&](int c, const uint32_t (&o)[16], float by) {   // columns c .. c + 15
-                    uint32_t w[8];
+                const int head = seg.g * a.share + packed - token * a.share;
+                const long long row = seg.row0 + token;
+                // 32 columns of the warp's rows at a time go through shared memory, so that four lanes store a row's 64 bytes side by side
+                const uint32_t stage = staging + (4 * h + quarter) * 2048;
+                __nv_bfloat16 *to[4];
+                const int piece = lane & 3;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float u = __uint_as_float(o[2 * i]) * by, v = __uint_as_float(o[2 * i + 1]) * by;
-                        fine = fine && (c + 2 * i >= dim || (fabsf(u) <= FLT_MAX && fabsf(v) <= FLT_MAX));
+                for (int i = 0; i < 4; ++i) {
+                    const int rr = h * 128 + quarter * 32 + 8 * i + (lane >> 2), pr = seg.packed0 + rr, tk = a.shares.divide(pr);
+                    to[i] = rr < seg.rows ? static_cast<__nv_bfloat16 *>(a.out) + (seg.row0 + tk) * a.out_pitch + (seg.g * a.share + pr - tk * a.share) * dim + 8 * piece : nullptr;
+                }
+                float check = 0.0f;   // zero times every output: NaN where one is not finite
+                auto store = [&](int c, const float (&o)[32], float by) {   // columns c .. c + 31
+                    uint32_t w[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const float u = o[2 * i] * by, v = o[2 * i + 1] * by;
+                        if (c + 2 * i < dim) check = fmaf(v, 0.0f, fmaf(u, 0.0f, check));
                         w[i] = sees ? ptx::pack_bf16x2(u, v) : 0u;
                     }
-                    if (there && c < dim) *reinterpret_cast<uint4 *>(dst + c) = make_uint4(w[0], w[1], w[2], w[3]);
-                    if (there && c + 8 < dim) *reinterpret_cast<uint4 *>(dst + c + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ptx::sts128(stage + lane * 64 + ((i ^ ((lane >> 1) & 3)) << 4), w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int rr = 8 * i + (lane >> 2);
+                        const float4 v = ptx::lds128(stage + rr * 64 + ((piece ^ ((rr >> 1) & 3)) << 4));
+                        if (to[i] && c + 8 * piece < dim) *reinterpret_cast<float4 *>(to[i] + c) = v;
+                    }
+                    __syncwarp();
                 };
                 auto store_sum = [&](float top, float total) {
                     if (a.lse && there) a.lse[row * a.heads + head] = sees ? top * kLn2 + logf(total) : -INFINITY;
                 };
-                bool done = whole;
-                if (whole) {
+                bool done = seg.whole;
+                if (seg.whole) {
                     const float by = 1.0f / sum;
-                    for (int c = 0; c < 16 * steps; c += 16) {
-                        uint32_t o[16];
-                        pro::tmem_ld_32x16(o_addr + c, o);
+                    for (int c = 0; c < 16 * steps; c += 32) {
+                        uint32_t o[32];
+                        ptx::tmem_ld_32x32(o_addr + c, o);
                         ptx::tmem_ld_wait();
-                        store(c, o, by);
+                        float v[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
+                        store(c, v, by);
                     }
                     store_sum(ref, sum);
                 } else {
                     // four columns of all rows side by side, so that the rows' threads write and read runs
-                    float *part = args.parts.base + (2LL * blockIdx.x + (first >= range.begin)) * args.parts.floats + h * (128 * 128 + 256);
-                    for (int c = 0; c < 16 * steps; c += 16) {
-                        uint32_t o[16];
-                        pro::tmem_ld_32x16(o_addr + c, o);
+                    float *part = args.parts.base + (2LL * blockIdx.x + seg.tail) * args.parts.floats + h * (128 * 128 + 256);
+                    for (int c = 0; c < 16 * steps; c += 32) {
+                        uint32_t o[32];
+                        ptx::tmem_ld_32x32(o_addr + c, o);
                         ptx::tmem_ld_wait();
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 8; ++i)
                             *reinterpret_cast<uint4 *>(part + ((c / 4 + i) * 128 + r) * 4) = begun ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0u, 0u, 0u, 0u);
                     }
                     *reinterpret_cast<float2 *>(part + 128 * 128 + 2 * r) = make_float2(ref, sum);
-                    const int b0 = static_cast<int>(first / range.per), b1 = static_cast<int>(last / range.per);
+                    const int b0 = seg.b0, b1 = seg.b1;
                     __threadfence();
                     pro::all_of(4 + h, 128, true);
                     if (r == 0) {
@@ -564,22 +685,19 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                             total = fmaf(ml.y, tok::share_of(ml.x, top), total);
                         }
                         const float by = 1.0f / total;
-                        for (int c = 0; c < 16 * steps; c += 16) {
-                            float v[16] = {};
+                        for (int c = 0; c < 16 * steps; c += 32) {
+                            float v[32] = {};
                             for (int b = b0; b <= b1; ++b) {
                                 const float *from = slot(b);
                                 const float f = tok::share_of(__ldcg(from + 128 * 128 + 2 * r), top);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
+                                for (int i = 0; i < 8; ++i) {
                                     const float4 u = __ldcg(reinterpret_cast<const float4 *>(from + ((c / 4 + i) * 128 + r) * 4));
                                     v[4 * i] = fmaf(u.x, f, v[4 * i]); v[4 * i + 1] = fmaf(u.y, f, v[4 * i + 1]);
                                     v[4 * i + 2] = fmaf(u.z, f, v[4 * i + 2]); v[4 * i + 3] = fmaf(u.w, f, v[4 * i + 3]);
                                 }
                             }
-                            uint32_t o[16];
-#pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(v[i]);
-                            store(c, o, by);
+                            store(c, v, by);
                         }
                         store_sum(top, total);
                     }
@@ -587,18 +705,21 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is
                 // formed once more from its own keys alone.
                 __syncwarp();
-                for (uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && !fine); bad; bad &= bad - 1) {
+                for (uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && check != 0.0f); bad; bad &= bad - 1) {
                     const int p = seg.packed0 + h * 128 + quarter * 32 + __ffs(bad) - 1;
-                    attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + p / a.share, place.q.row0 + p / a.share, place.g * a.share + p % a.share, lane);
+                    attention_row<__nv_bfloat16, kind>(a, seg.s, seg.pos0 + a.shares.divide(p), seg.row0 + a.shares.divide(p), seg.g * a.share + p - a.shares.divide(p) * a.share, lane);
                 }
             }
             ptx::tc_fence_before();   // the accumulator has been read: the next tile's products may write it (they wait for its weights)
-            at += seg.blocks;
-            if (at < range.end && !next_tile(a, place, kPromptRows, kPromptKeys)) break;
+            release(tile);
         }
     }
 
     ptx::tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        for (int i = 0; i < 64; ++i) __nanosleep(1000);   // copies still in flight land before the memory is handed on
+    }
     __syncthreads();
     if (warp == 4) {
         ptx::tc_fence_after();

@@ -112,7 +112,7 @@ __device__ __forceinline__ void lds_words(uint32_t (&v)[WORDS], uint32_t addr)
 struct TokensArgs {
     Attention a;
     Parts parts;
-    int least;        // blocks of the line per block of the grid, at least
+    Cut cut;
 };
 
 template <int D16, bool CODES>
@@ -131,7 +131,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     grid_dependency_launch();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
     Place place;
-    Range range = range_of_block<kTokensThreads>(a, kTokensRows, kTokensKeys, args.least, place);
+    Range range = range_of_block<kTokensThreads>(a, args.cut, place);
     const uint32_t q_tile = ptx::smem_u32(tokens_smem), ring = q_tile + kTokensRows * S::kQPitch + warp * S::kStages * S::kStage;
     const int dim = a.pages.dim, pieces = dim / 8;
     // a head narrower than the padded width: its tail columns stay zero
@@ -142,12 +142,17 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     };
 
     for (long long at = range.begin; at < range.end;) {
-        const int n_blocks = static_cast<int>(min(static_cast<long long>(place.blocks.count - place.off), range.end - at));
-        const bool whole = place.off == 0 && n_blocks == place.blocks.count;
+        const Part part = part_of(place, range, at, args.cut);
+        at += part.places;
+        if (part.blocks == 0) {
+            if (at < range.end && !next_tile(a, place, args.cut)) break;
+            continue;
+        }
+        const int n_blocks = part.blocks;
         const int packed0 = place.tile * kTokensRows, rows = min(kTokensRows, place.q.count * a.share - packed0);
-        const int p0 = place.q.pos0 + packed0 / a.share, p1 = place.q.pos0 + (packed0 + rows - 1) / a.share;
+        const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1);
         const int low = a.window ? p0 - a.window + 1 : 0;   // keys below it are visible only among the first ones
-        auto tile_key = [&](int i) { return block_key(place.blocks, place.off + i, kTokensKeys) + warp * 16; };
+        auto tile_key = [&](int i) { return block_key(place.blocks, part.from + i, kTokensKeys) + warp * 16; };
         auto wanted = [&](int key) { return key <= p1 && (key >= low || key < a.sinks); };   // by any row of the tile
 
         // ---- the ring
@@ -220,7 +225,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             const int c = threadIdx.x & 15;
             float v[8] = {};
             if (r < rows && c < pieces) {
-                const int packed = packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
+                const int packed = packed0 + r, row = place.q.row0 + a.shares.divide(packed), head = place.g * a.share + packed - a.shares.divide(packed) * a.share;
                 load8(v, static_cast<const __nv_bfloat16 *>(a.q) + row * a.q_pitch + head * dim + c * 8);
             }
             uint32_t w[4];
@@ -261,7 +266,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const int r = g8 + 8 * i;
-            pos[i] = r < rows ? place.q.pos0 + (packed0 + r) / a.share : -1;
+            pos[i] = r < rows ? place.q.pos0 + a.shares.divide(packed0 + r) : -1;
             to_score[i] = a.scale * (CODES ? row_power[r] : 1.0f);
         }
 
@@ -433,8 +438,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         }
         __syncthreads();
         auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
-            const int packed = packed0 + r, row = place.q.row0 + packed / a.share, head = place.g * a.share + packed % a.share;
-            const bool sees = place.q.pos0 + packed / a.share >= 0;   // itself at least
+            const int packed = packed0 + r, row = place.q.row0 + a.shares.divide(packed), head = place.g * a.share + packed - a.shares.divide(packed) * a.share;
+            const bool sees = place.q.pos0 + a.shares.divide(packed) >= 0;   // itself at least
             const float inv = sees ? 1.0f / sum : 0.0f;
             bool fine = true;
 #pragma unroll
@@ -446,8 +451,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             store8(static_cast<__nv_bfloat16 *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
             if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
         };
-        const long long first = at - place.off, last = first + place.blocks.count - 1;   // the tile's blocks on the line
-        float *part = args.parts.base + (2LL * blockIdx.x + (first >= range.begin)) * args.parts.floats;
+        float *slot_own = args.parts.base + (2LL * blockIdx.x + (part.first_block >= range.begin)) * args.parts.floats;
         for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
             const int r = i / pieces, c = i % pieces;
             float v[8] = {};
@@ -458,15 +462,15 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += u[e];
             }
-            if (whole) {
+            if (part.whole) {
                 finish(r, c, v, total_ml[r][0], total_ml[r][1]);
             } else {
-                store8(part + r * dim + c * 8, v);
-                if (c == 0) *reinterpret_cast<float2 *>(part + kTokensRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
+                store8(slot_own + r * dim + c * 8, v);
+                if (c == 0) *reinterpret_cast<float2 *>(slot_own + kTokensRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
             }
         }
-        if (!whole) {
-            const int b0 = static_cast<int>(first / range.per), b1 = static_cast<int>(last / range.per);
+        if (!part.whole) {
+            const int b0 = static_cast<int>(part.first_block / range.per), b1 = static_cast<int>(part.last_block / range.per);
             __threadfence();
             __syncthreads();
             if (threadIdx.x == 0) {
@@ -502,11 +506,10 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         for (int rest = bad_rows, n = 0; rest; rest &= rest - 1, ++n) {
             if (n % kTokensWarps != warp) continue;
             const int packed = packed0 + __ffs(rest) - 1;
-            attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + packed / a.share, place.q.row0 + packed / a.share, place.g * a.share + packed % a.share, lane);
+            attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + a.shares.divide(packed), place.q.row0 + a.shares.divide(packed), place.g * a.share + packed - a.shares.divide(packed) * a.share, lane);
         }
         __syncthreads();   // what the next tile writes again has been read
-        at += n_blocks;
-        if (at < range.end && !next_tile(a, place, kTokensRows, kTokensKeys)) break;
+        if (at < range.end && !next_tile(a, place, args.cut)) break;
     }
 }
 
