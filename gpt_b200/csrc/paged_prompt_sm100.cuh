@@ -185,10 +185,11 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
     auto s_full = [&](int h) { return bar + 8u * (12 + h); };
     auto p_full = [&](int h) { return bar + 8u * (14 + h); };
     auto o_full = [&](int h) { return bar + 8u * (16 + h); };
-    const uint32_t q_full = bar + 8u * 18, q_empty = bar + 8u * 19, drain = bar + 8u * 20;
-    auto seg_full = [&](int i) { return bar + 8u * (21 + i % kPromptSegments); };
-    auto seg_empty = [&](int i) { return bar + 8u * (21 + kPromptSegments + i % kPromptSegments); };
-    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + (bar - base) + 8 * (21 + 2 * kPromptSegments));
+    auto p_half = [&](int h) { return bar + 8u * (18 + h); };
+    const uint32_t q_full = bar + 8u * 20, q_empty = bar + 8u * 21, drain = bar + 8u * 22;
+    auto seg_full = [&](int i) { return bar + 8u * (23 + i % kPromptSegments); };
+    auto seg_empty = [&](int i) { return bar + 8u * (23 + kPromptSegments + i % kPromptSegments); };
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(gen + (bar - base) + 8 * (23 + 2 * kPromptSegments));
     volatile uint32_t *abort_flag = tmem_slot + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *status = a.batch.status;
@@ -202,6 +203,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         }
         for (int h = 0; h < 2; ++h) {
             ptx::mbar_init(s_full(h), 1);
+            ptx::mbar_init(p_half(h), 128);
             ptx::mbar_init(p_full(h), 128);
             ptx::mbar_init(o_full(h), 1);
         }
@@ -313,24 +315,45 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             }
             if (more) look_up();
             if constexpr (CODES) {
+                // pieces of sixteen codes (two of eight where rows begin at odd multiples of eight); four are on their way while the four before become bf16
                 const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
-                constexpr int kPer = 8;
-                // pieces of eight codes, kPer of them under way per thread
-                for (int i0 = 0; i0 < kPromptKeys * 8 * NB / 64; i0 += kPer) {
-                    uint2 w[kPer];
+                constexpr int kPer = 4, kBatches = kPromptKeys * 4 * NB / 64 / kPer;
+                const bool wide = dim % 16 == 0;
+                const int c = t % (4 * NB), r0 = t / (4 * NB);   // the thread's columns 16 c .. 16 c + 15 of every (64 / 4 NB)-th row
+                const bool low_on = c * 16 < dim, high_on = c * 16 + 8 < dim;
+                uint4 w[2][kPer];
+                auto load = [&](int batch, uint4 (&to)[kPer]) {
 #pragma unroll
                     for (int u = 0; u < kPer; ++u) {
-                        const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
-                        const long long row = row_at[which][turn][r];
-                        w[u] = row >= 0 && c < pieces ? *reinterpret_cast<const uint2 *>(data + row * dim + c * 8) : make_uint2(0u, 0u);
+                        const long long row = row_at[which][turn][r0 + (batch * kPer + u) * (16 / NB)];
+                        const uint8_t *from = data + row * dim + c * 16;
+                        to[u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (row >= 0 && wide && low_on) {
+                            to[u] = *reinterpret_cast<const uint4 *>(from);
+                        } else if (row >= 0 && !wide) {
+                            if (low_on) *reinterpret_cast<uint2 *>(&to[u].x) = *reinterpret_cast<const uint2 *>(from);
+                            if (high_on) *reinterpret_cast<uint2 *>(&to[u].z) = *reinterpret_cast<const uint2 *>(from + 8);
+                        }
                     }
+                };
+                load(0, w[0]);
+#pragma unroll
+                for (int batch = 0; batch < kBatches; ++batch) {
+                    if (batch + 1 < kBatches) load(batch + 1, w[(batch + 1) & 1]);
 #pragma unroll
                     for (int u = 0; u < kPer; ++u) {
-                        const int idx = (i0 + u) * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
-                        const int e = row_e[which][turn][r];
-                        const uint32_t power = (120 + min(e, 7) + 127) << 7, rest = e > 7 ? (e - 7 + 127) << 7 : 0;
-                        const uint2 x = pro::codes_to_bf16(w[u].x, power * 0x10001u, rest * 0x10001u), y = pro::codes_to_bf16(w[u].y, power * 0x10001u, rest * 0x10001u);
-                        if (c < 2 * steps) ptx::sts128(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                        const int r = r0 + (batch * kPer + u) * (16 / NB), e = row_e[which][turn][r];
+                        const uint32_t power = ((120 + min(e, 7) + 127) << 7) * 0x10001u, rest = e > 7 ? ((e - 7 + 127) << 7) * 0x10001u : 0u;
+                        const uint4 v = w[batch & 1][u];
+                        const uint32_t at = dst + (c >> 2) * kPromptBlock + r * 128;
+                        if (2 * c < 2 * steps) {
+                            const uint2 x = pro::codes_to_bf16(v.x, power, rest), y = pro::codes_to_bf16(v.y, power, rest);
+                            ptx::sts128(at + (((2 * c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                        }
+                        if (2 * c + 1 < 2 * steps) {
+                            const uint2 x = pro::codes_to_bf16(v.z, power, rest), y = pro::codes_to_bf16(v.w, power, rest);
+                            ptx::sts128(at + (((2 * c + 1 & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                        }
                     }
                 }
             }
@@ -386,18 +409,19 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         if (ok && b >= 0 && wanted[h]) {
-                            ok = wait(p_full(h), turns[h] & 1, DEV_TIMEOUT_MMA_TMEM);
-                            if (!ok) break;
-                            ptx::tc_fence_after();
-                            if (issuer) {
-                                uint32_t acc = begun[h];
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    pro::mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 8 * k, dv.at(vs * S::kTile + k * 2048), idesc_o, acc);
-                                    acc = 1;
+                            for (int part = 0; part < 2; ++part) {
+                                if (ok) ok = wait(part ? p_full(h) : p_half(h), turns[h] & 1, DEV_TIMEOUT_MMA_TMEM);
+                                if (!ok) break;
+                                ptx::tc_fence_after();
+                                if (issuer) {
+#pragma unroll
+                                    for (int k = 4 * part; k < 4 * part + 4; ++k)
+                                        pro::mma_ts(tmem + 256 + 128 * h, tmem + 128 * h + 8 * k, dv.at(vs * S::kTile + k * 2048), idesc_o, k > 0 || begun[h]);
                                 }
+                                __syncwarp();
                             }
-                            __syncwarp();
+                            if (!ok) break;
                             begun[h] = true;
                             turns[h]++;
                         }
@@ -514,6 +538,37 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(s_addr + 32 * c, x[c]);
                 ptx::tmem_ld_wait();
+                if (CAPPED) {
+                    // no score of the warp's rows beyond the cap: tanh is a polynomial; else the scores go through TMEM once more, 32 at a time (rare, and little code)
+                    float widest[4] = {};
+#pragma unroll
+                    for (int i = 0; i < kPromptKeys; ++i) widest[i & 3] = fmaxf(widest[i & 3], fabsf(__uint_as_float(x[i >> 5][i & 31])));
+                    const float most = fmaxf(fmaxf(widest[0], widest[1]), fmaxf(widest[2], widest[3]));
+                    if (__all_sync(0xffffffffu, most * args.cap_arg <= 1.0f)) {
+#pragma unroll
+                        for (int i = 0; i < kPromptKeys; i += 2) {
+                            float u, v;
+                            const unsigned long long t = ptx::mul2(pro::pair(__uint_as_float(x[i >> 5][i & 31]), __uint_as_float(x[i >> 5][(i & 31) + 1])), ptx::both(args.cap_arg));
+                            pro::unpair(ptx::mul2(pro::tanh_inner2(t), ptx::both(args.cap_log2)), u, v);
+                            x[i >> 5][i & 31] = __float_as_uint(u);
+                            x[i >> 5][(i & 31) + 1] = __float_as_uint(v);
+                        }
+                    } else {
+#pragma unroll 1
+                        for (int c = 0; c < 8; ++c) {
+                            uint32_t y[16];
+                            pro::tmem_ld_32x16(s_addr + 16 * c, y);
+                            ptx::tmem_ld_wait();
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(pro::capped(__uint_as_float(y[i]) * args.cap_arg, args.cap_log2));
+                            pro::tmem_st_32x16(s_addr + 16 * c, y);
+                        }
+                        pro::tmem_st_wait();
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(s_addr + 32 * c, x[c]);
+                        ptx::tmem_ld_wait();
+                    }
+                }
                 if (!whole) {
                     // keys up to `high`, but only those from `low` on or before `first`: a bit per key
                     const int high = position - key0, low = a.window ? high - a.window + 1 : 0, first = a.sinks - key0;
@@ -524,22 +579,12 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         for (int i = 0; i < 32; ++i) x[c][i] = seen & (1u << i) ? x[c][i] : 0xff800000u;   // minus infinity
                     }
                 }
-                bool near_zero = true;   // no score of the warp's rows beyond the cap: tanh is a polynomial
-                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, least[4] = {INFINITY, INFINITY, INFINITY, INFINITY};
+                float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int i = 0; i < kPromptKeys; ++i) {
-                    const float v = __uint_as_float(x[i >> 5][i & 31]);
-                    most[i & 3] = fmaxf(most[i & 3], v);
-                    if (CAPPED) least[i & 3] = fminf(least[i & 3], v == -INFINITY ? 0.0f : v);
-                }
+                for (int i = 0; i < kPromptKeys; i += 2)
+                    most[(i >> 1) & 3] = fmaxf(fmaxf(most[(i >> 1) & 3], __uint_as_float(x[i >> 5][i & 31])), __uint_as_float(x[i >> 5][(i & 31) + 1]));
                 float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                if (CAPPED) {
-                    const float down = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
-                    near_zero = __all_sync(0xffffffffu, fmaxf(top, -down) * args.cap_arg <= 1.0f);
-                    if (top > -INFINITY) top = pro::capped(top * args.cap_arg, args.cap_log2);
-                } else {
-                    top *= args.scale_log2;
-                }
+                if (!CAPPED) top *= args.scale_log2;
                 const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
                 if (!begun) {
                     ref = top;
@@ -548,6 +593,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     const float f = grow ? tok::exp2_fast(ref - top) : 1.0f;
                     if (grow) ref = top;
                     sum *= f;
+#pragma unroll 1
                     for (int c = 0; c < 16 * steps; c += 16) {
                         uint32_t o[16];
                         pro::tmem_ld_32x16(o_addr + c, o);
@@ -559,38 +605,27 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 }
                 begun = true;
                 const float use = ref == -INFINITY ? 0.0f : ref;   // nothing seen yet: every weight is 2^-inf = 0
-                const unsigned long long scale2 = ptx::both(CAPPED ? args.cap_arg : args.scale_log2), minus_ref = ptx::both(-use);
+                const unsigned long long scale2 = ptx::both(args.scale_log2), minus_ref = ptx::both(-use);
                 unsigned long long sums[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t w[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float s0 = __uint_as_float(x[c][2 * i]), s1 = __uint_as_float(x[c][2 * i + 1]);
+                        const unsigned long long v = pro::pair(__uint_as_float(x[c][2 * i]), __uint_as_float(x[c][2 * i + 1]));
                         float e0, e1;
-                        if (!CAPPED) {
-                            pro::unpair(ptx::fma2(pro::pair(s0, s1), scale2, minus_ref), e0, e1);
-                        } else if (near_zero) {
-                            // the polynomial of a hidden score (minus infinity) is NaN: hidden again below
-                            pro::unpair(ptx::fma2(pro::tanh_inner2(ptx::mul2(pro::pair(s0, s1), scale2)), ptx::both(args.cap_log2), minus_ref), e0, e1);
-                            if (!whole) {
-                                if (s0 == -INFINITY) e0 = -INFINITY;
-                                if (s1 == -INFINITY) e1 = -INFINITY;
-                            }
-                        } else {
-                            e0 = pro::capped(s0 * args.cap_arg, args.cap_log2) - use;
-                            e1 = pro::capped(s1 * args.cap_arg, args.cap_log2) - use;
-                            if (!whole) {
-                                if (s0 == -INFINITY) e0 = -INFINITY;
-                                if (s1 == -INFINITY) e1 = -INFINITY;
-                            }
-                        }
+                        pro::unpair(CAPPED ? ptx::add2(v, minus_ref) : ptx::fma2(v, scale2, minus_ref), e0, e1);
                         e0 = tok::exp2_fast(e0);
                         e1 = tok::exp2_fast(e1);
                         sums[i & 1] = ptx::add2(sums[i & 1], pro::pair(e0, e1));
                         w[i] = ptx::pack_bf16x2(e0, e1);
                     }
                     pro::tmem_st_32x16(s_addr + 16 * c, w);
+                    if (c == 1) {   // the first 64 keys' weights: their products may begin
+                        pro::tmem_st_wait();
+                        ptx::tc_fence_before();
+                        ptx::mbar_arrive(p_half(h));
+                    }
                 }
                 {
                     float e0, e1;
