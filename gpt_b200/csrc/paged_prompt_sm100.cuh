@@ -5,8 +5,9 @@
 //   softmax     a thread per row: the row's scores in registers, running reference and sum in fp32; weights go back to TMEM over S, rounded to bf16 (eight bits:
 //               the output has no more; the sum is that of the unrounded weights, as the logarithm of the sum needs it)
 //   O += P V    tcgen05.mma with P from TMEM and V from shared memory as stored (MN-major)
-// The halves take turns on the tensor pipe: while one is in softmax the other's products run.  O is scaled only when a row's maximum has grown by more than 2^8
-// since the last time.  The grid is one block per SM, each with an equal range of the line; queries of the next tile are fetched while the last one is stored.
+// The halves take turns on the tensor pipe: while one is in softmax the other's products run.  O is scaled only when a row's maximum has grown by more than
+// 2^32 since the last time: weights of bf16 have fp32's exponents, so that neither they nor their sums leave the range before (with a limit of 2^8 a third of the blocks
+// of a prompt with uneven keys paid 1 200 cycles for it).  The grid is one block per SM, each with an equal range of the line; queries of the next tile are fetched while the last one is stored.
 //
 //   warps 0-1, 2-3   keys, values (named barriers 2 and 3): pages are looked up per key, rows come by asynchronous 16-byte copies into the swizzled layout that the tensor core reads (a
 //                    page is as small as eight tokens; an e4m3 row goes through registers and becomes bf16 there, exactly); all four fetch queries
@@ -120,32 +121,35 @@ __device__ __forceinline__ unsigned long long tanh_inner2(unsigned long long x)
     return ptx::mul2(p, x);
 }
 
-// Four codes as four bf16 values times a power of two.  A code's bits in a bf16's place (exponent and mantissa side by side) stand for code * 2^-120, subnormal
-// ones among them; one product by 2^(120 + e) puts them right, exactly (e up to 7; the rest, for values beyond 57344, in a second one).
+// Eight codes as bf16 values times a power of two.  A code's bits in a bf16's place (exponent and mantissa side by side) stand for code * 2^-120, subnormal
+// ones among them; one product by 2^(120 + e) puts them right, exactly, for e up to 7 (values up to 57344).
 __device__ __forceinline__ uint32_t bf16_mul(uint32_t a, uint32_t b)
 {
     uint32_t d;
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
 }
-__device__ __forceinline__ uint2 codes_to_bf16(uint32_t w, uint32_t power, uint32_t power_rest)
+__device__ __forceinline__ uint4 codes8_to_bf16(uint2 w, uint32_t power)
 {
-    uint32_t even = ((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u), odd = ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u);   // codes 0, 2 and 1, 3
-    even = bf16_mul(even, power);
-    odd = bf16_mul(odd, power);
-    if (power_rest) {
-        even = bf16_mul(even, power_rest);
-        odd = bf16_mul(odd, power_rest);
+    const uint32_t e0 = bf16_mul(((w.x << 4) & 0x07f007f0u) | ((w.x << 8) & 0x80008000u), power), o0 = bf16_mul(((w.x >> 4) & 0x07f007f0u) | (w.x & 0x80008000u), power);
+    const uint32_t e1 = bf16_mul(((w.y << 4) & 0x07f007f0u) | ((w.y << 8) & 0x80008000u), power), o1 = bf16_mul(((w.y >> 4) & 0x07f007f0u) | (w.y & 0x80008000u), power);
+    return make_uint4(__byte_perm(e0, o0, 0x5410), __byte_perm(e0, o0, 0x7632), __byte_perm(e1, o1, 0x5410), __byte_perm(e1, o1, 0x7632));
+}
+// A bit set: one of sixteen codes is the format's NaN (all bits but the sign).
+__device__ __forceinline__ uint32_t nan_among(const uint4 &w)
+{
+    return (((w.x & 0x7f7f7f7fu) + 0x01010101u) | ((w.y & 0x7f7f7f7fu) + 0x01010101u) | ((w.z & 0x7f7f7f7fu) + 0x01010101u) | ((w.w & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u;
+}
+// The same for what is rare: exponents from 8 on, NaN.
+__device__ __noinline__ uint4 codes8_to_bf16_any(uint2 w, float scale)
+{
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = codes2((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
+        r[i] = ptx::pack_bf16x2(v.x * scale, v.y * scale);
     }
-    // the format's NaN: all bits but the sign set
-    const uint32_t nan = (w & 0x7f7f7f7fu) + 0x01010101u;
-    if (nan & 0x80808080u) {
-        if (nan & 0x00000080u) even |= 0x00007fffu;
-        if (nan & 0x00008000u) odd |= 0x00007fffu;
-        if (nan & 0x00800000u) even |= 0x7fff0000u;
-        if (nan & 0x80000000u) odd |= 0x7fff0000u;
-    }
-    return make_uint2(__byte_perm(even, odd, 0x5410), __byte_perm(even, odd, 0x7632));
+    return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
 }  // namespace pro
@@ -160,6 +164,7 @@ struct Segment {
     bool whole, tail;         // all of the tile's blocks; the tile begins in this range
     int b0, b1;               // blocks of the grid that share the tile
 };
+constexpr float kPromptGrowth = 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled
 constexpr int kPromptSegments = 4, kPromptSegmentWarps = 13;   // ring; warps that read it
 
 template <int NB, bool CODES, bool CAPPED>
@@ -343,17 +348,15 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
 #pragma unroll
                     for (int u = 0; u < kPer; ++u) {
                         const int r = r0 + (batch * kPer + u) * (16 / NB), e = row_e[which][turn][r];
-                        const uint32_t power = ((120 + min(e, 7) + 127) << 7) * 0x10001u, rest = e > 7 ? ((e - 7 + 127) << 7) * 0x10001u : 0u;
                         const uint4 v = w[batch & 1][u];
-                        const uint32_t at = dst + (c >> 2) * kPromptBlock + r * 128;
-                        if (2 * c < 2 * steps) {
-                            const uint2 x = pro::codes_to_bf16(v.x, power, rest), y = pro::codes_to_bf16(v.y, power, rest);
-                            ptx::sts128(at + (((2 * c & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
+                        const uint32_t at = dst + (c >> 2) * kPromptBlock + r * 128, power = ((120 + min(e, 7) + 127) << 7) * 0x10001u;
+                        uint4 x = pro::codes8_to_bf16(make_uint2(v.x, v.y), power), y = pro::codes8_to_bf16(make_uint2(v.z, v.w), power);
+                        if (e > 7 || pro::nan_among(v)) {
+                            x = pro::codes8_to_bf16_any(make_uint2(v.x, v.y), scale_of(e + 127));
+                            y = pro::codes8_to_bf16_any(make_uint2(v.z, v.w), scale_of(e + 127));
                         }
-                        if (2 * c + 1 < 2 * steps) {
-                            const uint2 x = pro::codes_to_bf16(v.z, power, rest), y = pro::codes_to_bf16(v.w, power, rest);
-                            ptx::sts128(at + (((2 * c + 1 & 7) ^ (r & 7)) << 4), x.x, x.y, y.x, y.y);
-                        }
+                        if (2 * c < 2 * steps) ptx::sts128(at + (((2 * c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+                        if (2 * c + 1 < 2 * steps) ptx::sts128(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), y.x, y.y, y.z, y.w);
                     }
                 }
             }
@@ -526,14 +529,17 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             const int token = a.shares.divide(packed), position = there ? seg.pos0 + token : -1;
             float ref = -INFINITY, sum = 0.0f;   // what the weights stand against (base 2), their sum
             bool begun = false;
-            for (int b = 0; b < seg.blocks; ++b) {
-                const int key0 = block_key(seg.keys, seg.from + b, kPromptKeys);
-                if (!needs(seg, h, key0)) continue;
+            const int blocks = seg.blocks, half_first = seg.first[h], half_last = seg.last[h], half_low = seg.low[h];
+            const KeyBlocks keys = seg.keys;
+            int index = seg.from;
+            for (int b = 0; b < blocks; ++b, ++index) {
+                const int key0 = block_key(keys, index, kPromptKeys);
+                if (key0 > half_last || (key0 + kPromptKeys - 1 < half_low && key0 >= a.sinks)) continue;   // not needed, as below
                 ok = wait(s_full(h), turns & 1);
                 if (!ok) break;
                 ptx::tc_fence_after();
                 turns++;
-                const bool whole = key0 + kPromptKeys - 1 <= seg.first[h] && (a.window == 0 || key0 > seg.last[h] - a.window || key0 + kPromptKeys - 1 < a.sinks);
+                const bool whole = key0 + kPromptKeys - 1 <= half_first && (a.window == 0 || key0 > half_last - a.window || key0 + kPromptKeys - 1 < a.sinks);
                 uint32_t x[4][32];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32(s_addr + 32 * c, x[c]);
@@ -585,7 +591,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     most[(i >> 1) & 3] = fmaxf(fmaxf(most[(i >> 1) & 3], __uint_as_float(x[i >> 5][i & 31])), __uint_as_float(x[i >> 5][(i & 31) + 1]));
                 float top = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                 if (!CAPPED) top *= args.scale_log2;
-                const bool grow = top > ref + 8.0f || (ref == -INFINITY && top > -INFINITY);
+                const bool grow = top > ref + kPromptGrowth || (ref == -INFINITY && top > -INFINITY);
                 if (!begun) {
                     ref = top;
                 } else if (__any_sync(0xffffffffu, grow)) {
@@ -636,22 +642,23 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 ptx::tc_fence_before();
                 ptx::mbar_arrive(p_full(h));
             }
+            // where the outputs go, while the last products run
+            const bool sees = position >= 0;
+            const int head = seg.g * a.share + packed - token * a.share, piece = lane & 3;
+            const long long row = seg.row0 + token;
+            const uint32_t stage = staging + (4 * h + quarter) * 2048;
+            __nv_bfloat16 *to[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int rr = h * 128 + quarter * 32 + 8 * i + (lane >> 2), pr = seg.packed0 + rr, tk = a.shares.divide(pr);
+                to[i] = rr < seg.rows ? static_cast<__nv_bfloat16 *>(a.out) + (seg.row0 + tk) * a.out_pitch + (seg.g * a.share + pr - tk * a.share) * dim + 8 * piece : nullptr;
+            }
+            const float by_whole = 1.0f / sum;
             if (ok) ok = wait(o_full(h), tile & 1);
             ptx::tc_fence_after();
             if (!pro::all_of(4 + h, 128, ok)) break;
             if (h * 128 < seg.rows) {
-                const bool sees = position >= 0;
-                const int head = seg.g * a.share + packed - token * a.share;
-                const long long row = seg.row0 + token;
                 // 32 columns of the warp's rows at a time go through shared memory, so that four lanes store a row's 64 bytes side by side
-                const uint32_t stage = staging + (4 * h + quarter) * 2048;
-                __nv_bfloat16 *to[4];
-                const int piece = lane & 3;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int rr = h * 128 + quarter * 32 + 8 * i + (lane >> 2), pr = seg.packed0 + rr, tk = a.shares.divide(pr);
-                    to[i] = rr < seg.rows ? static_cast<__nv_bfloat16 *>(a.out) + (seg.row0 + tk) * a.out_pitch + (seg.g * a.share + pr - tk * a.share) * dim + 8 * piece : nullptr;
-                }
                 float check = 0.0f;   // zero times every output: NaN where one is not finite
                 auto store = [&](int c, const float (&o)[32], float by) {   // columns c .. c + 31
                     uint32_t w[16];
@@ -677,7 +684,6 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 };
                 bool done = seg.whole;
                 if (seg.whole) {
-                    const float by = 1.0f / sum;
                     for (int c = 0; c < 16 * steps; c += 32) {
                         uint32_t o[32];
                         ptx::tmem_ld_32x32(o_addr + c, o);
@@ -685,7 +691,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         float v[32];
 #pragma unroll
                         for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
-                        store(c, v, by);
+                        store(c, v, by_whole);
                     }
                     store_sum(ref, sum);
                 } else {
