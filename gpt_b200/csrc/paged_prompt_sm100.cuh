@@ -99,28 +99,11 @@ __device__ __forceinline__ float rcp_fast(float x)
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-__device__ __forceinline__ unsigned long long pair(float a, float b)
-{
-    unsigned long long v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
-    return v;
-}
-__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-
+using tok::pair;
+using tok::tanh_inner2;
+using tok::unpair;
 // cap * tanh(x), x the score over the cap: cap - 2 cap / (1 + exp(2 x))
 __device__ __forceinline__ float capped(float x, float cap) { return fmaf(-2.0f * cap, rcp_fast(1.0f + tok::exp2_fast(x * 2.8853900817779268f)), cap); }
-// tanh of two values within [-1, 1]: x times a polynomial in x^2, the Chebyshev fit of degree 7 of tanh(x) / x (largest error 5e-9, with fp32 rounding 7e-8)
-__device__ __forceinline__ unsigned long long tanh_inner2(unsigned long long x)
-{
-    constexpr float c[8] = {1.0f, -0.33333307504653931f, 0.13332527875900269f, -0.053887963294982910f, 0.021501919254660606f, -0.0079579148441553116f, 0.0023032133467495441f,
-                            -0.00035729847149923444f};
-    const unsigned long long u = ptx::mul2(x, x);
-    unsigned long long p = ptx::both(c[7]);
-#pragma unroll
-    for (int i = 6; i >= 0; --i) p = ptx::fma2(p, u, ptx::both(c[i]));
-    return ptx::mul2(p, x);
-}
-
 // Eight codes as bf16 values times a power of two.  A code's bits in a bf16's place (exponent and mantissa side by side) stand for code * 2^-120, subnormal
 // ones among them; one product by 2^(120 + e) puts them right, exactly, for e up to 7 (values up to 57344).
 __device__ __forceinline__ uint32_t bf16_mul(uint32_t a, uint32_t b)
@@ -306,7 +289,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         const int idx = i * 64 + t, r = idx / (8 * NB), c = idx % (8 * NB);
                         const long long row = row_at[which][turn][r];
                         const bool on = row >= 0 && c < pieces;
-                        if (c < 2 * steps) tok::copy<16>(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? data + row * dim + c * 8 : data, on);
+                        if (c < 2 * steps) tok::copy_or_zero<16>(dst + (c >> 3) * kPromptBlock + r * 128 + (((c & 7) ^ (r & 7)) << 4), on ? data + row * dim + c * 8 : data, on);
                     }
                 }
             }
@@ -377,7 +360,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     const int r = i / (8 * NB), c = i % (8 * NB), packed = packed0 + r, token = a.shares.divide(packed);
                     const bool on = r < rows && c < pieces;
                     if (c < 2 * steps)
-                        tok::copy<16>(q_base + (r >> 7) * S::kTile + (c >> 3) * kPromptBlock + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                        tok::copy_or_zero<16>(q_base + (r >> 7) * S::kTile + (c >> 3) * kPromptBlock + (r & 127) * 128 + (((c & 7) ^ (r & 7)) << 4),
                                       on ? q + token * a.q_pitch + (packed - token * a.share) * dim + c * 8 : q, on);
                 }
                 asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");

@@ -29,7 +29,9 @@ constexpr int kTokensPart = kTokensRows * 128 + 2 * kTokensRows;   // floats of 
 // D16: dimensions in steps of 16 (zeros behind the head's own)
 template <int D16, bool CODES>
 struct TokensShape {
-    static constexpr int kDim = 16 * D16;
+    static constexpr int kDim = 16 * D16, kBytes = CODES ? 1 : 2;
+    // copies: pieces of sixteen bytes per row (a power of two), rows that a warp takes in one turn, turns for sixteen rows
+    static constexpr int kPieces = CODES ? (D16 > 4 ? 8 : D16) : (D16 > 4 ? 16 : 2 * D16), kRowsPerTurn = 32 / kPieces, kTurns = 16 / kRowsPerTurn;
     // pitches that spread what the lanes of one load touch over all banks
     static constexpr int kKeyPitch = CODES ? (D16 == 8 ? 144 : 16 * D16) : 2 * kDim + 16;
     static constexpr int kValuePitch = CODES ? (D16 == 8 ? 144 : D16 == 6 ? 112 : D16 == 4 ? 80 : 48) : 2 * kDim + 16;
@@ -72,14 +74,42 @@ __device__ __forceinline__ float exp2_fast(float x)
 }
 // Factor that brings what stands against maximum m to maximum `top`.  A part that saw nothing holds zeros (or NaN, which stay) and counts as it is.
 __device__ __forceinline__ float share_of(float m, float top) { return m == -INFINITY ? 1.0f : exp2_fast(m - top); }
-// bytes of shared memory, from nothing where `from` is not to be read
 template <int BYTES>
-__device__ __forceinline__ void copy(uint32_t dst, const void *from, bool there)
+__device__ __forceinline__ void copy(uint32_t dst, const void *from)
+{
+    static_assert(BYTES == 16);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(from) : "memory");
+}
+// zeros where `from` is not to be read
+template <int BYTES>
+__device__ __forceinline__ void copy_or_zero(uint32_t dst, const void *from, bool there)
 {
     if constexpr (BYTES == 16)
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(from), "r"(there ? 16 : 0) : "memory");
     else
         asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(from), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ const uint8_t *shared_pointer(const uint8_t *p, int from)
+{
+    return reinterpret_cast<const uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(p), from));
+}
+__device__ __forceinline__ unsigned long long pair(float a, float b)
+{
+    unsigned long long v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void unpair(unsigned long long v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+// tanh of two values within [-1, 1]: x times a polynomial in x^2, the Chebyshev fit of degree 7 of tanh(x) / x (largest error 5e-9, with fp32 rounding 7e-8)
+__device__ __forceinline__ unsigned long long tanh_inner2(unsigned long long x)
+{
+    constexpr float c[8] = {1.0f, -0.33333307504653931f, 0.13332527875900269f, -0.053887963294982910f, 0.021501919254660606f, -0.0079579148441553116f, 0.0023032133467495441f,
+                            -0.00035729847149923444f};
+    const unsigned long long u = ptx::mul2(x, x);
+    unsigned long long p = ptx::both(c[7]);
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = ptx::fma2(p, u, ptx::both(c[i]));
+    return ptx::mul2(p, x);
 }
 // two codes as two halves
 __device__ __forceinline__ uint32_t halves(uint32_t pair)
@@ -133,7 +163,15 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     Place place;
     Range range = range_of_block<kTokensThreads>(a, args.cut, place);
     const uint32_t q_tile = ptx::smem_u32(tokens_smem), ring = q_tile + kTokensRows * S::kQPitch + warp * S::kStages * S::kStage;
-    const int dim = a.pages.dim, pieces = dim / 8;
+    const int dim = a.pages.dim, pieces = dim / 8, mask = (1 << a.pages.page_shift) - 1;
+    // sixteen-byte pieces of a row per lane; where codes' rows begin at odd multiples of eight they are copied by eights
+    const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
+    const int row_bytes = dim * S::kBytes;
+    const bool wide = row_bytes % 16 == 0;
+    const long long head_bytes = static_cast<long long>(row_bytes) << a.pages.page_shift, value_bytes = head_bytes * a.pages.kv_heads, page_bytes = 2 * value_bytes;
+    const int lane_row = lane / S::kPieces, lane_piece = lane % S::kPieces, lane_from = lane_row * row_bytes + lane_piece * 16;
+    const bool lane_on = lane_piece * 16 < row_bytes;
+    const uint32_t key_to = lane_row * S::kKeyPitch + lane_piece * 16, value_to = 16 * S::kKeyPitch + lane_row * S::kValuePitch + lane_piece * 16;
     // a head narrower than the padded width: its tail columns stay zero
     auto clear_tail = [&] {
         if (dim == S::kDim) return;
@@ -156,62 +194,56 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         auto wanted = [&](int key) { return key <= p1 && (key >= low || key < a.sinks); };   // by any row of the tile
 
         // ---- the ring
-        // lanes with an even number look up the page of the tile's first eight keys, the others that of the last eight
-        auto page_for = [&](int i) {
-            if (i >= n_blocks) return -1;
-            const int key = tile_key(i) + 8 * (lane & 1);
-            return key <= p1 && (key + 7 >= low || key < a.sinks) ? page_of(a.batch, a.pages, place.s, key) : -1;
+        // lanes with an even number look up where the tile's first eight keys lie, the others the last eight: those of a page's head lie one behind the other
+        int next_page = -1;
+        const uint8_t *next_rows = nullptr;
+        auto look_up = [&](int i) {
+            next_page = -1;
+            if (i < n_blocks) {
+                const int key = tile_key(i) + 8 * (lane & 1);
+                if (key <= p1 && (key + 7 >= low || key < a.sinks)) next_page = page_of(a.batch, a.pages, place.s, key);
+                next_rows = data + max(next_page, 0) * page_bytes + place.g * head_bytes + (key & mask) * row_bytes;
+            }
         };
-        int next_page = page_for(0);
+        look_up(0);
         auto fetch = [&](int i) {
             const int stage = i % S::kStages;
             const uint32_t dst = ring + stage * S::kStage;
             const int page[2] = {__shfl_sync(0xffffffffu, next_page, 0), __shfl_sync(0xffffffffu, next_page, 1)};
-            next_page = page_for(i + 1);
+            const uint8_t *rows8[2] = {shared_pointer(next_rows, 0), shared_pointer(next_rows, 1)};
+            look_up(i + 1);
             if (i < n_blocks) {
-                const int t = tile_key(i), mask = (1 << a.pages.page_shift) - 1;
-                if constexpr (CODES) {
-                    const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
-                    if (dim % 16 == 0) {
+                const int t = tile_key(i);
+                if (page[0] >= 0 && page[1] >= 0 && t + 15 <= p1 && (t >= low || t + 16 <= a.sinks) && wide) {   // every key is wanted
 #pragma unroll
-                        for (int j = 0; j < D16 / 2; ++j) {
-                            const int idx = j * 32 + lane, r = idx / D16, c = idx % D16, key = t + r, pg = page[r >> 3];
-                            const bool on = c * 16 < dim && pg >= 0 && wanted(key);
-#pragma unroll
-                            for (int which = 0; which < 2; ++which) {
-                                const uint8_t *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 16 : data;
-                                const uint32_t to = dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 16;
-                                if (c * 16 < dim) copy<16>(to, src, on);
-                            }
+                    for (int j = 0; j < S::kTurns; ++j) {
+                        const int first = j * S::kRowsPerTurn;
+                        const uint8_t *from = S::kRowsPerTurn == 16 ? (lane_row >= 8 ? rows8[1] - 8 * row_bytes : rows8[0]) : rows8[first >> 3] + (first & 7) * row_bytes;
+                        if (lane_on) {
+                            copy<16>(dst + first * S::kKeyPitch + key_to, from + lane_from);
+                            copy<16>(dst + first * S::kValuePitch + value_to, from + lane_from + value_bytes);
                         }
-                    } else {
-                        for (int idx = lane; idx < 16 * pieces; idx += 32) {
-                            const int r = idx / pieces, c = idx % pieces, key = t + r, pg = page[r >> 3];
-                            const bool on = pg >= 0 && wanted(key);
-#pragma unroll
-                            for (int which = 0; which < 2; ++which) {
-                                const uint8_t *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 8 : data;
-                                copy<8>(dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 8, src, on);
-                            }
-                        }
-                    }
-                    if (lane < 4) {   // powers of two: eight keys a copy, keys' then values'
-                        const int half = lane & 1, which = lane >> 1, pg = page[half];
-                        const uint8_t *src = pg >= 0 ? a.pages.scales + a.pages.place(pg, which, place.g, (t + 8 * half) & mask) : a.pages.scales;
-                        copy<8>(dst + 16 * (S::kKeyPitch + S::kValuePitch) + 16 * which + 8 * half, src, pg >= 0);
                     }
                 } else {
-                    const __nv_bfloat16 *data = static_cast<const __nv_bfloat16 *>(a.pages.data);
-#pragma unroll
-                    for (int j = 0; j < D16; ++j) {
-                        const int idx = j * 32 + lane, r = idx / (2 * D16), c = idx % (2 * D16), key = t + r, pg = page[r >> 3];
-                        const bool on = c < pieces && pg >= 0 && wanted(key);
-#pragma unroll
-                        for (int which = 0; which < 2; ++which) {
-                            const __nv_bfloat16 *src = on ? data + a.pages.place(pg, which, place.g, key & mask) * dim + c * 8 : data;
-                            if (c < pieces) copy<16>(dst + (which ? 16 * S::kKeyPitch + r * S::kValuePitch : r * S::kKeyPitch) + c * 16, src, on);
+                    const int step = wide ? 16 : 8, chunks = row_bytes / step;
+                    for (int idx = lane; idx < 16 * chunks; idx += 32) {
+                        const int r = idx / chunks, c = idx % chunks;
+                        const bool on = page[r >> 3] >= 0 && wanted(t + r);
+                        const uint8_t *from = on ? rows8[r >> 3] + (r & 7) * row_bytes + c * step : data;
+                        const uint32_t key_at = dst + r * S::kKeyPitch + c * step, value_at = dst + 16 * S::kKeyPitch + r * S::kValuePitch + c * step;
+                        if (wide) {
+                            copy_or_zero<16>(key_at, from, on);
+                            copy_or_zero<16>(value_at, on ? from + value_bytes : data, on);
+                        } else {
+                            copy_or_zero<8>(key_at, from, on);
+                            copy_or_zero<8>(value_at, on ? from + value_bytes : data, on);
                         }
                     }
+                }
+                if (CODES && lane < 4) {   // powers of two: eight keys a copy, keys' then values'
+                    const int half = lane & 1, which = lane >> 1, pg = page[half];
+                    const uint8_t *src = pg >= 0 ? a.pages.scales + a.pages.place(pg, which, place.g, (t + 8 * half) & mask) : a.pages.scales;
+                    copy_or_zero<8>(dst + 16 * (S::kKeyPitch + S::kValuePitch) + 16 * which + 8 * half, src, pg >= 0);
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -267,7 +299,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         for (int i = 0; i < 2; ++i) {
             const int r = g8 + 8 * i;
             pos[i] = r < rows ? place.q.pos0 + a.shares.divide(packed0 + r) : -1;
-            to_score[i] = a.scale * (CODES ? row_power[r] : 1.0f);
+            to_score[i] = (a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e) * (CODES ? row_power[r] : 1.0f);   // over the cap, or in base 2
         }
 
         float m[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // ref: against which the weighted values stand (codes only)
@@ -318,13 +350,23 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             for (int i = 0; i < 2; ++i) {
                 if (i == 1 && !second) break;
                 float top = -INFINITY, top_ref = -INFINITY;
+                if (a.cap > 0.0f) {   // a polynomial where all of the warp's scores lie within the cap
+                    float u[4] = {x[0][2 * i] * to_score[i], x[0][2 * i + 1] * to_score[i], x[1][2 * i] * to_score[i], x[1][2 * i + 1] * to_score[i]};
+                    if (__all_sync(0xffffffffu, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))) <= 1.0f)) {
+                        unpair(tanh_inner2(pair(u[0], u[1])), u[0], u[1]);
+                        unpair(tanh_inner2(pair(u[2], u[3])), u[2], u[3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) u[e] = tanhf(u[e]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) x[e >> 1][2 * i + (e & 1)] = u[e];
+                }
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float v = x[j][2 * i + e] * to_score[i];
-                        if (a.cap > 0.0f) v = a.cap * tanhf(v / a.cap);
-                        v *= kLog2e;
+                        float v = x[j][2 * i + e] * (a.cap > 0.0f ? a.cap * kLog2e : to_score[i]);
                         if (!all_seen && !visible(a, t + 8 * j + 2 * t4 + e, pos[i])) v = -INFINITY;
                         x[j][2 * i + e] = v;
                         top = fmaxf(top, v);
