@@ -78,23 +78,24 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
     OnDevice device;
     CUDA_TRY(ctx, device.enter(ctx->device));
     a.k = k; a.v = v; a.k_pitch = k_pitch; a.v_pitch = v_pitch;
-    while ((1 << a.lanes_log2) < pages->dim / 8) ++a.lanes_log2;
-    // about four pieces per thread while that fills the GPU, one row per block at least
-    const int per_row = 2 * pages->kv_heads << a.lanes_log2;
-    const int most = std::min(kvp::kRowMax, std::max(1, 4 * kvp::kRowThreads / per_row));
-    a.rows_per_block = std::max(1, std::min(most, rows->rows / (2 * ctx->num_sms)));
+    const bool sixteens = pages->dim % 16 == 0;
+    while ((1 << a.lanes_log2) < pages->dim / (sixteens ? 16 : 8)) ++a.lanes_log2;
+    // a row's threads, as many rows side by side as the block has room for; a few rows per thread while that fills the GPU
+    const int all_columns = 2 * pages->kv_heads << a.lanes_log2;
+    a.columns = std::min(all_columns, kvp::kRowThreads);
+    const int side = kvp::kRowThreads / a.columns, threads = (side * a.columns + 31) / 32 * 32;
+    a.rows_per_block = std::max(1, std::min({kvp::kRowMax, kvp::row_turns(WRITE) * side, rows->rows / (2 * ctx->num_sms)}));
     const int blocks = (rows->rows + a.rows_per_block - 1) / a.rows_per_block;
-    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(blocks), dim3(kvp::kRowThreads), 0, a); };
-    cudaError_t e;
-    if (dtype == GPTB200_DTYPE_F32)
-        e = pages->kind == GPTB200_KV_E4M3 ? launch(kvp::kv_rows_kernel<float, kvp::KIND_E4M3, WRITE>)
-            : pages->kind == GPTB200_KV_F32 ? launch(kvp::kv_rows_kernel<float, kvp::KIND_F32, WRITE>)
-                                            : launch(kvp::kv_rows_kernel<float, kvp::KIND_BF16, WRITE>);
-    else
-        e = pages->kind == GPTB200_KV_E4M3 ? launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_E4M3, WRITE>)
-            : pages->kind == GPTB200_KV_F32 ? launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_F32, WRITE>)
-                                            : launch(kvp::kv_rows_kernel<__nv_bfloat16, kvp::KIND_BF16, WRITE>);
-    CUDA_TRY(ctx, e);
+    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(blocks), dim3(threads), 0, a); };
+    auto launch_kind = [&](auto type) {
+        using T = decltype(type);
+        switch (pages->kind) {
+            case GPTB200_KV_E4M3: return sixteens ? launch(kvp::kv_rows_kernel<T, kvp::KIND_E4M3, WRITE, 2>) : launch(kvp::kv_rows_kernel<T, kvp::KIND_E4M3, WRITE, 1>);
+            case GPTB200_KV_F32: return sixteens ? launch(kvp::kv_rows_kernel<T, kvp::KIND_F32, WRITE, 2>) : launch(kvp::kv_rows_kernel<T, kvp::KIND_F32, WRITE, 1>);
+            default: return sixteens ? launch(kvp::kv_rows_kernel<T, kvp::KIND_BF16, WRITE, 2>) : launch(kvp::kv_rows_kernel<T, kvp::KIND_BF16, WRITE, 1>);
+        }
+    };
+    CUDA_TRY(ctx, dtype == GPTB200_DTYPE_F32 ? launch_kind(float()) : launch_kind(__nv_bfloat16()));
     ctx->launches++;
     return GPTB200_OK;
 }
@@ -114,7 +115,7 @@ int attention_rows(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
 
 // A kernel that cuts the line of work into equal ranges: `per_sm` blocks on every SM, a part of a tile in scratch for either end of a range.
 template <typename Args>
-int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, int smem, int per_sm, int part_floats)
+int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, int smem, int per_sm, int most_blocks, int part_floats)
 {
     const void *key = reinterpret_cast<const void *>(kernel);
     if (!ctx->configured.count(key)) {
@@ -122,7 +123,7 @@ int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, in
         ctx->configured.insert(key);
     }
     const int sms = ctx->max_sms > 0 ? std::min(ctx->max_sms, ctx->num_sms) : ctx->num_sms;
-    const int blocks = std::min(sms * per_sm, kPagedTickets);
+    const int blocks = std::min(sms * per_sm, most_blocks);
     const int rc = ensure_workspace(ctx, size_t(2) * blocks * part_floats * sizeof(float));
     if (rc != GPTB200_OK) return rc;
     args.parts = {ctx->ws, ctx->d_paged_tickets, part_floats};
@@ -131,21 +132,30 @@ int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, in
     return GPTB200_OK;
 }
 
-template <int D16, bool CODES>
+template <int D16, bool CODES, int NT>
 int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args)
 {
-    return run_line(ctx, kvp::paged_tokens_kernel<D16, CODES>, args, kvp::kTokensThreads, kvp::TokensShape<D16, CODES>::kSmem, CODES ? 3 : 2, kvp::kTokensPart);
+    using S = kvp::TokensShape<D16, CODES, NT>;
+    args.cut.tile_rows = S::kRows;
+    return run_line(ctx, kvp::paged_tokens_kernel<D16, CODES, NT>, args, kvp::kTokensThreads, S::kSmem, S::kPerSm, std::min(S::kMaxBlocks, kPagedTickets), kvp::kTokensPart);
 }
 
-int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
+template <int D16>
+int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args, bool codes, bool few)
 {
-    kvp::TokensArgs args{a, {}, {kvp::kTokensRows, kvp::kTokensKeys, 1, 5}};
+    if (codes) return few ? run_tokens<D16, true, 1>(ctx, args) : run_tokens<D16, true, 2>(ctx, args);
+    return few ? run_tokens<D16, false, 1>(ctx, args) : run_tokens<D16, false, 2>(ctx, args);
+}
+
+int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind, bool few)
+{
+    kvp::TokensArgs args{a, {}, {0, kvp::kTokensKeys, 1, 5}};
     const bool codes = kind == GPTB200_KV_E4M3;
     switch ((a.pages.dim + 31) / 32) {
-        case 1: return codes ? run_tokens<2, true>(ctx, args) : run_tokens<2, false>(ctx, args);
-        case 2: return codes ? run_tokens<4, true>(ctx, args) : run_tokens<4, false>(ctx, args);
-        case 3: return codes ? run_tokens<6, true>(ctx, args) : run_tokens<6, false>(ctx, args);
-        default: return codes ? run_tokens<8, true>(ctx, args) : run_tokens<8, false>(ctx, args);
+        case 1: return run_tokens<2>(ctx, args, codes, few);
+        case 2: return run_tokens<4>(ctx, args, codes, few);
+        case 3: return run_tokens<6>(ctx, args, codes, few);
+        default: return run_tokens<8>(ctx, args, codes, few);
     }
 }
 
@@ -153,7 +163,7 @@ template <int NB, bool CODES>
 int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args)
 {
     return run_line(ctx, args.a.cap > 0.0f ? kvp::paged_prompt_kernel<NB, CODES, true> : kvp::paged_prompt_kernel<NB, CODES, false>, args, kvp::kPromptThreads,
-                    kvp::PromptShape<NB>::kSmem, 1, kvp::kPromptPart);
+                    kvp::PromptShape<NB>::kSmem, 1, kPagedTickets / 2, kvp::kPromptPart);
 }
 
 int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
@@ -214,7 +224,7 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
     a.sinks = a.window ? sinks : 0;
     if (dtype == GPTB200_DTYPE_BF16 && pages->kind != GPTB200_KV_F32)
-        return 1LL * rows->max_new * a.share > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind);
+        return 1LL * rows->max_new * a.share > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind, 1LL * rows->max_new * a.share <= 8);
     return dtype == GPTB200_DTYPE_F32 ? attention_rows<float>(ctx, a, pages->kind) : attention_rows<__nv_bfloat16>(ctx, a, pages->kind);
 }
 

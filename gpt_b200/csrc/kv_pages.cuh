@@ -140,9 +140,8 @@ __device__ __forceinline__ uint32_t to_codes2(float a, float b)
 __device__ __forceinline__ float power_of_two(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
 __device__ __forceinline__ float scale_of(uint32_t stored) { return __uint_as_float(stored << 23); }
 
-__device__ __forceinline__ void load8_codes(float (&v)[8], const uint8_t *src, float scale)
+__device__ __forceinline__ void codes8(float (&v)[8], uint2 w, float scale)
 {
-    const uint2 w = *reinterpret_cast<const uint2 *>(src);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 c = codes2((i < 2 ? w.x : w.y) >> (16 * (i & 1)));
@@ -150,6 +149,8 @@ __device__ __forceinline__ void load8_codes(float (&v)[8], const uint8_t *src, f
         v[2 * i + 1] = c.y * scale;
     }
 }
+
+__device__ __forceinline__ void load8_codes(float (&v)[8], const uint8_t *src, float scale) { codes8(v, *reinterpret_cast<const uint2 *>(src), scale); }
 
 // The smallest e with most <= 448 * 2^e, from most's exponent and mantissa (448 = 1.75 * 2^8).
 __device__ __forceinline__ int exponent_for(float most)
@@ -159,10 +160,17 @@ __device__ __forceinline__ int exponent_for(float most)
     return min(max(e, kMinExponent), kMaxExponent);
 }
 
-// Rows of keys and values <-> pages.  A piece of eight elements per lane: as many lanes as a head has pieces (a power of two of them, so that the row's
-// largest value is a few shuffles) take one (row, keys or values, head) at a time.  Bound by DRAM: nothing is read or written twice.
+// Rows of keys and values <-> pages.  A piece of sixteen elements per lane (eight where a head has an odd number of eights); as many lanes as a head has pieces (a power of two of them) hold a head, so that a row's
+// largest value is a few shuffles.  A thread keeps to its piece of the row and walks down the rows: no index is formed twice.  Bound by DRAM as far as copies go; with
+// codes by instructions (a row's largest value, a conversion per pair), which is why the largest value of bf16 rows is found two at a time on their bits.
 constexpr int kRowThreads = 256;
-constexpr int kRowMax = 32;   // rows per block, at most
+constexpr int kRowMax = 64;    // rows per block, at most
+// Pieces under way per thread, blocks per SM, rows per thread.  Writing (24 400 rows of 8 heads of 128 from bf16 to codes): 39.5 us with four blocks of four pieces each, 5.1 TB/s;
+// 56 us with rows looked up by a warp each and two blocks.  Reading (16 600 rows of 4 heads back): 25.5 us with eight blocks and one piece, 4.3 TB/s; 33 us with
+// four pieces each.
+__host__ __device__ constexpr int row_batch(bool write) { return write ? 4 : 1; }
+__host__ __device__ constexpr int row_blocks(bool write) { return write ? 4 : 8; }
+__host__ __device__ constexpr int row_turns(bool write) { return write ? 8 : 4; }
 
 struct RowsArgs {
     Pages pages;
@@ -170,98 +178,205 @@ struct RowsArgs {
     void *k, *v;
     long long k_pitch, v_pitch;
     int lanes_log2;      // lanes per head
+    int columns;         // threads that share a row: all its pieces, or the block
     int rows_per_block;
 };
 
+// Eight elements as they lie in memory.
+template <typename T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> {
+    uint4 w;
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p) { w = *reinterpret_cast<const uint4 *>(p); }
+    __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
+        const uint32_t x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = bf16_low(x[i]);
+            v[2 * i + 1] = bf16_high(x[i]);
+        }
+    }
+    // bits of the largest magnitude as fp32; not finite ones are larger than all others
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        const uint32_t m = __vmaxu2(__vmaxu2(w.x & 0x7fff7fffu, w.y & 0x7fff7fffu), __vmaxu2(w.z & 0x7fff7fffu, w.w & 0x7fff7fffu));
+        return max(m & 0xffff0000u, m << 16);
+    }
+};
+template <> struct Raw8<float> {
+    uint4 w, u;
+    __device__ __forceinline__ void load(const float *p)
+    {
+        w = *reinterpret_cast<const uint4 *>(p);
+        u = *reinterpret_cast<const uint4 *>(p + 4);
+    }
+    __device__ __forceinline__ void zero() { w = u = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const
+    {
+        const uint32_t x[8] = {w.x, w.y, w.z, w.w, u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(x[i]);
+    }
+    __device__ __forceinline__ uint32_t largest() const
+    {
+        constexpr uint32_t bits = 0x7fffffffu;
+        return max(max(max(w.x & bits, w.y & bits), max(w.z & bits, w.w & bits)), max(max(u.x & bits, u.y & bits), max(u.z & bits, u.w & bits)));
+    }
+};
+
 // WRITE: rows of T into pages of KIND, else the other way.
-template <typename T, int KIND, bool WRITE>
-__global__ void __launch_bounds__(kRowThreads)
+// EIGHTS: groups of eight elements per piece.
+template <typename T, int KIND, bool WRITE, int EIGHTS>
+__global__ void __launch_bounds__(kRowThreads, row_blocks(WRITE))
 kv_rows_kernel(const RowsArgs a)
 {
+    constexpr int kRowBatch = row_batch(WRITE);
     __shared__ int where[kRowMax][2];   // page (-1: none) and token within it
     grid_dependency_wait();
     grid_dependency_launch();
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int first = blockIdx.x * a.rows_per_block, rows = min(a.rows_per_block, a.batch.rows - first);
-    for (int r = warp; r < rows; r += kRowThreads / 32) {
-        const int s = sequence_of_row(a.batch, first + r, lane);
-        if (lane == 0) {
-            int page = -1, token = 0;
-            if (s >= 0) {
-                const Sequence q = sequence_of(a.batch, s);
-                const int nth = first + r - q.row0, position = q.pos0 + nth;
-                if (nth >= 0 && nth < q.count && position >= 0) {
-                    page = page_of(a.batch, a.pages, s, position);
-                    token = position & ((1 << a.pages.page_shift) - 1);
-                }
-            }
-            where[r][0] = page;
-            where[r][1] = token;
-        }
-    }
-    __syncthreads();
-    const int pieces = a.pages.dim / 8, per = 1 << a.lanes_log2, piece = threadIdx.x & (per - 1), heads = a.pages.kv_heads;
-    const int units = rows * 2 * heads, stride = kRowThreads >> a.lanes_log2, rounds = (units + stride - 1) / stride;
-    const bool active = piece < pieces;
-#pragma unroll 4
-    for (int round = 0; round < rounds; ++round) {
-        const int u = round * stride + (threadIdx.x >> a.lanes_log2);
-        const int r = u / (2 * heads), which = u / heads % 2, h = u % heads;
-        const bool in = u < units && active;
-        const int page = in ? where[r][0] : -1;
-        const bool on = page >= 0;
-        T *row = nullptr;
-        long long at = 0;
-        if (on) {
-            row = static_cast<T *>(which ? a.v : a.k) + static_cast<long long>(first + r) * (which ? a.v_pitch : a.k_pitch) + h * a.pages.dim + piece * 8;
-            at = a.pages.place(page, which, h, where[r][1]);
-        }
-        float v[8] = {};
-        if constexpr (WRITE) {
-            if (on) load8(v, row);
-            if constexpr (KIND == KIND_E4M3) {
-                float most = 0.0f;
-                uint32_t bad = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool finite = fabsf(v[i]) <= FLT_MAX;
-                    bad |= static_cast<uint32_t>(!finite) << i;
-                    if (!finite) v[i] = 0.0f;
-                    most = fmaxf(most, fabsf(v[i]));
-                }
-                for (int o = per >> 1; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int e = exponent_for(most);
-                const float by = power_of_two(-e);
-                uint32_t c[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    c[i] = to_codes2(v[2 * i] * by, v[2 * i + 1] * by);
-                    // the format has no infinity: both kinds become its NaN
-                    if (bad >> (2 * i) & 1) c[i] = (c[i] & 0xff00u) | 0x7fu;
-                    if (bad >> (2 * i + 1) & 1) c[i] = (c[i] & 0x00ffu) | 0x7f00u;
-                }
-                if (on) {
-                    *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.pages.data) + at * a.pages.dim + piece * 8) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
-                    if (piece == 0) a.pages.scales[at] = static_cast<uint8_t>(e + 127);
-                }
-            } else if constexpr (KIND == KIND_BF16) {
-                if (on) store8(static_cast<__nv_bfloat16 *>(a.pages.data) + at * a.pages.dim + piece * 8, v);
-            } else {
-                if (on) store8(static_cast<float *>(a.pages.data) + at * a.pages.dim + piece * 8, v);
-            }
-        } else if (on) {
-            if constexpr (KIND == KIND_E4M3)
-                load8_codes(v, static_cast<const uint8_t *>(a.pages.data) + at * a.pages.dim + piece * 8, scale_of(a.pages.scales[at]));
-            else if constexpr (KIND == KIND_BF16)
-                load8(v, static_cast<const __nv_bfloat16 *>(a.pages.data) + at * a.pages.dim + piece * 8);
+    const int per = 1 << a.lanes_log2, heads = a.pages.kv_heads, dim = a.pages.dim, all_columns = 2 * heads << a.lanes_log2;
+    const int row0 = threadIdx.x / a.columns, column0 = threadIdx.x - row0 * a.columns, step = blockDim.x / a.columns;
+    // a thread per row: the loads of a look-up depend on one another, so the rows' chains run side by side
+    for (int r = threadIdx.x; r < rows; r += blockDim.x) {
+        const int row = first + r;
+        int low = 0, high = a.batch.sequences, page = -1, token = 0;   // the last s with row_starts[s] <= row
+        while (high - low > 1) {
+            const int middle = low + (high - low) / 2;
+            if (a.batch.row_starts[middle] <= row)
+                low = middle;
             else
-                load8(v, static_cast<const float *>(a.pages.data) + at * a.pages.dim + piece * 8);
-            store8(row, v);
+                high = middle;
+        }
+        const Sequence q = sequence_of(a.batch, low);
+        const int nth = row - q.row0, position = q.pos0 + nth;
+        if (nth >= 0 && nth < q.count && position >= 0) {
+            page = page_of(a.batch, a.pages, low, position);
+            token = position & ((1 << a.pages.page_shift) - 1);
+        }
+        where[r][0] = page;
+        where[r][1] = token;
+    }
+    const long long head_tokens = 1LL << a.pages.page_shift, page_tokens = 2 * heads * head_tokens;
+    bool begun = false;
+    for (int c0 = 0; c0 < all_columns; c0 += a.columns) {
+        const int column = c0 + column0, unit = column >> a.lanes_log2, piece = column & (per - 1), which = unit >= heads, h = which ? unit - heads : unit;
+        const bool active = row0 < step && column < all_columns && piece * 8 * EIGHTS < dim;
+        const long long pitch = which ? a.v_pitch : a.k_pitch, head_at = (which * heads + h) * head_tokens;
+        T *column_rows = static_cast<T *>(which ? a.v : a.k) + first * pitch + h * dim + piece * 8 * EIGHTS;
+        Raw8<T> raw[kRowBatch][EIGHTS];
+        auto load_rows = [&](int base) {   // the rows' own addresses need no page
+#pragma unroll
+            for (int i = 0; i < kRowBatch; ++i) {
+                const int r = base + i * step;
+#pragma unroll
+                for (int x = 0; x < EIGHTS; ++x) {
+                    raw[i][x].zero();
+                    if (active && r < rows) raw[i][x].load(column_rows + r * pitch + 8 * x);
+                }
+            }
+        };
+        if constexpr (WRITE) load_rows(row0);
+        if (!begun) __syncthreads();
+        begun = true;
+        for (int base = 0; base < rows; base += kRowBatch * step) {   // the same for all threads: shuffles below
+            if constexpr (!WRITE) {
+                const int r = base + row0, page = active && r < rows ? where[r][0] : -1;
+                if (page >= 0) {
+                    const long long at = page * page_tokens + head_at + where[r][1], from = at * dim + piece * 8 * EIGHTS;
+                    float v[EIGHTS][8];
+                    if constexpr (KIND == KIND_E4M3) {
+                        const float scale = scale_of(a.pages.scales[at]);
+                        const uint8_t *codes = static_cast<const uint8_t *>(a.pages.data) + from;
+                        if constexpr (EIGHTS == 2) {
+                            const uint4 w = *reinterpret_cast<const uint4 *>(codes);
+                            codes8(v[0], make_uint2(w.x, w.y), scale);
+                            codes8(v[1], make_uint2(w.z, w.w), scale);
+                        } else {
+                            load8_codes(v[0], codes, scale);
+                        }
+                    } else {
+#pragma unroll
+                        for (int x = 0; x < EIGHTS; ++x) {
+                            if constexpr (KIND == KIND_BF16)
+                                load8(v[x], static_cast<const __nv_bfloat16 *>(a.pages.data) + from + 8 * x);
+                            else
+                                load8(v[x], static_cast<const float *>(a.pages.data) + from + 8 * x);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < EIGHTS; ++x) store8(column_rows + r * pitch + 8 * x, v[x]);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kRowBatch; ++i) {
+                    const int r = base + row0 + i * step, page = active && r < rows ? where[r][0] : -1;
+                    const bool on = page >= 0;
+                    const long long at = on ? page * page_tokens + head_at + where[r][1] : 0, to = at * dim + piece * 8 * EIGHTS;
+                    float v[EIGHTS][8];
+#pragma unroll
+                    for (int x = 0; x < EIGHTS; ++x) raw[i][x].get(v[x]);
+                    if constexpr (KIND == KIND_E4M3) {
+                        constexpr uint32_t infinity = 0x7f800000u;
+                        uint32_t most = raw[i][0].largest(), bad = 0;
+                        if constexpr (EIGHTS == 2) most = max(most, raw[i][1].largest());
+                        if (most >= infinity) {   // the largest finite one counts
+                            most = 0;
+#pragma unroll
+                            for (int e = 0; e < 8 * EIGHTS; ++e) {
+                                const uint32_t bits = __float_as_uint(v[e >> 3][e & 7]) & 0x7fffffffu;
+                                if (bits >= infinity) {
+                                    bad |= 1u << e;
+                                    v[e >> 3][e & 7] = 0.0f;
+                                } else {
+                                    most = max(most, bits);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int o = 1; o < 16; o <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o < per ? o : 0));
+                        const int exponent = exponent_for(__uint_as_float(most));
+                        const float by = power_of_two(-exponent);
+                        uint32_t w[2 * EIGHTS];
+#pragma unroll
+                        for (int x = 0; x < EIGHTS; ++x) {
+                            uint32_t c[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) c[e] = to_codes2(v[x][2 * e] * by, v[x][2 * e + 1] * by);
+                            if (bad) {   // the format has no infinity: both kinds become its NaN
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    if (bad >> (8 * x + 2 * e) & 1) c[e] = (c[e] & 0xff00u) | 0x7fu;
+                                    if (bad >> (8 * x + 2 * e + 1) & 1) c[e] = (c[e] & 0x00ffu) | 0x7f00u;
+                                }
+                            }
+                            w[2 * x] = __byte_perm(c[0], c[1], 0x5410);
+                            w[2 * x + 1] = __byte_perm(c[2], c[3], 0x5410);
+                        }
+                        if (on) {
+                            uint8_t *codes = static_cast<uint8_t *>(a.pages.data) + to;
+                            if constexpr (EIGHTS == 2)
+                                *reinterpret_cast<uint4 *>(codes) = make_uint4(w[0], w[1], w[2], w[3]);
+                            else
+                                *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
+                            if (piece == 0) a.pages.scales[at] = static_cast<uint8_t>(exponent + 127);
+                        }
+                    } else if (on) {
+#pragma unroll
+                        for (int x = 0; x < EIGHTS; ++x) {
+                            if constexpr (KIND == KIND_BF16)
+                                store8(static_cast<__nv_bfloat16 *>(a.pages.data) + to + 8 * x, v[x]);
+                            else
+                                store8(static_cast<float *>(a.pages.data) + to + 8 * x, v[x]);
+                        }
+                    }
+                }
+                if (base + kRowBatch * step < rows) load_rows(base + kRowBatch * step + row0);
+            }
         }
     }
 }
-
-// ---- attention
 
 // Division of numbers below 2^31 by a number known on the host, as a product and a shift (Granlund and Montgomery, Division by invariant integers using
 // multiplication, 1994): a tile's positions take half a dozen divisions by the group's size, which were 3 000 cycles between two tiles.
@@ -285,6 +400,8 @@ inline Divisor divisor(uint32_t by)
     d.factor = static_cast<uint32_t>((((1ull << d.shift) - by) << 32) / by + 1);
     return d;
 }
+
+// ---- attention
 
 struct Attention {
     Pages pages;

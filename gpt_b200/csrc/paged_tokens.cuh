@@ -1,11 +1,12 @@
 // Attention of a few new rows per sequence (single tokens above all) over a paged cache, in bf16.
 //
-// A tile is sixteen packed query rows of one sequence and key / value head (kv_pages.cuh: the line of work).  Each warp of a block takes sixteen keys of every
-// block of 64 in turn: asynchronous copies bring them, and their values, into a ring of its own; scores and weighted values are mma.sync products of 16 x 8 x 16, the
-// weights going from one to the other in registers; maximum and sum run along in fp32.  The warps meet once per tile.
+// A tile is eight (NT = 1) or sixteen packed query rows of one sequence and key / value head (kv_pages.cuh: the line of work).  Each warp of a block takes sixteen
+// keys of every block of 64 in turn: asynchronous copies bring them, and their values, into a ring of its own; scores and weighted values are mma.sync products of
+// 16 x 8 x 16 with keys, then dimensions, as their rows and the tile's rows as columns: a group of up to eight query heads fills them, where rows of the tile as rows
+// of the product would leave half of it empty and hold twice the accumulators.  Maximum and sum run along in fp32.  The warps meet once per tile.
 //
-// Bound by the cache's bytes: 16 query rows against 4 * dim bytes of a bf16 key and value are 16 flops a byte, a tenth of what mma.sync sustains, so the legacy
-// instructions do here; what counts is bytes in flight, hence the rings (50 to 100 KB per block, two or three blocks per SM) and no barrier inside the loop.
+// Bound by the cache's bytes: 8 query rows against 4 * dim bytes of a bf16 key and value are 8 flops a byte, a twentieth of what mma.sync sustains, so the legacy
+// instructions do here; what counts is bytes in flight and instructions per byte, hence the rings (40 to 100 KB per block) and no barrier inside the loop.
 //
 // Codes (e4m3) go through registers once, to fp16, which holds every code exactly; their powers of two never touch the products:
 //   scores   q of a row is divided by a power of two (its largest value's), so that fp16 holds it as bf16 did; the row's and the key's powers multiply the score
@@ -23,11 +24,11 @@ namespace gptb200 {
 namespace kvp {
 
 constexpr int kTokensWarps = 4, kTokensThreads = kTokensWarps * 32;
-constexpr int kTokensRows = 16, kTokensKeys = 64;
-constexpr int kTokensPart = kTokensRows * 128 + 2 * kTokensRows;   // floats of a part in scratch
+constexpr int kTokensMaxRows = 16, kTokensKeys = 64;
+constexpr int kTokensPart = kTokensMaxRows * 128 + 2 * kTokensMaxRows;   // floats of a part in scratch
 
 // D16: dimensions in steps of 16 (zeros behind the head's own)
-template <int D16, bool CODES>
+template <int D16, bool CODES, int NT>
 struct TokensShape {
     static constexpr int kDim = 16 * D16, kBytes = CODES ? 1 : 2;
     // copies: pieces of sixteen bytes per row (a power of two), rows that a warp takes in one turn, turns for sixteen rows
@@ -36,12 +37,16 @@ struct TokensShape {
     static constexpr int kKeyPitch = CODES ? (D16 == 8 ? 144 : 16 * D16) : 2 * kDim + 16;
     static constexpr int kValuePitch = CODES ? (D16 == 8 ? 144 : D16 == 6 ? 112 : D16 == 4 ? 80 : 48) : 2 * kDim + 16;
     static constexpr int kStage = 16 * (kKeyPitch + kValuePitch) + (CODES ? 32 : 0);
-    static constexpr int kStages = 3;
+        static constexpr int kStages = NT == 1 && !CODES ? 2 : 3;
+    static constexpr int kRows = 8 * NT;
+    static constexpr int kPerSm = CODES ? 3 : 2;   // blocks on an SM
     static constexpr int kQPitch = 2 * kDim + 16;
     static constexpr int kRing = kTokensWarps * kStages * kStage;
     static constexpr int kMergePitch = kDim + 4;
-    static constexpr int kMerge = kTokensWarps * kTokensRows * kMergePitch * 4;
-    static constexpr int kSmem = kTokensRows * kQPitch + (kRing > kMerge ? kRing : kMerge);
+    static constexpr int kMerge = kTokensWarps * kRows * kMergePitch * 4;
+    static constexpr int kMaxBlocks = kPerSm * 160;                  // of the grid: a tile may be shared by all of them ...
+    static constexpr int kPartSums = kMaxBlocks * kRows * 8;         // ... whose maxima and sums then lie in shared memory
+    static constexpr int kLarger = kRing > kMerge ? kRing : kMerge, kSmem = kRows * kQPitch + (kLarger > kPartSums ? kLarger : kPartSums);
 };
 
 namespace tok {
@@ -124,6 +129,13 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
     return h;
 }
+// an 8 x 8 matrix of sixteen-bit values, a row per four lanes, transposed
+__device__ __forceinline__ uint32_t transposed(uint32_t v)
+{
+    uint32_t t;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+    return t;
+}
 template <int WORDS>
 __device__ __forceinline__ void lds_words(uint32_t (&v)[WORDS], uint32_t addr)
 {
@@ -145,16 +157,18 @@ struct TokensArgs {
     Cut cut;
 };
 
-template <int D16, bool CODES>
-__global__ void __launch_bounds__(kTokensThreads, CODES ? 3 : 2)
+template <int D16, bool CODES, int NT>
+__global__ void __launch_bounds__(kTokensThreads, TokensShape<D16, CODES, NT>::kPerSm)
 paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 {
     using namespace tok;
-    using S = TokensShape<D16, CODES>;
+    using S = TokensShape<D16, CODES, NT>;
+    constexpr int kRows = S::kRows;
+    constexpr float kGrowth = CODES ? 8.0f : 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled: fp16 weights end at 2^16
     constexpr int kind = CODES ? KIND_E4M3 : KIND_BF16;
     constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
     extern __shared__ __align__(16) uint8_t tokens_smem[];
-    __shared__ float merge_ml[kTokensWarps][kTokensRows][2], total_ml[kTokensRows][2], row_power[kTokensRows];
+    __shared__ float merge_ml[kTokensWarps][kRows][2], total_ml[kRows][2], row_power[kRows];
     __shared__ int bad_rows, arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
@@ -162,7 +176,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g8 = lane >> 2, t4 = lane & 3;
     Place place;
     Range range = range_of_block<kTokensThreads>(a, args.cut, place);
-    const uint32_t q_tile = ptx::smem_u32(tokens_smem), ring = q_tile + kTokensRows * S::kQPitch + warp * S::kStages * S::kStage;
+    const uint32_t q_tile = ptx::smem_u32(tokens_smem), ring = q_tile + kRows * S::kQPitch + warp * S::kStages * S::kStage;
     const int dim = a.pages.dim, pieces = dim / 8, mask = (1 << a.pages.page_shift) - 1;
     // sixteen-byte pieces of a row per lane; where codes' rows begin at odd multiples of eight they are copied by eights
     const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
@@ -187,7 +201,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             continue;
         }
         const int n_blocks = part.blocks;
-        const int packed0 = place.tile * kTokensRows, rows = min(kTokensRows, place.q.count * a.share - packed0);
+        const int packed0 = place.tile * kRows, rows = min(kRows, place.q.count * a.share - packed0);
         const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1);
         const int low = a.window ? p0 - a.window + 1 : 0;   // keys below it are visible only among the first ones
         auto tile_key = [&](int i) { return block_key(place.blocks, part.from + i, kTokensKeys) + warp * 16; };
@@ -253,7 +267,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         for (int i = 0; i < S::kStages - 1; ++i) fetch(i);
 
         // ---- the queries: a row's eight dimensions per lane, sixteen lanes a row
-        for (int r = threadIdx.x >> 4; r < kTokensRows; r += kTokensThreads / 16) {
+        for (int r = threadIdx.x >> 4; r < kRows; r += kTokensThreads / 16) {
             const int c = threadIdx.x & 15;
             float v[8] = {};
             if (r < rows && c < pieces) {
@@ -280,140 +294,152 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
         }
         if (threadIdx.x == 0) bad_rows = 0;
         __syncthreads();
-        uint32_t qf[D16][4];
+        // queries as B operands: columns are rows of the tile
+        uint32_t qf[NT][D16][2];
 #pragma unroll
-        for (int k = 0; k < D16; ++k) {
-            if constexpr (CODES) {
-                uint32_t u[2], v[2];
-                lds_words<2>(u, q_tile + g8 * S::kQPitch + (t4 * 4 * D16 + 4 * k) * 2);
-                lds_words<2>(v, q_tile + (g8 + 8) * S::kQPitch + (t4 * 4 * D16 + 4 * k) * 2);
-                qf[k][0] = u[0]; qf[k][1] = v[0]; qf[k][2] = u[1]; qf[k][3] = v[1];
-            } else {
-                ldsm4(qf[k], q_tile + (lane & 15) * S::kQPitch + (k * 16 + ((lane >> 4) << 3)) * 2);
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int k = 0; k < D16; ++k) {
+                if constexpr (CODES) {
+                    lds_words<2>(qf[n][k], q_tile + (8 * n + g8) * S::kQPitch + (t4 * 4 * D16 + 4 * k) * 2);
+                } else {
+                    lds_words<1>(reinterpret_cast<uint32_t(&)[1]>(qf[n][k][0]), q_tile + (8 * n + g8) * S::kQPitch + (16 * k + 2 * t4) * 2);
+                    lds_words<1>(reinterpret_cast<uint32_t(&)[1]>(qf[n][k][1]), q_tile + (8 * n + g8) * S::kQPitch + (16 * k + 2 * t4 + 8) * 2);
+                }
             }
-        }
-        const bool second = rows > 8;   // rows 8 .. 15 are there
-        int pos[2];
-        float to_score[2];
+        // a lane's rows: 2 t4 and 2 t4 + 1 of every eight
+        int pos[NT][2];
+        float to_score[NT][2], m[NT][2], ref[NT][2], l[NT][2] = {};   // m: what the sums stand against, ref: what the weighted values stand against (codes; else m)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = g8 + 8 * i;
-            pos[i] = r < rows ? place.q.pos0 + a.shares.divide(packed0 + r) : -1;
-            to_score[i] = (a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e) * (CODES ? row_power[r] : 1.0f);   // over the cap, or in base 2
-        }
-
-        float m[2] = {-INFINITY, -INFINITY}, ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};   // ref: against which the weighted values stand (codes only)
-        float O[2 * D16][4] = {};
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t4 + e;
+                pos[n][e] = r < rows ? place.q.pos0 + a.shares.divide(packed0 + r) : -1;
+                to_score[n][e] = (a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e) * (CODES ? row_power[r] : 1.0f);   // over the cap, or in base 2
+                m[n][e] = ref[n][e] = -INFINITY;
+            }
+        const float cap_log2 = a.cap * kLog2e;
+        float O[NT][D16][4] = {};
         for (int it = 0; it < n_blocks; ++it) {
             fetch(it + S::kStages - 1);
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
             __syncwarp();
             const int t = tile_key(it);
             const uint32_t kt = ring + it % S::kStages * S::kStage, vt = kt + 16 * S::kKeyPitch, et = vt + 16 * S::kValuePitch;
-            float x[2][4] = {};
-            float value_e[2][2];   // exponents of the values of the lane's keys
+            // scores: rows of the product are keys g8 and g8 + 8, columns rows of the tile
+            float x[NT][4] = {};
+            float value_e[2] = {};   // exponents of the two keys' values
             if constexpr (CODES) {
-                // keys g8 and g8 + 8: the lane's 4 * D16 codes of each
+                constexpr int kWords = D16 % 4 == 0 ? 4 : 2;
+#pragma unroll
+                for (int k = 0; k < D16; k += kWords) {
+                    uint32_t u[kWords], v[kWords];
+                    lds_words<kWords>(u, kt + g8 * S::kKeyPitch + t4 * 4 * D16 + 4 * k);
+                    lds_words<kWords>(v, kt + (g8 + 8) * S::kKeyPitch + t4 * 4 * D16 + 4 * k);
+#pragma unroll
+                    for (int i = 0; i < kWords; ++i) {
+                        const uint32_t f[4] = {halves(u[i]), halves(v[i]), halves(u[i] >> 16), halves(v[i] >> 16)};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) mma<true>(x[n], f, qf[n][k + i][0], qf[n][k + i][1]);
+                    }
+                }
+                uint32_t ke[2], ve[2];
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const uint32_t from = kt + (g8 + 8 * j) * S::kKeyPitch + t4 * 4 * D16;
-                    constexpr int kWords = D16 % 4 == 0 ? 4 : 2;
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(ke[j]) : "r"(et + g8 + 8 * j));
+                    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(ve[j]) : "r"(et + 16 + g8 + 8 * j));
+                    value_e[j] = static_cast<float>(static_cast<int>(ve[j]) - 127);
 #pragma unroll
-                    for (int k = 0; k < D16; k += kWords) {
-                        uint32_t w[kWords];
-                        lds_words<kWords>(w, from + 4 * k);
-#pragma unroll
-                        for (int i = 0; i < kWords; ++i) mma<true>(x[j], qf[k + i], halves(w[i]), halves(w[i] >> 16));
+                    for (int n = 0; n < NT; ++n) {
+                        x[n][2 * j] *= scale_of(ke[j]);
+                        x[n][2 * j + 1] *= scale_of(ke[j]);
                     }
-                    uint16_t ke, ve;
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(ke) : "r"(et + 8 * j + 2 * t4));
-                    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(ve) : "r"(et + 16 + 8 * j + 2 * t4));
-                    const float k0 = scale_of(ke & 255u), k1 = scale_of(ke >> 8);
-                    x[j][0] *= k0; x[j][1] *= k1; x[j][2] *= k0; x[j][3] *= k1;
-                    value_e[j][0] = static_cast<float>(static_cast<int>(ve & 255u) - 127);
-                    value_e[j][1] = static_cast<float>(static_cast<int>(ve >> 8) - 127);
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < D16; ++k) {
                     uint32_t f[4];
-                    ldsm4(f, kt + ((lane & 7) + ((lane >> 4) << 3)) * S::kKeyPitch + (k * 16 + (((lane >> 3) & 1) << 3)) * 2);
-                    mma<false>(x[0], qf[k], f[0], f[1]);
-                    mma<false>(x[1], qf[k], f[2], f[3]);
+                    ldsm4(f, kt + (lane & 15) * S::kKeyPitch + (k * 16 + ((lane >> 4) << 3)) * 2);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma<false>(x[n], f, qf[n][k][0], qf[n][k][1]);
                 }
             }
             const bool all_seen = t + 15 <= p0 && (a.window == 0 || t > p1 - a.window || t + 15 < a.sinks) && p0 >= 0;
-            uint32_t weights[4];
-            float turn[2] = {1.0f, 1.0f};
-            float w[2][4] = {};
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                if (i == 1 && !second) break;
-                float top = -INFINITY, top_ref = -INFINITY;
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[n][i] *= to_score[n][i & 1];
                 if (a.cap > 0.0f) {   // a polynomial where all of the warp's scores lie within the cap
-                    float u[4] = {x[0][2 * i] * to_score[i], x[0][2 * i + 1] * to_score[i], x[1][2 * i] * to_score[i], x[1][2 * i + 1] * to_score[i]};
-                    if (__all_sync(0xffffffffu, fmaxf(fmaxf(fabsf(u[0]), fabsf(u[1])), fmaxf(fabsf(u[2]), fabsf(u[3]))) <= 1.0f)) {
-                        unpair(tanh_inner2(pair(u[0], u[1])), u[0], u[1]);
-                        unpair(tanh_inner2(pair(u[2], u[3])), u[2], u[3]);
+                    if (__all_sync(0xffffffffu, fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3]))) <= 1.0f)) {
+                        unpair(tanh_inner2(pair(x[n][0], x[n][1])), x[n][0], x[n][1]);
+                        unpair(tanh_inner2(pair(x[n][2], x[n][3])), x[n][2], x[n][3]);
                     } else {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) u[e] = tanhf(u[e]);
+                        for (int i = 0; i < 4; ++i) x[n][i] = tanhf(x[n][i]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) x[e >> 1][2 * i + (e & 1)] = u[e];
+                    for (int i = 0; i < 4; ++i) x[n][i] *= cap_log2;
                 }
+            }
+            if (!all_seen) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (!visible(a, t + g8 + 8 * (i >> 1), pos[n][i & 1])) x[n][i] = -INFINITY;
+            }
+            // A row's maximum only has to be near: as long as no score is far beyond it, nothing is exchanged between the lanes.
+            bool grow = false;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float top = fmaxf(x[n][e], x[n][2 + e]);
+                    grow = grow || top > m[n][e] + kGrowth || (m[n][e] == -INFINITY && top > -INFINITY);
+                    if (CODES) grow = grow || fmaxf(x[n][e] + value_e[0], x[n][2 + e] + value_e[1]) > ref[n][e] + kGrowth;
+                }
+            if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        float v = x[j][2 * i + e] * (a.cap > 0.0f ? a.cap * kLog2e : to_score[i]);
-                        if (!all_seen && !visible(a, t + 8 * j + 2 * t4 + e, pos[i])) v = -INFINITY;
-                        x[j][2 * i + e] = v;
-                        top = fmaxf(top, v);
-                        if (CODES) top_ref = fmaxf(top_ref, v + value_e[j][e]);
-                    }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float now = fmaxf(m[i], top), use = now == -INFINITY ? 0.0f : now;   // nothing seen yet: every weight is 2^-inf = 0
-                const float f = exp2_fast(m[i] - use);
-                m[i] = now;
-                l[i] *= f;
-                float use_ref = use;
-                if constexpr (CODES) {
-                    top_ref = fmaxf(top_ref, __shfl_xor_sync(0xffffffffu, top_ref, 1));
-                    top_ref = fmaxf(top_ref, __shfl_xor_sync(0xffffffffu, top_ref, 2));
-                    const float now_ref = fmaxf(ref[i], top_ref);
-                    use_ref = now_ref == -INFINITY ? 0.0f : now_ref;
-                    turn[i] = exp2_fast(ref[i] - use_ref);
-                    ref[i] = now_ref;
-                } else {
-                    turn[i] = f;
-                }
+                        float top = fmaxf(x[n][e], x[n][2 + e]), top_ref = CODES ? fmaxf(x[n][e] + value_e[0], x[n][2 + e] + value_e[1]) : 0.0f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+                        for (int o = 4; o < 32; o <<= 1) {
+                            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                            if (CODES) top_ref = fmaxf(top_ref, __shfl_xor_sync(0xffffffffu, top_ref, o));
+                        }
+                        const float now = fmaxf(m[n][e], top), now_ref = CODES ? fmaxf(ref[n][e], top_ref) : now;
+                        const float f = now == -INFINITY ? 1.0f : exp2_fast(m[n][e] - now), f_ref = now_ref == -INFINITY ? 1.0f : exp2_fast(ref[n][e] - now_ref);
+                        l[n][e] *= f;
+                        m[n][e] = now;
+                        ref[n][e] = now_ref;
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float p = exp2_fast(x[j][2 * i + e] - use);
-                        l[i] += p;
-                        w[j][2 * i + e] = CODES ? exp2_fast(x[j][2 * i + e] + value_e[j][e] - use_ref) : p;
+                        for (int u = 0; u < D16; ++u) {
+                            O[n][u][e] *= f_ref;
+                            O[n][u][2 + e] *= f_ref;
+                        }
                     }
             }
-            // weights as the second product's A operand: rows g8 / g8 + 8, keys 2 t4 and 2 t4 + 8
+            // weights: from rows of keys to the B operand's columns of rows of the tile by one transposition of 8 x 8 each
+            uint32_t weights[NT][2];
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
+            for (int n = 0; n < NT; ++n) {
+                float w[4];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) weights[2 * j + i] = CODES ? pack_half2(w[j][2 * i], w[j][2 * i + 1]) : ptx::pack_bf16x2(w[j][2 * i], w[j][2 * i + 1]);
-            if (__any_sync(0xffffffffu, turn[0] != 1.0f || turn[1] != 1.0f)) {
-#pragma unroll
-                for (int u = 0; u < 2 * D16; ++u) {
-                    O[u][0] *= turn[0];
-                    O[u][1] *= turn[0];
-                    O[u][2] *= turn[1];
-                    O[u][3] *= turn[1];
+                for (int i = 0; i < 4; ++i) {
+                    const int e = i & 1;
+                    const float against = m[n][e] == -INFINITY ? 0.0f : m[n][e];   // nothing seen yet: every weight is 2^-inf = 0
+                    const float p = exp2_fast(x[n][i] - against);
+                    l[n][e] += p;
+                    w[i] = CODES ? exp2_fast(x[n][i] + value_e[i >> 1] - (ref[n][e] == -INFINITY ? 0.0f : ref[n][e])) : p;
                 }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) weights[n][j] = transposed(CODES ? pack_half2(w[2 * j], w[2 * j + 1]) : ptx::pack_bf16x2(w[2 * j], w[2 * j + 1]));
             }
             if constexpr (CODES) {
-                // dimensions g8 * 2 D16 + u of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: column g8 of tile u
+                // dimensions g8 * 2 D16 + ... of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: the product's rows g8 and g8 + 8 of step u are dimensions 2 u and 2 u + 1 among them
                 constexpr int kWords = D16 / 2;
                 uint32_t c[4][kWords];
 #pragma unroll
@@ -422,18 +448,20 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 for (int i = 0; i < kWords; ++i) {
                     const uint32_t lo0 = __byte_perm(c[0][i], c[1][i], 0x5140), lo1 = __byte_perm(c[0][i], c[1][i], 0x7362);
                     const uint32_t hi0 = __byte_perm(c[2][i], c[3][i], 0x5140), hi1 = __byte_perm(c[2][i], c[3][i], 0x7362);
-                    mma<true>(O[4 * i], weights, halves(lo0), halves(hi0));
-                    mma<true>(O[4 * i + 1], weights, halves(lo0 >> 16), halves(hi0 >> 16));
-                    mma<true>(O[4 * i + 2], weights, halves(lo1), halves(hi1));
-                    mma<true>(O[4 * i + 3], weights, halves(lo1 >> 16), halves(hi1 >> 16));
+                    const uint32_t f0[4] = {halves(lo0), halves(lo0 >> 16), halves(hi0), halves(hi0 >> 16)}, f1[4] = {halves(lo1), halves(lo1 >> 16), halves(hi1), halves(hi1 >> 16)};
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma<true>(O[n][2 * i], f0, weights[n][0], weights[n][1]);
+                        mma<true>(O[n][2 * i + 1], f1, weights[n][0], weights[n][1]);
+                    }
                 }
             } else {
 #pragma unroll
-                for (int u = 0; u < 2 * D16; u += 2) {
+                for (int u = 0; u < D16; ++u) {
                     uint32_t f[4];
-                    ldsm4t(f, vt + (lane & 15) * S::kValuePitch + (u * 8 + ((lane >> 4) << 3)) * 2);
-                    mma<false>(O[u], weights, f[0], f[1]);
-                    mma<false>(O[u + 1], weights, f[2], f[3]);
+                    ldsm4t(f, vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kValuePitch + (16 * u + (((lane >> 3) & 1) << 3)) * 2);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) mma<false>(O[n][u], f, weights[n][0], weights[n][1]);
                 }
             }
             __syncwarp();   // this stage may be filled again
@@ -442,42 +470,41 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 
         // ---- the warps' parts
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (t4 == 0) {
-                merge_ml[warp][g8 + 8 * i][0] = m[i];
-                merge_ml[warp][g8 + 8 * i][1] = l[i];
-            }
-        }
-        __syncthreads();   // every warp is done with its ring: the sums take its place
-        float *merge = reinterpret_cast<float *>(tokens_smem + kTokensRows * S::kQPitch);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int r = g8 + 8 * i;
-            float top = merge_ml[0][r][0];
+            for (int e = 0; e < 2; ++e) {
 #pragma unroll
-            for (int w = 1; w < kTokensWarps; ++w) top = fmaxf(top, merge_ml[w][r][0]);
-            float sum = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kTokensWarps; ++w)
-                sum += merge_ml[w][r][1] * share_of(merge_ml[w][r][0], top);
-            if (warp == 0 && t4 == 0) {
-                total_ml[r][0] = top;
-                total_ml[r][1] = sum;
-            }
-            const float f = share_of(CODES ? ref[i] : m[i], top);
-#pragma unroll
-            for (int u = 0; u < 2 * D16; ++u) {
-                float *to = merge + (warp * kTokensRows + r) * S::kMergePitch;
-                if constexpr (CODES) {
-                    to[(2 * t4) * 2 * D16 + u] = O[u][2 * i] * f;
-                    to[(2 * t4 + 1) * 2 * D16 + u] = O[u][2 * i + 1] * f;
-                } else {
-                    *reinterpret_cast<float2 *>(to + u * 8 + 2 * t4) = make_float2(O[u][2 * i] * f, O[u][2 * i + 1] * f);
+                for (int o = 4; o < 32; o <<= 1) l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], o);
+                if (g8 == 0) {
+                    merge_ml[warp][8 * n + 2 * t4 + e][0] = m[n][e];
+                    merge_ml[warp][8 * n + 2 * t4 + e][1] = l[n][e];
                 }
             }
-        }
+        __syncthreads();   // every warp is done with its ring: the sums take its place
+        float *merge = reinterpret_cast<float *>(tokens_smem + kRows * S::kQPitch);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 8 * n + 2 * t4 + e;
+                float top = merge_ml[0][r][0];
+#pragma unroll
+                for (int w = 1; w < kTokensWarps; ++w) top = fmaxf(top, merge_ml[w][r][0]);
+                float sum = 0.0f;
+#pragma unroll
+                for (int w = 0; w < kTokensWarps; ++w) sum += merge_ml[w][r][1] * share_of(merge_ml[w][r][0], top);
+                if (warp == 0 && g8 == 0) {
+                    total_ml[r][0] = top;
+                    total_ml[r][1] = sum;
+                }
+                const float f = share_of(CODES ? ref[n][e] : m[n][e], top);
+                float *to = merge + (warp * kRows + r) * S::kMergePitch;
+#pragma unroll
+                for (int u = 0; u < D16; ++u) {
+                    to[CODES ? g8 * 2 * D16 + 2 * u : 16 * u + g8] = O[n][u][e] * f;
+                    to[CODES ? g8 * 2 * D16 + 2 * u + 1 : 16 * u + g8 + 8] = O[n][u][2 + e] * f;
+                }
+            }
         __syncthreads();
         auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
             const int packed = packed0 + r, row = place.q.row0 + a.shares.divide(packed), head = place.g * a.share + packed - a.shares.divide(packed) * a.share;
@@ -500,7 +527,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 #pragma unroll
             for (int w = 0; w < kTokensWarps; ++w) {
                 float u[8];
-                load8(u, merge + (w * kTokensRows + r) * S::kMergePitch + c * 8);
+                load8(u, merge + (w * kRows + r) * S::kMergePitch + c * 8);
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += u[e];
             }
@@ -508,7 +535,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 finish(r, c, v, total_ml[r][0], total_ml[r][1]);
             } else {
                 store8(slot_own + r * dim + c * 8, v);
-                if (c == 0) *reinterpret_cast<float2 *>(slot_own + kTokensRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
+                if (c == 0) *reinterpret_cast<float2 *>(slot_own + kTokensMaxRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
             }
         }
         if (!part.whole) {
@@ -523,22 +550,42 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             }
             __syncthreads();
             if (arrived_last) {
+                // the parts' maxima and sums first, into shared memory, all of them under way at once; a part's factor takes the place of its maximum
+                auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats; };
+                const int parts = b1 - b0 + 1;
+                float2 *ml = reinterpret_cast<float2 *>(merge);
+                for (int i = threadIdx.x; i < parts * rows; i += kTokensThreads) ml[i] = __ldcg(reinterpret_cast<const float2 *>(slot(b0 + i / rows) + kTokensMaxRows * 128 + 2 * (i % rows)));
+                __syncthreads();
+                for (int r = warp; r < rows; r += kTokensWarps) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[i * rows + r].x);
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    for (int i = lane; i < parts; i += 32) {
+                        float2 &v = ml[i * rows + r];
+                        v.x = share_of(v.x, top);
+                        sum = fmaf(v.y, v.x, sum);
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) {
+                        total_ml[r][0] = top;
+                        total_ml[r][1] = sum;
+                    }
+                }
+                __syncthreads();
                 for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
                     const int r = i / pieces, c = i % pieces;
-                    auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats; };
-                    float top = -INFINITY, sum = 0.0f, v[8] = {};
-                    for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(slot(b) + kTokensRows * 128 + 2 * r));
-#pragma unroll 4
-                    for (int b = b0; b <= b1; ++b) {
-                        const float *from = slot(b);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(from + kTokensRows * 128 + 2 * r));
-                        const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from + r * dim + c * 8)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + r * dim + c * 8 + 4));
-                        const float f = share_of(ml.x, top);
-                        sum = fmaf(ml.y, f, sum);
+                    float v[8] = {};
+#pragma unroll 8
+                    for (int n = 0; n < parts; ++n) {
+                        const float *from = slot(b0 + n) + r * dim + c * 8;
+                        const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + 4));
+                        const float f = ml[n * rows + r].x;
                         v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
                         v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
                     }
-                    finish(r, c, v, top, sum);
+                    finish(r, c, v, total_ml[r][0], total_ml[r][1]);
                 }
             }
         }
