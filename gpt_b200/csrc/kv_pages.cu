@@ -5,6 +5,7 @@
 
 #include "ctx_internal.h"
 #include "paged_prompt_sm100.cuh"
+#include "paged_rows.cuh"
 
 using namespace gptb200;
 
@@ -100,19 +101,6 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
     return GPTB200_OK;
 }
 
-template <typename T>
-int attention_rows(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
-{
-    const long long warps = 1LL * a.batch.rows * a.heads, blocks = (warps + kvp::kRowWarps - 1) / kvp::kRowWarps;
-    if (blocks > INT_MAX) return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %d heads", a.batch.rows, a.heads);
-    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(static_cast<unsigned>(blocks)), dim3(kvp::kRowWarps * 32), 0, a); };
-    CUDA_TRY(ctx, kind == GPTB200_KV_E4M3 ? launch(kvp::attention_rows_kernel<T, kvp::KIND_E4M3>)
-                  : kind == GPTB200_KV_F32 ? launch(kvp::attention_rows_kernel<T, kvp::KIND_F32>)
-                                           : launch(kvp::attention_rows_kernel<T, kvp::KIND_BF16>));
-    ctx->launches++;
-    return GPTB200_OK;
-}
-
 // A kernel that cuts the line of work into equal ranges: `per_sm` blocks on every SM, a part of a tile in scratch for either end of a range.
 template <typename Args>
 int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, int smem, int per_sm, int most_blocks, int part_floats)
@@ -157,6 +145,17 @@ int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind, bool f
         case 3: return run_tokens<6>(ctx, args, codes, few);
         default: return run_tokens<8>(ctx, args, codes, few);
     }
+}
+
+template <typename T, int KIND>
+int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, int max_rows)
+{
+    kvp::TokensArgs args{a, {}, {1, kvp::kFewKeys, 1, 3}};
+    if (max_rows <= 1) return run_line(ctx, kvp::paged_few_kernel<T, KIND, 1>, args, kvp::kTokensThreads, kvp::few_smem(1), kvp::kFewPerSm, kvp::few_blocks(1), kvp::kTokensPart);
+    args.cut.tile_rows = 4;
+    if (max_rows <= 4) return run_line(ctx, kvp::paged_few_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::few_smem(4), kvp::kFewPerSm, kvp::few_blocks(4), kvp::kTokensPart);
+    args.cut = {kvp::kRowsTile, kvp::kRowsKeys, 1, 5};
+    return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), kvp::kRowsPerSm, kvp::kRowsPerSm * 160, kvp::kTokensPart);
 }
 
 template <int NB, bool CODES>
@@ -223,9 +222,14 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     a.scale = scale; a.cap = cap;
     a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
     a.sinks = a.window ? sinks : 0;
-    if (dtype == GPTB200_DTYPE_BF16 && pages->kind != GPTB200_KV_F32)
-        return 1LL * rows->max_new * a.share > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind, 1LL * rows->max_new * a.share <= 8);
-    return dtype == GPTB200_DTYPE_F32 ? attention_rows<float>(ctx, a, pages->kind) : attention_rows<__nv_bfloat16>(ctx, a, pages->kind);
+    // queries of one key / value head that meet its keys together, at most (rows that one sequence has more of are further tiles)
+    const int max_rows = static_cast<int>(std::min<long long>(1LL * rows->max_new * a.share, INT_MAX));
+    if (dtype == GPTB200_DTYPE_F32) {
+        return pages->kind == GPTB200_KV_E4M3 ? run_fma<float, kvp::KIND_E4M3>(ctx, a, max_rows)
+               : pages->kind == GPTB200_KV_F32 ? run_fma<float, kvp::KIND_F32>(ctx, a, max_rows) : run_fma<float, kvp::KIND_BF16>(ctx, a, max_rows);
+    }
+    if (pages->kind == GPTB200_KV_F32) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, a, max_rows);
+    return max_rows > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind, max_rows <= 8);
 }
 
 }  // extern "C"

@@ -694,26 +694,5 @@ __device__ void attention_row(const Attention &a, int s, int position, int row, 
     if (a.lse && lane == 0) a.lse[static_cast<long long>(row) * a.heads + head] = keys > 0 ? top + logf(l) : -INFINITY;
 }
 
-constexpr int kRowWarps = 4;
-
-// A warp per (row, head).
-template <typename T, int KIND>
-__global__ void __launch_bounds__(kRowWarps * 32)
-attention_rows_kernel(const Attention a)
-{
-    grid_dependency_wait();
-    grid_dependency_launch();
-    const long long w = static_cast<long long>(blockIdx.x) * kRowWarps + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
-    if (w >= static_cast<long long>(a.batch.rows) * a.heads) return;
-    const int row = static_cast<int>(w / a.heads), head = static_cast<int>(w % a.heads);
-    const int s = sequence_of_row(a.batch, row, lane);
-    if (s < 0) return;
-    const Sequence q = sequence_of(a.batch, s);
-    const int nth = row - q.row0;
-    if (nth < 0 || nth >= q.count) return;
-    attention_row<T, KIND>(a, s, q.pos0 + nth, row, head, lane);
-}
-
 }  // namespace kvp
 }  // namespace gptb200

@@ -157,6 +157,107 @@ struct TokensArgs {
     Cut cut;
 };
 
+// The end of a tile, for a block of kTokensThreads threads that holds its rows' sums in shared memory: merge [SUMS][ROWS][pitch] weighted values (added up here) against
+// total_ml [ROWS] = (maximum in base 2, sum).  A whole tile is stored; else the part goes to scratch, and the block that arrives last puts the parts together.
+// sums: room for (blocks of the grid) x ROWS pairs, which may be `merge` itself.  bad_rows is zero on entry.
+template <typename T, int KIND, int ROWS, int SUMS>
+__device__ __forceinline__ void finish_tile(const Attention &a, const Parts &parts, const Place &place, const Part &part, const Range &range, int rows, const float *merge, int pitch,
+                                            float (*total_ml)[2], float2 *sums, int *bad_rows, int *arrived_last)
+{
+    constexpr float kLn2 = 0.69314718055994531f;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.pages.dim, pieces = dim / 8, packed0 = place.tile * ROWS;
+    auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
+        const int packed = packed0 + r, token = a.shares.divide(packed), row = place.q.row0 + token, head = place.g * a.share + packed - token * a.share;
+        const bool sees = place.q.pos0 + token >= 0;   // itself at least
+        const float inv = sees ? 1.0f / sum : 0.0f;
+        bool fine = true;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            v[e] *= inv;
+            fine = fine && fabsf(v[e]) <= FLT_MAX;
+        }
+        if (!fine) atomicOr(bad_rows, 1 << r);
+        store8(static_cast<T *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
+        if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
+    };
+    float *own = parts.base + (2LL * blockIdx.x + (part.first_block >= range.begin)) * parts.floats;
+    for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
+        const int r = i / pieces, c = i % pieces;
+        float v[8] = {};
+#pragma unroll
+        for (int w = 0; w < SUMS; ++w) {
+            float u[8];
+            load8(u, merge + (w * ROWS + r) * pitch + c * 8);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += u[e];
+        }
+        if (part.whole) {
+            finish(r, c, v, total_ml[r][0], total_ml[r][1]);
+        } else {
+            store8(own + r * dim + c * 8, v);
+            if (c == 0) *reinterpret_cast<float2 *>(own + kTokensMaxRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
+        }
+    }
+    if (!part.whole) {
+        const int b0 = static_cast<int>(part.first_block / range.per), b1 = static_cast<int>(part.last_block / range.per), count = b1 - b0 + 1;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const unsigned int before = atomicAdd(parts.tickets + b0, 1u);
+            *arrived_last = before == static_cast<unsigned int>(b1 - b0);
+            if (*arrived_last) parts.tickets[b0] = 0u;
+            __threadfence();
+        }
+        __syncthreads();
+        if (*arrived_last) {
+            // the parts' maxima and sums first, all of them under way at once; a part's factor takes the place of its maximum
+            auto slot = [&](int b) { return parts.base + (2LL * b + (b == b0)) * parts.floats; };
+            for (int i = threadIdx.x; i < count * rows; i += kTokensThreads) sums[i] = __ldcg(reinterpret_cast<const float2 *>(slot(b0 + i / rows) + kTokensMaxRows * 128 + 2 * (i % rows)));
+            __syncthreads();
+            for (int r = warp; r < rows; r += kTokensWarps) {
+                float top = -INFINITY, sum = 0.0f;
+                for (int i = lane; i < count; i += 32) top = fmaxf(top, sums[i * rows + r].x);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int i = lane; i < count; i += 32) {
+                    float2 &v = sums[i * rows + r];
+                    v.x = tok::share_of(v.x, top);
+                    sum = fmaf(v.y, v.x, sum);
+                }
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0) {
+                    total_ml[r][0] = top;
+                    total_ml[r][1] = sum;
+                }
+            }
+            __syncthreads();
+            for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
+                const int r = i / pieces, c = i % pieces;
+                float v[8] = {};
+#pragma unroll 8
+                for (int n = 0; n < count; ++n) {
+                    const float *from = slot(b0 + n) + r * dim + c * 8;
+                    const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + 4));
+                    const float f = sums[n * rows + r].x;
+                    v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
+                    v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
+                }
+                finish(r, c, v, total_ml[r][0], total_ml[r][1]);
+            }
+        }
+    }
+    __syncthreads();
+    // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is formed once more
+    // from its own keys alone.
+    for (int rest = *bad_rows, n = 0; rest; rest &= rest - 1, ++n) {
+        if (n % kTokensWarps != warp) continue;
+        const int packed = packed0 + __ffs(rest) - 1, token = a.shares.divide(packed);
+        attention_row<T, KIND>(a, place.s, place.q.pos0 + token, place.q.row0 + token, place.g * a.share + packed - token * a.share, lane);
+    }
+    __syncthreads();   // what the next tile writes again has been read
+}
+
 template <int D16, bool CODES, int NT>
 __global__ void __launch_bounds__(kTokensThreads, TokensShape<D16, CODES, NT>::kPerSm)
 paged_tokens_kernel(const __grid_constant__ TokensArgs args)
@@ -166,7 +267,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     constexpr int kRows = S::kRows;
     constexpr float kGrowth = CODES ? 8.0f : 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled: fp16 weights end at 2^16
     constexpr int kind = CODES ? KIND_E4M3 : KIND_BF16;
-    constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.69314718055994531f;
+    constexpr float kLog2e = 1.4426950408889634f;
     extern __shared__ __align__(16) uint8_t tokens_smem[];
     __shared__ float merge_ml[kTokensWarps][kRows][2], total_ml[kRows][2], row_power[kRows];
     __shared__ int bad_rows, arrived_last;
@@ -506,98 +607,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 }
             }
         __syncthreads();
-        auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
-            const int packed = packed0 + r, row = place.q.row0 + a.shares.divide(packed), head = place.g * a.share + packed - a.shares.divide(packed) * a.share;
-            const bool sees = place.q.pos0 + a.shares.divide(packed) >= 0;   // itself at least
-            const float inv = sees ? 1.0f / sum : 0.0f;
-            bool fine = true;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                v[e] *= inv;
-                fine = fine && fabsf(v[e]) <= FLT_MAX;
-            }
-            if (!fine) atomicOr(&bad_rows, 1 << r);
-            store8(static_cast<__nv_bfloat16 *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
-            if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
-        };
-        float *slot_own = args.parts.base + (2LL * blockIdx.x + (part.first_block >= range.begin)) * args.parts.floats;
-        for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
-            const int r = i / pieces, c = i % pieces;
-            float v[8] = {};
-#pragma unroll
-            for (int w = 0; w < kTokensWarps; ++w) {
-                float u[8];
-                load8(u, merge + (w * kRows + r) * S::kMergePitch + c * 8);
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += u[e];
-            }
-            if (part.whole) {
-                finish(r, c, v, total_ml[r][0], total_ml[r][1]);
-            } else {
-                store8(slot_own + r * dim + c * 8, v);
-                if (c == 0) *reinterpret_cast<float2 *>(slot_own + kTokensMaxRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
-            }
-        }
-        if (!part.whole) {
-            const int b0 = static_cast<int>(part.first_block / range.per), b1 = static_cast<int>(part.last_block / range.per);
-            __threadfence();
-            __syncthreads();
-            if (threadIdx.x == 0) {
-                const unsigned int before = atomicAdd(args.parts.tickets + b0, 1u);
-                arrived_last = before == static_cast<unsigned int>(b1 - b0);
-                if (arrived_last) args.parts.tickets[b0] = 0u;
-                __threadfence();
-            }
-            __syncthreads();
-            if (arrived_last) {
-                // the parts' maxima and sums first, into shared memory, all of them under way at once; a part's factor takes the place of its maximum
-                auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats; };
-                const int parts = b1 - b0 + 1;
-                float2 *ml = reinterpret_cast<float2 *>(merge);
-                for (int i = threadIdx.x; i < parts * rows; i += kTokensThreads) ml[i] = __ldcg(reinterpret_cast<const float2 *>(slot(b0 + i / rows) + kTokensMaxRows * 128 + 2 * (i % rows)));
-                __syncthreads();
-                for (int r = warp; r < rows; r += kTokensWarps) {
-                    float top = -INFINITY, sum = 0.0f;
-                    for (int i = lane; i < parts; i += 32) top = fmaxf(top, ml[i * rows + r].x);
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                    for (int i = lane; i < parts; i += 32) {
-                        float2 &v = ml[i * rows + r];
-                        v.x = share_of(v.x, top);
-                        sum = fmaf(v.y, v.x, sum);
-                    }
-#pragma unroll
-                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                    if (lane == 0) {
-                        total_ml[r][0] = top;
-                        total_ml[r][1] = sum;
-                    }
-                }
-                __syncthreads();
-                for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
-                    const int r = i / pieces, c = i % pieces;
-                    float v[8] = {};
-#pragma unroll 8
-                    for (int n = 0; n < parts; ++n) {
-                        const float *from = slot(b0 + n) + r * dim + c * 8;
-                        const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + 4));
-                        const float f = ml[n * rows + r].x;
-                        v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
-                        v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
-                    }
-                    finish(r, c, v, total_ml[r][0], total_ml[r][1]);
-                }
-            }
-        }
-        __syncthreads();
-        // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is
-        // formed once more from its own keys alone.
-        for (int rest = bad_rows, n = 0; rest; rest &= rest - 1, ++n) {
-            if (n % kTokensWarps != warp) continue;
-            const int packed = packed0 + __ffs(rest) - 1;
-            attention_row<__nv_bfloat16, kind>(a, place.s, place.q.pos0 + a.shares.divide(packed), place.q.row0 + a.shares.divide(packed), place.g * a.share + packed - a.shares.divide(packed) * a.share, lane);
-        }
-        __syncthreads();   // what the next tile writes again has been read
+        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, range, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), &bad_rows, &arrived_last);
         if (at < range.end && !next_tile(a, place, args.cut)) break;
     }
 }
