@@ -40,7 +40,7 @@ EXPORTED_SYMBOLS = [
     "gptb200_softmax_cross_entropy_inplace", "gptb200_row_loss_mean", "gptb200_cross_entropy_loss_from_logits",
     "gptb200_adamw_step", "gptb200_scale_and_clip_grad", "gptb200_memory_info", "gptb200_clip_adamw_packed",
     "gptb200_embedding_decode", "gptb200_kv_cache_fill", "gptb200_attention_decode", "gptb200_advance_position",
-    "gptb200_kv_pages_write", "gptb200_kv_pages_read", "gptb200_attention_paged",
+    "gptb200_kv_pages_write", "gptb200_kv_pages_read", "gptb200_attention_paged", "gptb200_plan_attention_paged",
     "gptb200_loader_create", "gptb200_loader_destroy", "gptb200_loader_num_samples", "gptb200_loader_reset_epoch", "gptb200_loader_next_batch",
     "gptb200_bias_grad_noalloc",
     "gptb200_decoder_check_config", "gptb200_decoder_load", "gptb200_decoder_destroy", "gptb200_decoder_context", "gptb200_decoder_vocab",
@@ -144,6 +144,7 @@ def load_library(path: str | None = None) -> ctypes.CDLL:
         "gptb200_kv_pages_write": (i, [vp, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows), fp, ctypes.c_longlong, fp, ctypes.c_longlong, i]),
         "gptb200_kv_pages_read": (i, [vp, fp, ctypes.c_longlong, fp, ctypes.c_longlong, i, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows)]),
         "gptb200_attention_paged": (i, [vp, fp, ctypes.c_longlong, fp, fp, ctypes.c_longlong, i, i, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows), f32, f32, i, i]),
+        "gptb200_plan_attention_paged": (i, [i, i, i, ctypes.POINTER(_KvPages), ctypes.POINTER(_KvRows), f32, f32, i, i, ctypes.POINTER(i)]),
         "gptb200_loader_create": (i, [ctypes.POINTER(vp), ctypes.c_char_p, i]),
         "gptb200_loader_destroy": (i, [vp]),
         "gptb200_loader_num_samples": (ctypes.c_longlong, [vp]),
@@ -264,6 +265,18 @@ class KvRows:
     def __init__(self, row_starts, lengths, page_table, sequences: int, table_pitch: int, rows: int, max_new: int):
         self._tensors = (row_starts, lengths, page_table)
         self.struct = _KvRows(_ptr(row_starts), _ptr(lengths), _ptr(page_table), sequences, table_pitch, rows, max_new)
+
+
+PAGED_KERNELS = {0: "none", 1: "tokens", 2: "prompt", 3: "few", 4: "rows"}
+
+
+def plan_attention_paged(num_sms: int, dtype: int, heads: int, pages: KvPages, rows: KvRows, scale: float, cap: float = 0.0, window: int = 0, sinks: int = 0) -> dict:
+    """How Backend.attention_paged runs a call (host logic only); see gptb200_plan_attention_paged in include/gptb200.h.  Raises where the call would be refused."""
+    out = (ctypes.c_int * 4)()
+    rc = load_library().gptb200_plan_attention_paged(num_sms, dtype, heads, pages.struct, rows.struct, scale, cap, window, sinks, out)
+    if rc != 0:
+        raise GptB200Error(rc, "gptb200_plan_attention_paged")
+    return dict(kernel=PAGED_KERNELS[out[0]], tile_rows=out[1], blocks=out[2], scratch_kib=out[3])
 
 
 class Backend:

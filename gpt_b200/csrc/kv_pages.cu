@@ -51,7 +51,7 @@ int check_pages(gptb200_ctx *ctx, const gptb200_kv_pages *p, const gptb200_kv_ro
     while ((1 << shift) < p->page_tokens) ++shift;
     *pages = {p->data, p->kind == GPTB200_KV_E4M3 ? p->scales : nullptr, p->num_pages, shift, p->kv_heads, p->dim};
     const long long capacity = std::min<long long>(static_cast<long long>(b->table_pitch) << shift, 1 << 30);
-    *batch = {b->row_starts, b->lengths, b->page_table, b->sequences, b->table_pitch, b->rows, static_cast<int>(capacity), ctx->d_status};
+    *batch = {b->row_starts, b->lengths, b->page_table, b->sequences, b->table_pitch, b->rows, static_cast<int>(capacity), ctx ? ctx->d_status : nullptr};
     return GPTB200_OK;
 }
 
@@ -98,6 +98,45 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
     };
     CUDA_TRY(ctx, dtype == GPTB200_DTYPE_F32 ? launch_kind(float()) : launch_kind(__nv_bfloat16()));
     ctx->launches++;
+    return GPTB200_OK;
+}
+
+// Which kernel attends, and how its grid is made; host logic.
+struct PagedPlan {
+    int kernel;       // 0: nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 few / sixteen rows on FMAs
+    int tile_rows, per_sm, part_floats;
+};
+enum { PAGED_NONE = 0, PAGED_TOKENS = 1, PAGED_PROMPT = 2, PAGED_FEW = 3, PAGED_ROWS = 4 };
+
+PagedPlan plan_paged(int dtype, int kind, long long max_rows)
+{
+    const bool codes = kind == GPTB200_KV_E4M3;
+    if (dtype == GPTB200_DTYPE_F32 || kind == GPTB200_KV_F32) {
+        if (max_rows <= 1) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kTokensPart};
+        if (max_rows <= 4) return {PAGED_FEW, 4, kvp::kFewPerSm, kvp::kTokensPart};
+        return {PAGED_ROWS, kvp::kRowsTile, kvp::kRowsPerSm, kvp::kTokensPart};
+    }
+    if (max_rows > 32) return {PAGED_PROMPT, kvp::kPromptRows, 1, kvp::kPromptPart};
+    return {PAGED_TOKENS, max_rows <= 8 ? 8 : 16, codes ? 3 : 2, kvp::kTokensPart};
+}
+
+int check_attention(gptb200_ctx *ctx, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks, kvp::Attention *a)
+{
+    if (dtype != GPTB200_DTYPE_BF16 && dtype != GPTB200_DTYPE_F32) return fail(ctx, GPTB200_ERR_INVALID_ARG, "dtype %d is unknown", dtype);
+    const int rc = check_pages(ctx, pages, rows, &a->pages, &a->batch);
+    if (rc != GPTB200_OK) return rc;
+    if (heads <= 0 || heads % pages->kv_heads) return fail(ctx, GPTB200_ERR_INVALID_ARG, "%d heads are not a multiple of the cache's %d", heads, pages->kv_heads);
+    if (!(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap) || window < 0 || sinks < 0)
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "scale %g, cap %g, window %d, first tokens %d", scale, cap, window, sinks);
+    if (1LL * heads * pages->dim > INT_MAX / 64 || 1LL * rows->rows * heads > INT_MAX - 256)
+        return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %lld elements", rows->rows, 1LL * heads * pages->dim);
+    a->heads = heads;
+    a->share = heads / pages->kv_heads;
+    a->shares = kvp::divisor(a->share);
+    a->scale = scale;
+    a->cap = cap;
+    a->window = window >= a->batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
+    a->sinks = a->window ? sinks : 0;
     return GPTB200_OK;
 }
 
@@ -148,14 +187,15 @@ int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind, bool f
 }
 
 template <typename T, int KIND>
-int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, int max_rows)
+int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, const PagedPlan &plan)
 {
-    kvp::TokensArgs args{a, {}, {1, kvp::kFewKeys, 1, 3}};
-    if (max_rows <= 1) return run_line(ctx, kvp::paged_few_kernel<T, KIND, 1>, args, kvp::kTokensThreads, kvp::few_smem(1), kvp::kFewPerSm, kvp::few_blocks(1), kvp::kTokensPart);
-    args.cut.tile_rows = 4;
-    if (max_rows <= 4) return run_line(ctx, kvp::paged_few_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::few_smem(4), kvp::kFewPerSm, kvp::few_blocks(4), kvp::kTokensPart);
-    args.cut = {kvp::kRowsTile, kvp::kRowsKeys, 1, 5};
-    return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), kvp::kRowsPerSm, kvp::kRowsPerSm * 160, kvp::kTokensPart);
+    kvp::TokensArgs args{a, {}, {plan.tile_rows, kvp::kFewKeys, 1, 5}};
+    if (plan.kernel == PAGED_FEW) {
+        return plan.tile_rows == 1 ? run_line(ctx, kvp::paged_few_kernel<T, KIND, 1>, args, kvp::kTokensThreads, kvp::few_smem(1), plan.per_sm, kvp::kFewBlocks, plan.part_floats)
+                                   : run_line(ctx, kvp::paged_few_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::few_smem(4), plan.per_sm, kvp::kFewBlocks, plan.part_floats);
+    }
+    args.cut.keys = kvp::kRowsKeys;
+    return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
 }
 
 template <int NB, bool CODES>
@@ -203,33 +243,36 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
                             const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks)
 {
     if (!ctx) return GPTB200_ERR_INVALID_ARG;
-    if (dtype != GPTB200_DTYPE_BF16 && dtype != GPTB200_DTYPE_F32) return fail(ctx, GPTB200_ERR_INVALID_ARG, "dtype %d is unknown", dtype);
     kvp::Attention a{};
-    int rc = check_pages(ctx, pages, rows, &a.pages, &a.batch);
+    int rc = check_attention(ctx, dtype, heads, pages, rows, scale, cap, window, sinks, &a);
     if (rc != GPTB200_OK) return rc;
-    if (heads <= 0 || heads % pages->kv_heads) return fail(ctx, GPTB200_ERR_INVALID_ARG, "%d heads are not a multiple of the cache's %d", heads, pages->kv_heads);
-    if (!(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap) || window < 0 || sinks < 0)
-        return fail(ctx, GPTB200_ERR_INVALID_ARG, "scale %g, cap %g, window %d, first tokens %d", scale, cap, window, sinks);
     if (rows->sequences == 0 || rows->rows == 0) return GPTB200_OK;
     const long long width = 1LL * heads * pages->dim;
     if ((rc = check_rows(ctx, "q", q, q_pitch, width, dtype)) != GPTB200_OK || (rc = check_rows(ctx, "out", out, out_pitch, width, dtype)) != GPTB200_OK) return rc;
-    if (width > INT_MAX / 64 || 1LL * rows->rows * heads > INT_MAX - 256) return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %lld elements", rows->rows, width);
+    if (out == q) return fail(ctx, GPTB200_ERR_INVALID_ARG, "out is q");
     OnDevice device;
     CUDA_TRY(ctx, device.enter(ctx->device));
     a.q = q; a.out = out; a.lse = lse; a.q_pitch = q_pitch; a.out_pitch = out_pitch;
-    a.heads = heads; a.share = heads / pages->kv_heads;
-    a.shares = kvp::divisor(a.share);
-    a.scale = scale; a.cap = cap;
-    a.window = window >= a.batch.capacity ? 0 : window;   // no sequence is longer: it hides nothing
-    a.sinks = a.window ? sinks : 0;
-    // queries of one key / value head that meet its keys together, at most (rows that one sequence has more of are further tiles)
-    const int max_rows = static_cast<int>(std::min<long long>(1LL * rows->max_new * a.share, INT_MAX));
-    if (dtype == GPTB200_DTYPE_F32) {
-        return pages->kind == GPTB200_KV_E4M3 ? run_fma<float, kvp::KIND_E4M3>(ctx, a, max_rows)
-               : pages->kind == GPTB200_KV_F32 ? run_fma<float, kvp::KIND_F32>(ctx, a, max_rows) : run_fma<float, kvp::KIND_BF16>(ctx, a, max_rows);
-    }
-    if (pages->kind == GPTB200_KV_F32) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, a, max_rows);
-    return max_rows > 32 ? attention_prompt(ctx, a, pages->kind) : attention_tokens(ctx, a, pages->kind, max_rows <= 8);
+    const PagedPlan plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share);
+    if (plan.kernel == PAGED_PROMPT) return attention_prompt(ctx, a, pages->kind);
+    if (plan.kernel == PAGED_TOKENS) return attention_tokens(ctx, a, pages->kind, plan.tile_rows == 8);
+    if (dtype == GPTB200_DTYPE_BF16) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, a, plan);
+    return pages->kind == GPTB200_KV_E4M3 ? run_fma<float, kvp::KIND_E4M3>(ctx, a, plan)
+           : pages->kind == GPTB200_KV_F32 ? run_fma<float, kvp::KIND_F32>(ctx, a, plan) : run_fma<float, kvp::KIND_BF16>(ctx, a, plan);
+}
+
+int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks, int *plan4)
+{
+    if (num_sms <= 0 || !plan4) return GPTB200_ERR_INVALID_ARG;
+    kvp::Attention a{};
+    const int rc = check_attention(nullptr, dtype, heads, pages, rows, scale, cap, window, sinks, &a);
+    if (rc != GPTB200_OK) return rc;
+    PagedPlan plan{};
+    if (rows->sequences > 0 && rows->rows > 0) plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share);
+    const int blocks = num_sms * plan.per_sm;
+    const int out[4] = {plan.kernel, plan.tile_rows, blocks, static_cast<int>((2LL * blocks * plan.part_floats * sizeof(float)) >> 10)};
+    for (int i = 0; i < 4; ++i) plan4[i] = out[i];
+    return GPTB200_OK;
 }
 
 }  // extern "C"

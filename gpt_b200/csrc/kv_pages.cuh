@@ -14,6 +14,7 @@
 #include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
+#include "../../include/gptb200.h"
 #include "gemm_sm100.cuh"
 
 namespace gptb200 {
@@ -425,8 +426,8 @@ __host__ __device__ inline bool visible(const Attention &a, int key, int positio
 //
 // A tile is a number of packed query rows of one sequence and key / value head: row i of the tile is head i % share of token i / share, so that a group's
 // query heads meet keys and values once.  A tile's work is the blocks of keys that any of its rows sees; all tiles' blocks form one line (sequence, key / value
-// head, tile, block), which is cut into equal ranges, one per block of the grid: whatever the lengths, all blocks do the same work.  A range may begin and
-// end inside a tile; such parts go to scratch as (maximum, sum, weighted values), and the block that arrives last at a tile adds them up in the order of
+// head, tile, block), which is cut into equal ranges, one per block of the grid: whatever the lengths, all blocks do nearly the same work.  A range may begin and
+// end inside a tile, though a cut within an eighth of a range from a tile's edge moves to the edge; such parts go to scratch as (maximum, sum, weighted values), and the block that arrives last at a tile adds them up in the order of
 // the line, so that results do not depend on who that is.
 
 struct KeyBlocks {
@@ -495,26 +496,65 @@ __host__ __device__ inline bool next_tile(const Attention &a, Place &p, const Cu
 }
 
 struct Range {
-    long long begin, end;   // this block's part of the line
+    long long begin, end;   // this block's part of the line; the last one's has no end
     long long per;          // of every block of the grid
+    int snap;               // a cut this near to a tile's edge moves there
 };
+
+// Range c of a line of `total` places cut for `grid` blocks, before its beginning has moved to a tile's edge.
+__host__ __device__ inline Range range_of(long long total, int c, int grid, const Cut &cut)
+{
+    Range r;
+    r.per = (total + grid - 1) / grid;
+    if (r.per < cut.least) r.per = cut.least;
+    r.snap = static_cast<int>(r.per / 8 < 1 << 20 ? r.per / 8 : 1 << 20);
+    if (r.snap < cut.lead) r.snap = cut.lead;   // no cut among the places in front of a tile's blocks
+    r.begin = r.per * c;
+    r.end = r.begin + r.per < total ? r.begin + r.per : total + r.snap + 1;
+    if (r.begin >= total) r.begin = r.end = total;
+    return r;
+}
+// The beginning moves to a near edge of the tile that holds it; false: nothing is left.
+__host__ __device__ inline bool settle(const Attention &a, const Cut &cut, Range &r, Place &p)
+{
+    const int rest = cut.lead + p.blocks.count - p.off;
+    if (p.off <= r.snap) {
+        r.begin -= p.off;
+        p.off = 0;
+    } else if (rest <= r.snap) {
+        r.begin += rest;
+        if (!next_tile(a, p, cut)) return false;
+    }
+    return true;
+}
+
+// Whether the tile at `at` is the range's: one that goes on from the range before, one that ends in it, or one whose cut is not so near to its beginning that it moves there.
+__host__ __device__ inline bool takes(const Range &r, const Place &p, long long at, const Cut &cut)
+{
+    return at < r.end && (p.off > 0 || r.end - at >= cut.lead + p.blocks.count || r.end - at > r.snap);
+}
+// On to the next tile of the range.
+__host__ __device__ inline bool advance(const Attention &a, const Range &r, Place &p, long long at, const Cut &cut) { return at < r.end && next_tile(a, p, cut) && takes(r, p, at, cut); }
 
 // What of the tile at `at` lies in a range: places of the line, and blocks of keys among them.
 struct Part {
     int places, from, blocks;
-    bool whole;             // all of the tile's blocks
-    long long first_block, last_block;   // of the tile, on the line
+    bool whole;     // all of the tile's blocks
+    bool tail;      // the tile begins in this range
+    int b0, b1;     // blocks of the grid that share the tile
 };
 __host__ __device__ inline Part part_of(const Place &p, const Range &r, long long at, const Cut &cut)
 {
     Part t;
-    const int rest = cut.lead + p.blocks.count - p.off;
-    t.places = r.end - at < rest ? static_cast<int>(r.end - at) : rest;
+    const int all = cut.lead + p.blocks.count, rest = all - p.off;
+    const long long first = at - p.off;
+    t.places = r.end - at >= rest - r.snap ? rest : static_cast<int>(r.end - at);
     t.from = larger(p.off - cut.lead, 0);
     t.blocks = larger(p.off + t.places - cut.lead - t.from, 0);
     t.whole = t.blocks == p.blocks.count;
-    t.first_block = at - p.off + cut.lead;
-    t.last_block = t.first_block + p.blocks.count - 1;
+    t.tail = p.off == 0;
+    t.b0 = t.whole ? 0 : static_cast<int>((first + r.snap) / r.per);              // before the first cut that stays inside the tile
+    t.b1 = t.whole ? 0 : static_cast<int>((first + all - r.snap - 1) / r.per);    // behind the last one
     return t;
 }
 
@@ -573,10 +613,7 @@ __device__ inline Range range_of_block(const Attention &a, const Cut &cut, Place
         if (w < warp) before += sums[w];
         total += sums[w];
     }
-    Range r;
-    r.per = max((total + gridDim.x - 1) / gridDim.x, static_cast<long long>(cut.least));
-    r.begin = min(r.per * blockIdx.x, total);
-    r.end = min(r.begin + r.per, total);
+    Range r = range_of(total, blockIdx.x, gridDim.x, cut);
     if (r.begin >= r.end) return r;
     if (before <= r.begin && r.begin < before + mine) {   // one warp of the block
         long long rest = r.begin - before;
@@ -620,6 +657,7 @@ __device__ inline Range range_of_block(const Attention &a, const Cut &cut, Place
     }
     __syncthreads();
     place = found;
+    if (!settle(a, cut, r, place) || !takes(r, place, r.begin, cut)) r.begin = r.end;
     return r;
 }
 

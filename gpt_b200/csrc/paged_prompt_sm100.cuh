@@ -453,9 +453,10 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             bounded_wait(drain, 0u, abort_flag, status, DEV_TIMEOUT_DRAIN);
         } else if (warp == 5) {
             int n = 0;
-            for (long long at = range.begin; at <= range.end;) {
+            bool go = range.begin < range.end;
+            for (long long at = range.begin, ended = 0; !ended;) {
                 Segment seg{};
-                if (at < range.end) {
+                if (go) {
                     const Part part = part_of(place, range, at, args.cut);
                     seg.blocks = part.blocks;
                     seg.s = place.s;
@@ -474,16 +475,13 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         seg.low[h] = a.window ? seg.first[h] - a.window + 1 : 0;
                     }
                     seg.whole = part.whole;
-                    seg.tail = part.first_block >= range.begin;
-                    if (!part.whole) {
-                        seg.b0 = static_cast<int>(part.first_block / range.per);
-                        seg.b1 = static_cast<int>(part.last_block / range.per);
-                    }
+                    seg.tail = part.tail;
+                    seg.b0 = part.b0;
+                    seg.b1 = part.b1;
                     at += part.places;
-                    if (at < range.end) next_tile(a, place, args.cut);
-                    if (seg.blocks == 0) continue;   // only the tile's own costs fell into this range
+                    go = advance(a, range, place, at, args.cut);
                 } else {
-                    ++at;   // behind the end: the last entry
+                    ended = 1;   // the last entry: no blocks
                 }
                 if (!__all_sync(0xffffffffu, bounded_wait(seg_empty(n), segment_phase(n) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER))) break;
                 if (lane == 0) {

@@ -17,15 +17,15 @@ constexpr int kRowsTile = 16, kRowsKeys = 32, kRowsPerSm = 3;
 constexpr float kFmaGrowth = 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled
 constexpr float kLog2E = 1.4426950408889634f;
 
-__host__ __device__ constexpr int few_blocks(int) { return kFewPerSm * 160; }
+constexpr int kFewBlocks = kFewPerSm * 160, kRowsBlocks = kRowsPerSm * 160;   // of a grid, at most: so many parts' sums have room in shared memory
 __host__ __device__ constexpr int few_smem(int rows)
 {
-    const int merge = kTokensWarps * rows * 132 * 4, sums = kFewPerSm * 160 * rows * 8;
+    const int merge = kTokensWarps * rows * 132 * 4, sums = kFewBlocks * rows * 8;
     return merge > sums ? merge : sums;
 }
 __host__ __device__ constexpr int rows_smem()
 {
-    const int work = (kRowsTile + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * 16, sums = kRowsPerSm * 160 * kRowsTile * 8;
+    const int work = (kRowsTile + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * 16, sums = kRowsBlocks * kRowsTile * 8;
     return work > sums ? work : sums;
 }
 
@@ -55,10 +55,6 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
     for (long long at = range.begin; at < range.end;) {
         const Part part = part_of(place, range, at, args.cut);
         at += part.places;
-        if (part.blocks == 0) {
-            if (at < range.end && !next_tile(a, place, args.cut)) break;
-            continue;
-        }
         const int packed0 = place.tile * NR, rows = min(NR, place.q.count * a.share - packed0);
         const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1), low = a.window ? p0 - a.window + 1 : 0;
         float q[NR][8] = {}, acc[NR][8] = {}, m[NR], l[NR];
@@ -170,8 +166,8 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
             if (half == 0) store8(rows_shared + (warp * NR + r) * 132 + piece * 8, acc[r]);
         }
         __syncthreads();
-        finish_tile<T, KIND, NR, kTokensWarps>(a, args.parts, place, part, range, rows, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
-        if (at < range.end && !next_tile(a, place, args.cut)) break;
+        finish_tile<T, KIND, NR, kTokensWarps>(a, args.parts, place, part, rows, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
+        if (!advance(a, range, place, at, args.cut)) break;
     }
 }
 
@@ -197,10 +193,6 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
     for (long long at = range.begin; at < range.end;) {
         const Part part = part_of(place, range, at, args.cut);
         at += part.places;
-        if (part.blocks == 0) {
-            if (at < range.end && !next_tile(a, place, args.cut)) break;
-            continue;
-        }
         const int packed0 = place.tile * kRowsTile, rows = min(kRowsTile, place.q.count * a.share - packed0);
         const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1), low = a.window ? p0 - a.window + 1 : 0;
         auto look_up = [&](int i) {   // by the first warp
@@ -306,8 +298,8 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
             if (4 * lane < dim) *reinterpret_cast<float4 *>(queries + (4 * warp + i) * kPitch + 4 * lane) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
         }
         __syncthreads();
-        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, range, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
-        if (at < range.end && !next_tile(a, place, args.cut)) break;
+        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
+        if (!advance(a, range, place, at, args.cut)) break;
     }
 }
 

@@ -161,7 +161,7 @@ struct TokensArgs {
 // total_ml [ROWS] = (maximum in base 2, sum).  A whole tile is stored; else the part goes to scratch, and the block that arrives last puts the parts together.
 // sums: room for (blocks of the grid) x ROWS pairs, which may be `merge` itself.  bad_rows is zero on entry.
 template <typename T, int KIND, int ROWS, int SUMS>
-__device__ __forceinline__ void finish_tile(const Attention &a, const Parts &parts, const Place &place, const Part &part, const Range &range, int rows, const float *merge, int pitch,
+__device__ __forceinline__ void finish_tile(const Attention &a, const Parts &parts, const Place &place, const Part &part, int rows, const float *merge, int pitch,
                                             float (*total_ml)[2], float2 *sums, int *bad_rows, int *arrived_last)
 {
     constexpr float kLn2 = 0.69314718055994531f;
@@ -180,7 +180,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
         store8(static_cast<T *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
         if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
     };
-    float *own = parts.base + (2LL * blockIdx.x + (part.first_block >= range.begin)) * parts.floats;
+    float *own = parts.base + (2LL * blockIdx.x + part.tail) * parts.floats;
     for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
         const int r = i / pieces, c = i % pieces;
         float v[8] = {};
@@ -199,7 +199,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
         }
     }
     if (!part.whole) {
-        const int b0 = static_cast<int>(part.first_block / range.per), b1 = static_cast<int>(part.last_block / range.per), count = b1 - b0 + 1;
+        const int b0 = part.b0, b1 = part.b1, count = b1 - b0 + 1;
         __threadfence();
         __syncthreads();
         if (threadIdx.x == 0) {
@@ -297,10 +297,6 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     for (long long at = range.begin; at < range.end;) {
         const Part part = part_of(place, range, at, args.cut);
         at += part.places;
-        if (part.blocks == 0) {
-            if (at < range.end && !next_tile(a, place, args.cut)) break;
-            continue;
-        }
         const int n_blocks = part.blocks;
         const int packed0 = place.tile * kRows, rows = min(kRows, place.q.count * a.share - packed0);
         const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1);
@@ -607,8 +603,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 }
             }
         __syncthreads();
-        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, range, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), &bad_rows, &arrived_last);
-        if (at < range.end && !next_tile(a, place, args.cut)) break;
+        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), &bad_rows, &arrived_last);
+        if (!advance(a, range, place, at, args.cut)) break;
     }
 }
 

@@ -294,8 +294,8 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *   kv_pages_read    the same rows' values out of the pages: k and v are written.  With row counts equal to the lengths, whole sequences.
  *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
  *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
- *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they may be the same
- *           tensor only with the same pitch.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.
+ *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they share no
+ *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.
  *   All addresses are 16-byte aligned, pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
  *   other. */
 typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;
@@ -315,6 +315,11 @@ int gptb200_kv_pages_read(gptb200_ctx *ctx, void *k, long long k_pitch, void *v,
                           const gptb200_kv_rows *rows);
 int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, float *lse, const void *q, long long q_pitch, int dtype, int heads,
                             const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks);
+/* The checks of a call of gptb200_attention_paged but those of q and out, and how it runs on a GPU with num_sms SMs (host logic only; no address is read).
+ * plan4 = {kernel (0 nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 few / sixteen rows on fp32 FMAs), query rows of a tile (rows of a group's heads
+ * and tokens side by side), blocks of the grid, scratch KiB}. */
+int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks,
+                                 int *plan4);
 /* Gradient scaling, norm clipping and AdamW over one packed buffer of `segments` tensors in two launches: what the reference
  * does with device_scale_and_clip_grad followed by one device_adamw_step per tensor (src/model/gpt.cpp:644-677,
  * cuda/kernels/gradient_clip.cu:35-59, adamw.cu:71-97).  Tensor t covers elements [segment_ends[t-1], segment_ends[t]);

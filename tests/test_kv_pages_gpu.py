@@ -179,3 +179,276 @@ def test_attention(backend, lengths, counts, kv_heads, share, dim, page, cap, wi
         out, sums = attend(backend, c, q, heads, dtype, scale, cap, window, sinks, extra=8, lse=False)
         backend.synchronize()
         check(c, q, out, sums, heads, dtype, scale, cap, window, sinks)
+
+
+BOTH = [("bf16", "bf16"), ("bf16", "e4m3"), ("f32", "f32")]
+
+
+@pytest.mark.parametrize("dtype,kind", BOTH + [("f32", "e4m3")])
+@pytest.mark.parametrize("lengths,counts,kv_heads,share,dim,window,sinks", [
+    ([9000, 3], [1, 1], 1, 8, 32, 0, 0),            # one tile shared by every block of the grid
+    ([9000], [1], 1, 1, 128, 0, 0),
+    ([7000, 20], [2, 1], 1, 16, 64, 0, 0),
+    ([6000], [300], 1, 1, 64, 0, 0),
+    ([50000], [1], 1, 16, 16, 0, 0),
+    ([20000], [3], 1, 8, 128, 12000, 100),
+])
+def test_long_sequences(backend, lengths, counts, kv_heads, share, dim, window, sinks, dtype, kind):
+    c = Cache(kind, lengths, counts, kv_heads, dim, 64, seed=11, poison=True).cuda()
+    heads, scale = kv_heads * share, dim ** -0.5
+    q, _ = rows_in(c.rows, heads * dim, dtype, 0, 6)
+    out, sums = attend(backend, c, q, heads, dtype, scale, 0.0, window, sinks)
+    again, sums_again = attend(backend, c, q, heads, dtype, scale, 0.0, window, sinks)
+    backend.synchronize()
+    check(c, q, out, sums, heads, dtype, scale, 0.0, window, sinks)
+    assert torch.equal(out, again) and torch.equal(sums, sums_again)      # the parts' order does not depend on who arrives last
+    backend.set_option("max_sms", 7)                                       # another grid, another cut of the line
+    try:
+        out, sums = attend(backend, c, q, heads, dtype, scale, 0.0, window, sinks)
+        backend.synchronize()
+        check(c, q, out, sums, heads, dtype, scale, 0.0, window, sinks)
+    finally:
+        backend.set_option("max_sms", 0)
+
+
+@pytest.mark.parametrize("dtype,kind", BOTH + [("f32", "e4m3"), ("bf16", "f32")])
+@pytest.mark.parametrize("count", [1, 3, 40])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_a_row_does_not_see_does_not_matter(backend, dtype, kind, count, bad):
+    """Not finite keys and values that only later rows of the same tile see, or that lie in front of the window: they make those rows, and only those, not finite."""
+    dim, heads, window, sinks = 64, 4, 90, 2
+    c = Cache(kind, [200, 130], [count, count], 2, dim, 16, seed=3)
+    for s, length in enumerate(c.lengths):
+        for position in ([length - 1, length - count // 2 - 1] if count > 1 else []) + [20]:
+            for which in (0, 1):
+                if which == 0 and position != 20:
+                    continue      # of keys only one that nobody sees: a not finite score is a not finite row
+                page, token = int(c.table_cpu[s, position // c.page]), position % c.page
+                data = c.data_cpu.float()
+                data[page, which, :, token, 5] = bad
+                c.data_cpu = data.to(c.TYPES[kind])
+                c.values[page, which, :, token, 5] = float("nan") if kind == "e4m3" else bad
+    c.cuda()
+    q, _ = rows_in(c.rows, heads * dim, dtype, 0, 8)
+    out, sums = attend(backend, c, q, heads, dtype, 0.125, 0.0, window, sinks)
+    backend.synchronize()
+    want, lse, spread, slack = c.attention(q, heads, 0.125, 0.0, window, sinks)
+    got = out.double().cpu()
+    fine = torch.isfinite(want)
+    assert fine.any() and torch.equal(torch.isfinite(got), fine)
+    bound = torch.nan_to_num(spread, nan=0.0, posinf=0.0) * (2.0 ** -8 + 2 * (dim + 8) * 2.0 ** -23 * torch.nan_to_num(slack, nan=0.0, posinf=0.0) + 2.0 ** -17) + want.abs() * HALF[dtype]
+    assert ((got - want).abs()[fine] <= bound[fine] + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype,kind,share,count", [("bf16", "bf16", 4, 1), ("bf16", "e4m3", 2, 40), ("f32", "f32", 1, 1), ("f32", "f32", 2, 20)])
+def test_numbers_that_do_not_fit_are_reported(backend, dtype, kind, share, count):
+    import gpt_b200
+    lengths, counts = [300, 200, 150], [count] * 3
+    c = Cache(kind, lengths, counts, 2, 64, 16, seed=4).cuda()
+    q, _ = rows_in(c.rows, 2 * share * 64, dtype, 0, 8)
+    k, _ = rows_in(c.rows, 128, dtype, 0, 9)
+    dt = {"bf16": 0, "f32": 1}[dtype]
+    whole, _ = attend(backend, c, q, 2 * share, dtype, 0.125)
+    backend.synchronize()
+    before = c.data.view(torch.uint8).clone()
+    for array, at, value in [("table", (1, 3), c.num_pages), ("table", (1, 0), -7), ("table", (1, 12), 2**31 - 1), ("len_dev", 1, 10**6), ("len_dev", 1, -5), ("starts", 3, c.rows + 1)]:
+        t = getattr(c, array)
+        kept = t[at].clone()
+        t[at] = value
+        out, _ = attend(backend, c, q, 2 * share, dtype, 0.125)
+        with pytest.raises(gpt_b200.GptB200Error) as e:
+            backend.synchronize()
+        assert e.value.status == 1
+        if array != "starts":      # the other sequences are served
+            for s in (0, 2):
+                r = slice(s * count, s * count + count)
+                assert torch.equal(out[r], whole[r])
+        ko, vo = torch.empty_like(k), torch.empty_like(k)
+        backend.kv_pages_read(ko, ko.stride(0), vo, vo.stride(0), dt, c.pages, c.batch)
+        if array != "table" or at[1] * 16 >= lengths[1] - count:
+            with pytest.raises(gpt_b200.GptB200Error):
+                backend.synchronize()
+        t[at] = kept
+    backend.synchronize()
+    assert torch.equal(c.data.view(torch.uint8), before)
+    out, _ = attend(backend, c, q, 2 * share, dtype, 0.125)
+    backend.synchronize()
+    assert torch.equal(out, whole)
+
+
+def test_refusals_of_the_calls(backend):
+    import gpt_b200
+    c = Cache("bf16", [20], [2], 2, 64, 16).cuda()
+    q = torch.zeros(3, 256, dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros_like(q)
+    kv = torch.zeros(3, 128, dtype=torch.bfloat16, device="cuda")
+
+    def refused(call):
+        n = backend.launch_count()
+        with pytest.raises(gpt_b200.GptB200Error) as e:
+            call()
+        assert e.value.status == 1 and backend.launch_count() == n
+
+    refused(lambda: backend.attention_paged(out, 255, None, q, 256, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(out, 260, None, q, 256, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(out, 256, None, q, 248, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(out.data_ptr() + 2, 256, None, q, 256, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(out, 256, None, None, 256, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(q, 256, None, q, 256, 0, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.attention_paged(out, 256, None, q, 256, 5, 4, c.pages, c.batch, 0.1))
+    refused(lambda: backend.kv_pages_write(c.pages, c.batch, kv, 120, kv, 128, 0))
+    refused(lambda: backend.kv_pages_write(c.pages, c.batch, kv, 128, kv.data_ptr() + 8, 128, 0))
+    refused(lambda: backend.kv_pages_read(kv, 128, None, 128, 0, c.pages, c.batch))
+    refused(lambda: backend.kv_pages_read(kv, 128, kv, 132, 1, c.pages, c.batch))
+    for sequences, rows in ((0, 3), (1, 0)):                       # nothing to do: nothing is launched
+        empty = gpt_b200.KvRows(c.starts, c.len_dev, c.table, sequences, c.pitch, rows, 1)
+        n = backend.launch_count()
+        backend.attention_paged(out, 256, None, q, 256, 0, 4, c.pages, empty, 0.1)
+        backend.kv_pages_write(c.pages, empty, kv, 128, kv, 128, 0)
+        assert backend.launch_count() == n
+
+
+@pytest.mark.parametrize("dtype,kind", BOTH)
+@pytest.mark.parametrize("counts", [[1, 1, 1], [2, 40, 1]])
+def test_captured_calls_follow_their_arrays(backend, dtype, kind, counts):
+    """A step (write, attend) captured twice, on tables and lengths that change between replays; both graphs share the context's scratch."""
+    import gpt_b200
+    lengths, heads, dim = [700, 300, 90], 8, 64
+    c = Cache(kind, lengths, counts, 2, dim, 16, seed=21, spare=40).cuda()
+    dt = {"bf16": 0, "f32": 1}[dtype]
+    q, _ = rows_in(c.rows, heads * dim, dtype, 0, 8)
+    k, k_cpu = rows_in(c.rows, 2 * dim, dtype, 0, 9)
+    v, v_cpu = rows_in(c.rows, 2 * dim, dtype, 0, 10)
+    side = torch.cuda.Stream()
+    be = gpt_b200.Backend(0, side.cuda_stream)
+    outs, graphs = [torch.empty_like(q) for _ in range(2)], []
+    torch.cuda.synchronize()
+    for out, cap in zip(outs, (0.0, 30.0)):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            be.kv_pages_write(c.pages, c.batch, k, k.stride(0), v, v.stride(0), dt)
+            be.attention_paged(out, out.stride(0), None, q, q.stride(0), dt, heads, c.pages, c.batch, 0.2, cap)
+        graphs.append(g)
+    free = [p for p in range(c.num_pages) if p not in c.used]
+    for turn in range(3):
+        if turn:   # every sequence one token longer, a page more where it needs one; the first one's pages change places
+            for s in range(3):
+                at = c.lengths[s] // 16
+                if c.lengths[s] % 16 == 0:
+                    c.table_cpu[s, at] = free.pop()
+                c.lengths[s] += 1
+            a, b = int(c.table_cpu[0, 1]), int(c.table_cpu[0, 2])
+            c.table_cpu[0, 1], c.table_cpu[0, 2] = b, a
+            torch.cuda.synchronize()
+            c.len_dev.copy_(torch.tensor(c.lengths, dtype=torch.int32))
+            c.table.copy_(c.table_cpu)
+        for g in graphs:
+            with torch.cuda.stream(side):
+                g.replay()
+        be.synchronize()
+        c.data_cpu = c.data.cpu()
+        c.values = c.data_cpu.double() if kind != "e4m3" else torch.ldexp(c.data_cpu.float().double(), c.scales.cpu()[..., None].int() - 127)
+        for s, page, token in [(r, p, t) for r, p, t in places(c)]:
+            x = k_cpu[s].double().reshape(2, dim)
+            want = x.to(c.TYPES[kind]).double() if kind != "e4m3" else torch.ldexp(codes_of(x)[0], codes_of(x)[1][:, None].int() - 127)
+            assert torch.equal(c.values[page, 0, :, token], want)
+        for out, cap in zip(outs, (0.0, 30.0)):
+            want, _, spread, slack = c.attention(q, heads, 0.2, cap)
+            bound = spread * ((2.0 ** -8 if dtype == "bf16" else 0.0) + 2 * (dim + 8) * 2.0 ** -23 * slack + 2.0 ** -17) + want.abs() * HALF[dtype]
+            assert ((out.double().cpu() - want).abs() <= bound + 1e-30).all()
+    del graphs
+    be.close()
+
+
+def test_pools_beyond_two_to_the_31_elements(backend):
+    """Pages at the far end of a pool of more than 2^32 bytes, in bf16 and e4m3, for single tokens and a prompt."""
+    for kind, dtype, pages in (("bf16", torch.bfloat16, 2100), ("e4m3", torch.float8_e4m3fn, 4200)):
+        for count in (1, 70):
+            small = Cache(kind, [500, 90], [count, count], 4, 128, 1024, seed=5)
+            data = torch.zeros(pages, 2, 4, 1024, 128, dtype=torch.uint8 if kind == "e4m3" else dtype, device="cuda")
+            assert data.numel() > 2 ** 31
+            n = small.num_pages
+            data[-n:] = (small.data_cpu.view(torch.uint8) if kind == "e4m3" else small.data_cpu).cuda()
+            scales = torch.zeros(pages, 2, 4, 1024, dtype=torch.uint8, device="cuda") if kind == "e4m3" else None
+            if scales is not None:
+                scales[-n:] = small.scales_cpu.cuda()
+            big = Cache(kind, [500, 90], [count, count], 4, 128, 1024, seed=5)
+            big.cuda()
+            import gpt_b200
+            big.data, big.scales = data.view(torch.float8_e4m3fn) if kind == "e4m3" else data, scales
+            big.table = (big.table_cpu + (big.table_cpu >= 0) * (pages - n)).int().cuda()
+            big.pages = gpt_b200.KvPages(big.data, scales, Cache.KINDS[kind], pages, 1024, 4, 128)
+            big.batch = gpt_b200.KvRows(big.starts, big.len_dev, big.table, 2, big.pitch, big.rows, count)
+            q, _ = rows_in(big.rows, 8 * 128, "bf16", 0, 5)
+            out, sums = attend(backend, big, q, 8, "bf16", 0.1)
+            backend.synchronize()
+            check(big, q, out, sums, 8, "bf16", 0.1)
+            del data, scales, big
+            torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype,kind,heads,dim,window,sinks", [("f32", "f32", 12, 64, 0, 0), ("bf16", "e4m3", 8, 128, 60, 4), ("bf16", "bf16", 4, 40, 0, 0)])
+def test_a_served_batch(backend, dtype, kind, heads, dim, window, sinks):
+    """Prompts in portions, then single tokens, sequences joining and leaving: every step writes its rows and attends over the pages; at the end the cache is read back."""
+    import gpt_b200
+    g = torch.Generator().manual_seed(13)
+    kv_heads, page, num = 4, 16, 60
+    dt = {"bf16": 0, "f32": 1}[dtype]
+    data = torch.zeros(num, 2, kv_heads, page, dim, dtype=Cache.TYPES[kind] if kind != "e4m3" else torch.uint8, device="cuda")
+    scales = torch.zeros(num, 2, kv_heads, page, dtype=torch.uint8, device="cuda") if kind == "e4m3" else None
+    pool = gpt_b200.KvPages(data, scales, Cache.KINDS[kind], num, page, kv_heads, dim)
+    free, tables, history = list(range(num)), {}, {}
+    plan = [{0: 50, 1: 7}, {0: 50, 1: 1}, {0: 1, 1: 1, 2: 33}, {1: 1, 2: 1}, {1: 40, 3: 5}, {1: 1, 3: 1, 2: 1}]
+    for turn, step in enumerate(plan):
+        if turn == 3:
+            free += tables.pop(0)
+            history.pop(0)
+        order = sorted(step)
+        for s in order:
+            tables.setdefault(s, [])
+            history.setdefault(s, [torch.empty(0, kv_heads, dim, dtype=torch.float64) for _ in (0, 1)])
+            while len(tables[s]) * page < history[s][0].shape[0] + step[s]:
+                tables[s].append(free.pop(0))
+        rows = sum(step.values())
+        x = [torch.randn(rows, n * dim, generator=g).to(TYPES[dtype]) for n in (kv_heads, kv_heads, heads)]
+        at = 0
+        for s in order:
+            for which in (0, 1):
+                new = x[which][at:at + step[s]].double().reshape(-1, kv_heads, dim)
+                if kind == "e4m3":
+                    codes, e = codes_of(new)
+                    new = torch.ldexp(codes, e[..., None].int() - 127)
+                history[s][which] = torch.cat([history[s][which], new])
+            at += step[s]
+        width = max(len(tables[s]) for s in order)
+        table = torch.tensor([tables[s] + [-1] * (width - len(tables[s])) for s in order], dtype=torch.int32).cuda()
+        lengths = torch.tensor([history[s][0].shape[0] for s in order], dtype=torch.int32).cuda()
+        starts = torch.tensor([0] + [step[s] for s in order]).cumsum(0).int().cuda()
+        batch = gpt_b200.KvRows(starts, lengths, table, len(order), width, rows, max(step.values()))
+        k, v, q = (t.cuda() for t in x)
+        out = torch.empty_like(q)
+        backend.kv_pages_write(pool, batch, k, k.stride(0), v, v.stride(0), dt)
+        backend.attention_paged(out, out.stride(0), None, q, q.stride(0), dt, heads, pool, batch, dim ** -0.5, 0.0, window, sinks)
+        backend.synchronize()
+        at = 0
+        for s in order:
+            dense = Cache.__new__(Cache)
+            n, length = step[s], history[s][0].shape[0]
+            dense.kv_heads, dense.dim, dense.page, dense.lengths, dense.counts = kv_heads, dim, length, [length], [n]
+            dense.starts_cpu, dense.table_cpu, dense.rows = torch.tensor([0, n]), torch.zeros(1, 1, dtype=torch.int32), n
+            dense.values = torch.stack([h.permute(1, 0, 2) for h in history[s]])[None]
+            want, _, spread, slack = dense.attention(x[2][at:at + n], heads, dim ** -0.5, 0.0, window, sinks)
+            bound = spread * ((2.0 ** -8 if dtype == "bf16" else 0.0) + 2 * (dim + 8) * 2.0 ** -23 * slack + 2.0 ** -17) + want.abs() * HALF[dtype]
+            assert ((out[at:at + n].double().cpu() - want).abs() <= bound + 1e-30).all()
+            at += n
+    order = sorted(history)
+    width = max(len(tables[s]) for s in order)
+    table = torch.tensor([tables[s] + [-1] * (width - len(tables[s])) for s in order], dtype=torch.int32).cuda()
+    counts = [history[s][0].shape[0] for s in order]
+    starts, lengths = torch.tensor([0] + counts).cumsum(0).int().cuda(), torch.tensor(counts, dtype=torch.int32).cuda()
+    batch = gpt_b200.KvRows(starts, lengths, table, len(order), width, sum(counts), max(counts))
+    k, v = (torch.empty(sum(counts), kv_heads * dim, device="cuda") for _ in (0, 1))
+    backend.kv_pages_read(k, k.stride(0), v, v.stride(0), 1, pool, batch)
+    backend.synchronize()
+    for which, got in ((0, k), (1, v)):
+        assert torch.equal(got.double().cpu(), torch.cat([history[s][which] for s in order]).reshape(sum(counts), -1).to(torch.float32).double())
