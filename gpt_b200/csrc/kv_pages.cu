@@ -198,11 +198,18 @@ int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, const PagedPlan &plan)
     return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
 }
 
-template <int NB, bool CODES>
+template <int NB, bool CODES, bool CAPPED>
 int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args)
 {
-    return run_line(ctx, args.a.cap > 0.0f ? kvp::paged_prompt_kernel<NB, CODES, true> : kvp::paged_prompt_kernel<NB, CODES, false>, args, kvp::kPromptThreads,
+    return run_line(ctx, args.a.lse ? kvp::paged_prompt_kernel<NB, CODES, CAPPED, true> : kvp::paged_prompt_kernel<NB, CODES, CAPPED, false>, args, kvp::kPromptThreads,
                     kvp::PromptShape<NB>::kSmem, 1, kPagedTickets / 2, kvp::kPromptPart);
+}
+
+template <int NB>
+int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args, bool codes)
+{
+    if (args.a.cap > 0.0f) return codes ? run_prompt<NB, true, true>(ctx, args) : run_prompt<NB, false, true>(ctx, args);
+    return codes ? run_prompt<NB, true, false>(ctx, args) : run_prompt<NB, false, false>(ctx, args);
 }
 
 int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
@@ -221,8 +228,7 @@ int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
         const int rc = bf16_operand_map(ctx, &args.map, a.pages.data, rows, a.pages.dim, a.pages.dim, args.box_rows);
         if (rc != GPTB200_OK) return rc;
     }
-    if (a.pages.dim <= 64) return codes ? run_prompt<1, true>(ctx, args) : run_prompt<1, false>(ctx, args);
-    return codes ? run_prompt<2, true>(ctx, args) : run_prompt<2, false>(ctx, args);
+    return a.pages.dim <= 64 ? run_prompt<1>(ctx, args, codes) : run_prompt<2>(ctx, args, codes);
 }
 
 }  // namespace

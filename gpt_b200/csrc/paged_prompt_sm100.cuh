@@ -2,8 +2,10 @@
 //
 // A tile is 256 packed query rows of one sequence and key / value head (kv_pages.cuh: the line of work), worked on as two halves of 128; per block of 128 keys
 //   S = Q K^T   tcgen05.mma from shared memory, S in TMEM
-//   softmax     a thread per row: the row's scores in registers, running reference and sum in fp32; weights go back to TMEM over S, rounded to bf16 (eight bits:
-//               the output has no more; the sum is that of the unrounded weights, as the logarithm of the sum needs it)
+//   softmax     a thread per row: the row's scores in registers, running reference and sum in fp32; weights go back to TMEM over S, rounded to bf16 (the output has
+//               no more bits) and divided at the end by the sum of the rounded ones: what rounding does to all of them alike cancels, and where a few weights
+//               make up a row so does the rest (error of such rows 1.65 -> 1.05 times that of rounding the output alone; two terms per weight, which would do
+//               the same for all rows, cost 25 %).  SUMS: the logarithm of the sum is asked for, which takes the unrounded sum besides
 //   O += P V    tcgen05.mma with P from TMEM and V from shared memory as stored (MN-major)
 // The halves take turns on the tensor pipe: while one is in softmax the other's products run.  O is scaled only when a row's maximum has grown by more than
 // 2^32 since the last time: weights of bf16 have fp32's exponents, so that neither they nor their sums leave the range before (with a limit of 2^8 a third of the blocks
@@ -25,7 +27,7 @@ namespace kvp {
 constexpr int kPromptThreads = 512, kPromptRows = 256, kPromptKeys = 128;
 constexpr int kPromptBlock = 128 * 128;   // bytes of [128 rows x 64 bf16]
 constexpr int kPromptMaxStages = 3;
-constexpr int kPromptPart = kPromptRows * 128 + 2 * kPromptRows;   // floats of a part in scratch
+constexpr int kPromptPart = kPromptRows * 128 + 4 * kPromptRows;   // floats of a part in scratch
 
 template <int NB>   // 64-column blocks of a head
 struct PromptShape {
@@ -150,7 +152,7 @@ struct Segment {
 constexpr float kPromptGrowth = 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled
 constexpr int kPromptSegments = 4, kPromptSegmentWarps = 13;   // ring; warps that read it
 
-template <int NB, bool CODES, bool CAPPED>
+template <int NB, bool CODES, bool CAPPED, bool SUMS>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 paged_prompt_kernel(const __grid_constant__ PromptArgs args)
 {
@@ -508,7 +510,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             const int packed = seg.packed0 + h * 128 + r;
             const bool there = h * 128 + r < seg.rows;
             const int token = a.shares.divide(packed), position = there ? seg.pos0 + token : -1;
-            float ref = -INFINITY, sum = 0.0f;   // what the weights stand against (base 2), their sum
+            float ref = -INFINITY, sum = 0.0f, sum_rounded = 0.0f;   // what the weights stand against (base 2), their sum, that of the rounded ones
             bool begun = false;
             const int blocks = seg.blocks, half_first = seg.first[h], half_last = seg.last[h], half_low = seg.low[h];
             const KeyBlocks keys = seg.keys;
@@ -580,6 +582,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     const float f = grow ? tok::exp2_fast(ref - top) : 1.0f;
                     if (grow) ref = top;
                     sum *= f;
+                    sum_rounded *= f;
 #pragma unroll 1
                     for (int c = 0; c < 16 * steps; c += 16) {
                         uint32_t o[16];
@@ -593,7 +596,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 begun = true;
                 const float use = ref == -INFINITY ? 0.0f : ref;   // nothing seen yet: every weight is 2^-inf = 0
                 const unsigned long long scale2 = ptx::both(args.scale_log2), minus_ref = ptx::both(-use);
-                unsigned long long sums[2] = {0, 0};
+                unsigned long long sums[2] = {0, 0}, rounded[2] = {0, 0};
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
                     uint32_t w[16];
@@ -604,8 +607,9 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         pro::unpair(CAPPED ? ptx::add2(v, minus_ref) : ptx::fma2(v, scale2, minus_ref), e0, e1);
                         e0 = tok::exp2_fast(e0);
                         e1 = tok::exp2_fast(e1);
-                        sums[i & 1] = ptx::add2(sums[i & 1], pro::pair(e0, e1));
+                        if (SUMS) sums[i & 1] = ptx::add2(sums[i & 1], pro::pair(e0, e1));
                         w[i] = ptx::pack_bf16x2(e0, e1);
+                        rounded[i & 1] = ptx::add2(rounded[i & 1], pro::pair(bf16_low(w[i]), bf16_high(w[i])));
                     }
                     pro::tmem_st_32x16(s_addr + 16 * c, w);
                     if (c == 1) {   // the first 64 keys' weights: their products may begin
@@ -614,11 +618,13 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         ptx::mbar_arrive(p_half(h));
                     }
                 }
-                {
-                    float e0, e1;
+                float e0, e1;
+                if (SUMS) {
                     pro::unpair(ptx::add2(sums[0], sums[1]), e0, e1);
                     sum += e0 + e1;
                 }
+                pro::unpair(ptx::add2(rounded[0], rounded[1]), e0, e1);
+                sum_rounded += e0 + e1;
                 pro::tmem_st_wait();
                 ptx::tc_fence_before();
                 ptx::mbar_arrive(p_full(h));
@@ -634,7 +640,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 const int rr = h * 128 + quarter * 32 + 8 * i + (lane >> 2), pr = seg.packed0 + rr, tk = a.shares.divide(pr);
                 to[i] = rr < seg.rows ? static_cast<__nv_bfloat16 *>(a.out) + (seg.row0 + tk) * a.out_pitch + (seg.g * a.share + pr - tk * a.share) * dim + 8 * piece : nullptr;
             }
-            const float by_whole = 1.0f / sum;
+            const float by_whole = 1.0f / sum_rounded;
             if (ok) ok = wait(o_full(h), tile & 1);
             ptx::tc_fence_after();
             if (!pro::all_of(4 + h, 128, ok)) break;
@@ -661,7 +667,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     __syncwarp();
                 };
                 auto store_sum = [&](float top, float total) {
-                    if (a.lse && there) a.lse[row * a.heads + head] = sees ? top * kLn2 + logf(total) : -INFINITY;
+                    if (SUMS && there) a.lse[row * a.heads + head] = sees ? top * kLn2 + logf(total) : -INFINITY;
                 };
                 bool done = seg.whole;
                 if (seg.whole) {
@@ -677,7 +683,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     store_sum(ref, sum);
                 } else {
                     // four columns of all rows side by side, so that the rows' threads write and read runs
-                    float *part = args.parts.base + (2LL * blockIdx.x + seg.tail) * args.parts.floats + h * (128 * 128 + 256);
+                    float *part = args.parts.base + (2LL * blockIdx.x + seg.tail) * args.parts.floats + h * (128 * 128 + 512);
                     for (int c = 0; c < 16 * steps; c += 32) {
                         uint32_t o[32];
                         ptx::tmem_ld_32x32(o_addr + c, o);
@@ -686,7 +692,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         for (int i = 0; i < 8; ++i)
                             *reinterpret_cast<uint4 *>(part + ((c / 4 + i) * 128 + r) * 4) = begun ? make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]) : make_uint4(0u, 0u, 0u, 0u);
                     }
-                    *reinterpret_cast<float2 *>(part + 128 * 128 + 2 * r) = make_float2(ref, sum);
+                    *reinterpret_cast<float4 *>(part + 128 * 128 + 4 * r) = make_float4(ref, sum, sum_rounded, 0.0f);
                     const int b0 = seg.b0, b1 = seg.b1;
                     __threadfence();
                     pro::all_of(4 + h, 128, true);
@@ -699,19 +705,21 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     pro::all_of(4 + h, 128, true);
                     done = arrived_last[h];
                     if (done) {
-                        auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats + h * (128 * 128 + 256); };
-                        float top = -INFINITY, total = 0.0f;
-                        for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(slot(b) + 128 * 128 + 2 * r));
+                        auto slot = [&](int b) { return args.parts.base + (2LL * b + (b == b0)) * args.parts.floats + h * (128 * 128 + 512); };
+                        float top = -INFINITY, total = 0.0f, total_rounded = 0.0f;
+                        for (int b = b0; b <= b1; ++b) top = fmaxf(top, __ldcg(slot(b) + 128 * 128 + 4 * r));
                         for (int b = b0; b <= b1; ++b) {
-                            const float2 ml = __ldcg(reinterpret_cast<const float2 *>(slot(b) + 128 * 128 + 2 * r));
-                            total = fmaf(ml.y, tok::share_of(ml.x, top), total);
+                            const float4 ml = __ldcg(reinterpret_cast<const float4 *>(slot(b) + 128 * 128 + 4 * r));
+                            const float f = tok::share_of(ml.x, top);
+                            total = fmaf(ml.y, f, total);
+                            total_rounded = fmaf(ml.z, f, total_rounded);
                         }
-                        const float by = 1.0f / total;
+                        const float by = 1.0f / total_rounded;
                         for (int c = 0; c < 16 * steps; c += 32) {
                             float v[32] = {};
                             for (int b = b0; b <= b1; ++b) {
                                 const float *from = slot(b);
-                                const float f = tok::share_of(__ldcg(from + 128 * 128 + 2 * r), top);
+                                const float f = tok::share_of(__ldcg(from + 128 * 128 + 4 * r), top);
 #pragma unroll
                                 for (int i = 0; i < 8; ++i) {
                                     const float4 u = __ldcg(reinterpret_cast<const float4 *>(from + ((c / 4 + i) * 128 + r) * 4));

@@ -520,7 +520,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     }
             }
             // weights: from rows of keys to the B operand's columns of rows of the tile by one transposition of 8 x 8 each
-            uint32_t weights[NT][2];
+            uint32_t weights[NT][2], weights_rest[NT][2];   // bf16: a second term each, so that the products carry sixteen bits of a weight
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float w[4];
@@ -533,7 +533,15 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     w[i] = CODES ? exp2_fast(x[n][i] + value_e[i >> 1] - (ref[n][e] == -INFINITY ? 0.0f : ref[n][e])) : p;
                 }
 #pragma unroll
-                for (int j = 0; j < 2; ++j) weights[n][j] = transposed(CODES ? pack_half2(w[2 * j], w[2 * j + 1]) : ptx::pack_bf16x2(w[2 * j], w[2 * j + 1]));
+                for (int j = 0; j < 2; ++j) {
+                    if constexpr (CODES) {
+                        weights[n][j] = transposed(pack_half2(w[2 * j], w[2 * j + 1]));
+                    } else {
+                        const uint32_t first = ptx::pack_bf16x2(w[2 * j], w[2 * j + 1]);
+                        weights[n][j] = transposed(first);
+                        weights_rest[n][j] = transposed(ptx::pack_bf16x2(w[2 * j] - bf16_low(first), w[2 * j + 1] - bf16_high(first)));
+                    }
+                }
             }
             if constexpr (CODES) {
                 // dimensions g8 * 2 D16 + ... of keys 2 t4, 2 t4 + 1, 2 t4 + 8, 2 t4 + 9: the product's rows g8 and g8 + 8 of step u are dimensions 2 u and 2 u + 1 among them
@@ -558,7 +566,10 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     uint32_t f[4];
                     ldsm4t(f, vt + ((lane & 7) + ((lane >> 4) << 3)) * S::kValuePitch + (16 * u + (((lane >> 3) & 1) << 3)) * 2);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma<false>(O[n][u], f, weights[n][0], weights[n][1]);
+                    for (int n = 0; n < NT; ++n) {
+                        mma<false>(O[n][u], f, weights[n][0], weights[n][1]);
+                        mma<false>(O[n][u], f, weights_rest[n][0], weights_rest[n][1]);
+                    }
                 }
             }
             __syncwarp();   // this stage may be filled again

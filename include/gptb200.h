@@ -295,7 +295,8 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
  *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
  *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they share no
- *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.
+ *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold;
+ *           the order of sums, and so the last bits of a row, depend on the lengths of all sequences of the call.
  *   All addresses are 16-byte aligned, pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
  *   other. */
 typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;

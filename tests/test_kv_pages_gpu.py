@@ -250,6 +250,8 @@ def test_numbers_that_do_not_fit_are_reported(backend, dtype, kind, share, count
     dt = {"bf16": 0, "f32": 1}[dtype]
     whole, _ = attend(backend, c, q, 2 * share, dtype, 0.125)
     backend.synchronize()
+    want, _, spread, slack = c.attention(q, 2 * share, 0.125)
+    bound = spread * ((2.0 ** -8 if dtype == "bf16" else 0.0) + 2 * (c.dim + 8) * 2.0 ** -23 * slack + 2.0 ** -17) + want.abs() * HALF[dtype]
     before = c.data.view(torch.uint8).clone()
     for array, at, value in [("table", (1, 3), c.num_pages), ("table", (1, 0), -7), ("table", (1, 12), 2**31 - 1), ("len_dev", 1, 10**6), ("len_dev", 1, -5), ("starts", 3, c.rows + 1)]:
         t = getattr(c, array)
@@ -259,10 +261,12 @@ def test_numbers_that_do_not_fit_are_reported(backend, dtype, kind, share, count
         with pytest.raises(gpt_b200.GptB200Error) as e:
             backend.synchronize()
         assert e.value.status == 1
-        if array != "starts":      # the other sequences are served
+        if array != "starts":      # the other sequences are served; with other lengths the line of work is cut elsewhere, so that sums are added in another order
+            got = out.double().cpu()
             for s in (0, 2):
                 r = slice(s * count, s * count + count)
-                assert torch.equal(out[r], whole[r])
+                assert ((got - want).abs() <= bound)[r].all()
+                assert array != "table" or torch.equal(out[r], whole[r])
         ko, vo = torch.empty_like(k), torch.empty_like(k)
         backend.kv_pages_read(ko, ko.stride(0), vo, vo.stride(0), dt, c.pages, c.batch)
         if array != "table" or at[1] * 16 >= lengths[1] - count:
@@ -299,7 +303,7 @@ def test_refusals_of_the_calls(backend):
     refused(lambda: backend.kv_pages_write(c.pages, c.batch, kv, 120, kv, 128, 0))
     refused(lambda: backend.kv_pages_write(c.pages, c.batch, kv, 128, kv.data_ptr() + 8, 128, 0))
     refused(lambda: backend.kv_pages_read(kv, 128, None, 128, 0, c.pages, c.batch))
-    refused(lambda: backend.kv_pages_read(kv, 128, kv, 132, 1, c.pages, c.batch))
+    refused(lambda: backend.kv_pages_read(kv, 128, kv, 130, 1, c.pages, c.batch))
     for sequences, rows in ((0, 3), (1, 0)):                       # nothing to do: nothing is launched
         empty = gpt_b200.KvRows(c.starts, c.len_dev, c.table, sequences, c.pitch, rows, 1)
         n = backend.launch_count()
