@@ -303,8 +303,42 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 release(tile++);
                 more = another();
             }
-            if (more) look_up();
+            if (!CODES && more) look_up();
             if constexpr (CODES) {
+                // its look-up in three steps between the conversions, so that nothing waits for the table or the powers of two
+                int table_entry[2] = {-1, -1};
+                long long next_row[2] = {-1, -1};
+                uint32_t stored[2] = {127, 127};
+                bool wanted[2] = {false, false};
+                if (more) {
+                    const Segment &seg = segment(tile);
+                    const int key0 = block_key(seg.keys, seg.from + b, kPromptKeys), low = a.window ? seg.first[0] - a.window + 1 : 0, p1 = max(seg.last[0], seg.last[1]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int key = key0 + t + 64 * i;
+                        wanted[i] = key <= p1 && (key >= low || key < a.sinks);
+                        next_row[i] = key & mask;
+                        if (wanted[i]) table_entry[i] = a.batch.table[static_cast<long long>(seg.s) * a.batch.table_pitch + (key >> a.pages.page_shift)];
+                    }
+                }
+                auto second_step = [&] {
+                    if (!more) return;
+                    const int g = segment(tile).g;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const bool there = wanted[i] && table_entry[i] >= 0 && table_entry[i] < a.pages.num_pages;
+                        if (wanted[i] && !there) report_bad(status);
+                        next_row[i] = there ? a.pages.place(table_entry[i], which, g, static_cast<int>(next_row[i])) : -1;
+                        if (there) stored[i] = a.pages.scales[next_row[i]];
+                    }
+                };
+                auto third_step = [&] {
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        row_at[which][n & 1][t + 64 * i] = next_row[i];
+                        row_e[which][n & 1][t + 64 * i] = static_cast<int>(stored[i]) - 127;
+                    }
+                };
                 // pieces of sixteen codes (two of eight where rows begin at odd multiples of eight); four are on their way while the four before become bf16
                 const uint8_t *data = static_cast<const uint8_t *>(a.pages.data);
                 constexpr int kPer = 4, kBatches = kPromptKeys * 4 * NB / 64 / kPer;
@@ -330,20 +364,32 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
 #pragma unroll
                 for (int batch = 0; batch < kBatches; ++batch) {
                     if (batch + 1 < kBatches) load(batch + 1, w[(batch + 1) & 1]);
+                    if (batch == 1) second_step();
+                    uint32_t rare = 0;   // a branch per batch, not per piece: four conversions run side by side
+                    auto put = [&](int r, const uint4 &x, const uint4 &y) {
+                        const uint32_t at = dst + (c >> 2) * kPromptBlock + r * 128;
+                        if (2 * c < 2 * steps) ptx::sts128(at + (((2 * c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+                        if (2 * c + 1 < 2 * steps) ptx::sts128(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), y.x, y.y, y.z, y.w);
+                    };
 #pragma unroll
                     for (int u = 0; u < kPer; ++u) {
                         const int r = r0 + (batch * kPer + u) * (16 / NB), e = row_e[which][turn][r];
                         const uint4 v = w[batch & 1][u];
-                        const uint32_t at = dst + (c >> 2) * kPromptBlock + r * 128, power = ((120 + min(e, 7) + 127) << 7) * 0x10001u;
-                        uint4 x = pro::codes8_to_bf16(make_uint2(v.x, v.y), power), y = pro::codes8_to_bf16(make_uint2(v.z, v.w), power);
-                        if (e > 7 || pro::nan_among(v)) {
-                            x = pro::codes8_to_bf16_any(make_uint2(v.x, v.y), scale_of(e + 127));
-                            y = pro::codes8_to_bf16_any(make_uint2(v.z, v.w), scale_of(e + 127));
+                        const uint32_t power = ((120 + min(e, 7) + 127) << 7) * 0x10001u;
+                        rare |= pro::nan_among(v) | static_cast<uint32_t>(e > 7);
+                        put(r, pro::codes8_to_bf16(make_uint2(v.x, v.y), power), pro::codes8_to_bf16(make_uint2(v.z, v.w), power));
+                    }
+                    if (rare) {
+#pragma unroll
+                        for (int u = 0; u < kPer; ++u) {
+                            const int r = r0 + (batch * kPer + u) * (16 / NB);
+                            const float scale = scale_of(row_e[which][turn][r] + 127);
+                            const uint4 v = w[batch & 1][u];
+                            put(r, pro::codes8_to_bf16_any(make_uint2(v.x, v.y), scale), pro::codes8_to_bf16_any(make_uint2(v.z, v.w), scale));
                         }
-                        if (2 * c < 2 * steps) ptx::sts128(at + (((2 * c & 7) ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
-                        if (2 * c + 1 < 2 * steps) ptx::sts128(at + ((((2 * c + 1) & 7) ^ (r & 7)) << 4), y.x, y.y, y.z, y.w);
                     }
                 }
+                if (more) third_step();
             }
             if (by_box) {
                 if (t == 0)
