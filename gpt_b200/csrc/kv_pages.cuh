@@ -84,20 +84,6 @@ __host__ __device__ inline int page_of(const Batch &b, const Pages &p, int s, in
     return -1;
 }
 
-// The sequence that a row belongs to, by a whole warp (32 starts compared at once), or -1: a row behind the last sequence.
-__device__ __forceinline__ int sequence_of_row(const Batch &b, int row, int lane)
-{
-    int low = 0, high = b.sequences;   // the last s in [low, high) with row_starts[s] <= row
-    while (high - low > 1) {
-        const int step = (high - low + 31) / 32, at = low + lane * step;
-        const unsigned mask = __ballot_sync(0xffffffffu, at < high && b.row_starts[at] <= row);
-        const int last = mask ? 31 - __clz(mask) : 0;
-        high = min(high, low + (last + 1) * step);
-        low += last * step;
-    }
-    return b.row_starts[low] <= row && row < b.row_starts[low + 1] ? low : -1;
-}
-
 // ---- eight elements of one row
 
 __device__ __forceinline__ void load8(float (&v)[8], const float *src)
