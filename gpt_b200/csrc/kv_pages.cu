@@ -112,12 +112,16 @@ PagedPlan plan_paged(int dtype, int kind, long long max_rows)
 {
     const bool codes = kind == GPTB200_KV_E4M3;
     if (dtype == GPTB200_DTYPE_F32 || kind == GPTB200_KV_F32) {
-        if (max_rows <= 1) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kTokensPart};
-        if (max_rows <= 4) return {PAGED_FEW, 4, kvp::kFewPerSm, kvp::kTokensPart};
+        // a row at a time: 4 sequences of 1024, 12 heads of 64, 2 / 4 / 8 rows a head: 21 / 21 / 28 us, 32 of 4096, 8 heads of 128, 4 / 8 / 16 rows: 396 / 373 / 671 us;
+        // sixteen at a time 26 / 27 / 30 us and 394 / 364 / 453 us
+        if (max_rows <= 8) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kTokensPart};
         return {PAGED_ROWS, kvp::kRowsTile, kvp::kRowsPerSm, kvp::kTokensPart};
     }
-    if (max_rows > 32) return {PAGED_PROMPT, kvp::kPromptRows, 1, kvp::kPromptPart};
-    return {PAGED_TOKENS, max_rows <= 8 ? 8 : 16, codes ? 3 : 2, kvp::kTokensPart};
+    // 16 sequences of 4096, 8 heads of 128, in us: bf16, 24 / 32 / 48 rows a head: streamed 54 / 67 / 83, prompt 68 / 67 / 63; e4m3, 64 / 96 rows: 111 / 145 against 150 / 148
+    // (with 2 sequences, 64 rows: 27 against 40 and 31 against 53)
+    if (max_rows > (codes ? 96 : 40)) return {PAGED_PROMPT, kvp::kPromptRows, 1, kvp::kPromptPart};
+    // tiles of eight or sixteen rows: bf16, 12 / 16 rows: 46 / 55 against 49 / 50; e4m3, 16 / 32 rows: 47 / 72 against 48 / 65
+    return {PAGED_TOKENS, max_rows <= (codes ? 16 : 12) ? 8 : 16, codes ? 3 : 2, kvp::kTokensPart};
 }
 
 int check_attention(gptb200_ctx *ctx, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks, kvp::Attention *a)
@@ -190,10 +194,7 @@ template <typename T, int KIND>
 int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, const PagedPlan &plan)
 {
     kvp::TokensArgs args{a, {}, {plan.tile_rows, kvp::kFewKeys, 1, 5}};
-    if (plan.kernel == PAGED_FEW) {
-        return plan.tile_rows == 1 ? run_line(ctx, kvp::paged_few_kernel<T, KIND, 1>, args, kvp::kTokensThreads, kvp::few_smem(1), plan.per_sm, kvp::kFewBlocks, plan.part_floats)
-                                   : run_line(ctx, kvp::paged_few_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::few_smem(4), plan.per_sm, kvp::kFewBlocks, plan.part_floats);
-    }
+    if (plan.kernel == PAGED_FEW) return run_line(ctx, kvp::paged_few_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::kFewSmem, plan.per_sm, kvp::kFewBlocks, plan.part_floats);
     args.cut.keys = kvp::kRowsKeys;
     return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
 }

@@ -1,8 +1,8 @@
 // Attention over a paged cache on fp32 FMAs: queries or cache in fp32 (GPT-2's own precision), any kind of pages.  Both forms share the line of work and the end of a tile
 // with the tensor-core form of few rows (kv_pages.cuh, paged_tokens.cuh).
 //
-//   paged_few_kernel    up to NR rows of one key / value head (single tokens): half a warp holds a row of 128 (eight dimensions a lane) and takes every second key straight
-//                       from the pages; eight keys per warp are under way at a time.  Bound by the cache's bytes.
+//   paged_few_kernel    a row at a time (single tokens): half a warp holds a row of 128 (eight dimensions a lane) and takes every second key straight from the pages; eight
+//                       keys per warp are under way at a time.  Bound by the cache's bytes, and by latency where they are few.
 //   paged_rows_kernel   sixteen packed rows against blocks of 32 keys in shared memory: a warp's four rows meet a key per lane, then four dimensions per lane.  Bound by
 //                       shared-memory loads: eight wavefronts for sixteen FMAs a lane in the scores, five in the weighted values.
 #pragma once
@@ -18,11 +18,8 @@ constexpr float kFmaGrowth = 32.0f;   // of a row's maximum, base 2, before what
 constexpr float kLog2E = 1.4426950408889634f;
 
 constexpr int kFewBlocks = kFewPerSm * 160, kRowsBlocks = kRowsPerSm * 160;   // of a grid, at most: so many parts' sums have room in shared memory
-__host__ __device__ constexpr int few_smem(int rows)
-{
-    const int merge = kTokensWarps * rows * 132 * 4, sums = kFewBlocks * rows * 8;
-    return merge > sums ? merge : sums;
-}
+constexpr int kFewSmem = kFewBlocks * 8;   // the warps' sums, 132 floats each, have room in it
+static_assert(kFewSmem >= kTokensWarps * 132 * 4);
 __host__ __device__ constexpr int rows_smem()
 {
     const int work = (kRowsTile + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * 16, sums = kRowsBlocks * kRowsTile * 8;
@@ -36,13 +33,13 @@ __device__ __forceinline__ float score2(const Attention &a, float dot)
     return (a.cap > 0.0f ? a.cap * tanhf(x / a.cap) : x) * kLog2E;
 }
 
-template <typename T, int KIND, int NR>
+template <typename T, int KIND>
 __global__ void __launch_bounds__(kTokensThreads, kFewPerSm)
 paged_few_kernel(const __grid_constant__ TokensArgs args)
 {
     using tok::exp2_fast;
     extern __shared__ __align__(16) float rows_shared[];
-    __shared__ float warp_ml[kTokensWarps][NR][2], total_ml[NR][2];
+    __shared__ float warp_ml[kTokensWarps][2], total_ml[1][2];
     __shared__ int bad_rows, arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
@@ -55,27 +52,18 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
     for (long long at = range.begin; at < range.end;) {
         const Part part = part_of(place, range, at, args.cut);
         at += part.places;
-        const int packed0 = place.tile * NR, rows = min(NR, place.q.count * a.share - packed0);
-        const int p0 = place.q.pos0 + a.shares.divide(packed0), p1 = place.q.pos0 + a.shares.divide(packed0 + rows - 1), low = a.window ? p0 - a.window + 1 : 0;
-        float q[NR][8] = {}, acc[NR][8] = {}, m[NR], l[NR];
-        int pos[NR];
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int packed = packed0 + r, token = a.shares.divide(packed);
-            pos[r] = r < rows ? place.q.pos0 + token : -1;
-            if (r < rows && active) load8(q[r], static_cast<const T *>(a.q) + (place.q.row0 + token) * a.q_pitch + (place.g * a.share + packed - token * a.share) * dim + piece * 8);
-            m[r] = -INFINITY;
-            l[r] = 0.0f;
-        }
+        const int packed = place.tile, token = a.shares.divide(packed), position = place.q.pos0 + token, low = a.window ? position - a.window + 1 : 0;
+        float q[8] = {}, acc[8] = {}, m = -INFINITY, l = 0.0f;
+        if (active) load8(q, static_cast<const T *>(a.q) + (place.q.row0 + token) * a.q_pitch + (place.g * a.share + packed - token * a.share) * dim + piece * 8);
         auto first_key = [&](int i) { return block_key(place.blocks, part.from + i, kFewKeys) + warp * 16; };
-        auto wanted = [&](int key) { return key <= p1 && (key >= low || key < a.sinks); };
+        auto wanted = [&](int key) { return key <= position && (key >= low || key < a.sinks); };
         // pages of the warp's two groups of eight keys, one block ahead
         int pages[2];
         auto look_up = [&](int i) {
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 const int key = i < part.blocks ? first_key(i) + 8 * g : 0;
-                pages[g] = i < part.blocks && key <= p1 && (key + 7 >= low || key < a.sinks) ? page_of(a.batch, a.pages, place.s, key) : -1;
+                pages[g] = i < part.blocks && key <= position && (key + 7 >= low || key < a.sinks) ? page_of(a.batch, a.pages, place.s, key) : -1;
             }
         };
         look_up(0);
@@ -95,78 +83,69 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
                         load8_held<KIND>(v[u], a.pages, page[g], 1, place.g, key & mask, piece);
                     }
                 }
+                float x[4], top = -INFINITY;
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    float x[4], top = -INFINITY;
+                for (int u = 0; u < 4; ++u) {
+                    x[u] = 0.0f;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        x[u] = 0.0f;
+                    for (int e = 0; e < 8; ++e) x[u] = fmaf(q[e], k[u][e], x[u]);
+                }
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[u] = fmaf(q[r][e], k[u][e], x[u]);
-                    }
+                for (int o = 8; o > 0; o >>= 1)
 #pragma unroll
-                    for (int o = 8; o > 0; o >>= 1)
+                    for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], o);
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) x[u] += __shfl_xor_sync(0xffffffffu, x[u], o);
+                for (int u = 0; u < 4; ++u) {
+                    x[u] = wanted(t + 8 * g + 2 * u + half) ? score2(a, x[u]) : -INFINITY;
+                    top = fmaxf(top, x[u]);
+                }
+                if (top > m + kFmaGrowth || (m == -INFINITY && top > -INFINITY)) {   // the same for the half warp
+                    const float f = exp2_fast(m - top);
+                    m = top;
+                    l *= f;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        x[u] = visible(a, t + 8 * g + 2 * u + half, pos[r]) ? score2(a, x[u]) : -INFINITY;
-                        top = fmaxf(top, x[u]);
-                    }
-                    if (top > m[r] + kFmaGrowth || (m[r] == -INFINITY && top > -INFINITY)) {   // the same for the half warp
-                        const float f = exp2_fast(m[r] - top);
-                        m[r] = top;
-                        l[r] *= f;
+                    for (int e = 0; e < 8; ++e) acc[e] *= f;
+                }
+                const float against = m == -INFINITY ? 0.0f : m;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[r][e] *= f;
-                    }
-                    const float against = m[r] == -INFINITY ? 0.0f : m[r];
+                for (int u = 0; u < 4; ++u) {
+                    const float p = exp2_fast(x[u] - against);
+                    l += p;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const float p = exp2_fast(x[u] - against);
-                        l[r] += p;
-#pragma unroll
-                        for (int e = 0; e < 8; ++e) acc[r][e] = fmaf(p, v[u][e], acc[r][e]);
-                    }
+                    for (int e = 0; e < 8; ++e) acc[e] = fmaf(p, v[u][e], acc[e]);
                 }
             }
         }
         // the halves, then the warps
+        const float both = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)), to_both = tok::share_of(m, both);
+        m = both;
+        l *= to_both;
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const float top = fmaxf(m[r], __shfl_xor_sync(0xffffffffu, m[r], 16)), f = tok::share_of(m[r], top);
-            m[r] = top;
-            l[r] *= f;
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 16);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                acc[r][e] *= f;
-                acc[r][e] += __shfl_xor_sync(0xffffffffu, acc[r][e], 16);
-            }
-            if (lane == 0) {
-                warp_ml[warp][r][0] = m[r];
-                warp_ml[warp][r][1] = l[r];
-            }
+        for (int e = 0; e < 8; ++e) {
+            acc[e] *= to_both;
+            acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
+        }
+        if (lane == 0) {
+            warp_ml[warp][0] = m;
+            warp_ml[warp][1] = l;
         }
         __syncthreads();
+        float top = warp_ml[0][0], sum = 0.0f;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            float top = warp_ml[0][r][0], sum = 0.0f;
+        for (int w = 1; w < kTokensWarps; ++w) top = fmaxf(top, warp_ml[w][0]);
 #pragma unroll
-            for (int w = 1; w < kTokensWarps; ++w) top = fmaxf(top, warp_ml[w][r][0]);
-#pragma unroll
-            for (int w = 0; w < kTokensWarps; ++w) sum += warp_ml[w][r][1] * tok::share_of(warp_ml[w][r][0], top);
-            if (threadIdx.x == 0) {
-                total_ml[r][0] = top;
-                total_ml[r][1] = sum;
-            }
-            const float f = tok::share_of(m[r], top);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[r][e] *= f;
-            if (half == 0) store8(rows_shared + (warp * NR + r) * 132 + piece * 8, acc[r]);
+        for (int w = 0; w < kTokensWarps; ++w) sum += warp_ml[w][1] * tok::share_of(warp_ml[w][0], top);
+        if (threadIdx.x == 0) {
+            total_ml[0][0] = top;
+            total_ml[0][1] = sum;
         }
+        const float to_top = tok::share_of(m, top);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= to_top;
+        if (half == 0) store8(rows_shared + warp * 132 + piece * 8, acc);
         __syncthreads();
-        finish_tile<T, KIND, NR, kTokensWarps>(a, args.parts, place, part, rows, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
+        finish_tile<T, KIND, 1, kTokensWarps>(a, args.parts, place, part, 1, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }

@@ -36,9 +36,10 @@ def plan(dtype=BF16, heads=4, p=None, r=None, scale=0.125, cap=0.0, window=0, si
 
 
 @pytest.mark.parametrize("dtype,kind,heads,max_new,want", [
-    (BF16, BF16, 2, 1, ("tokens", 8, 296)), (BF16, BF16, 8, 2, ("tokens", 8, 296)), (BF16, E4M3, 8, 3, ("tokens", 16, 444)), (BF16, E4M3, 16, 4, ("tokens", 16, 444)),
-    (BF16, BF16, 16, 5, ("prompt", 256, 148)), (BF16, E4M3, 2, 33, ("prompt", 256, 148)), (BF16, BF16, 2, 2**31 - 1, ("prompt", 256, 148)), (BF16, BF16, 2, 0, ("tokens", 8, 296)),
-    (F32, F32, 2, 1, ("few", 1, 444)), (F32, E4M3, 4, 2, ("few", 4, 444)), (F32, BF16, 6, 2, ("rows", 16, 444)), (BF16, F32, 2, 100, ("rows", 16, 444)),
+    (BF16, BF16, 2, 1, ("tokens", 8, 296)), (BF16, BF16, 8, 3, ("tokens", 8, 296)), (BF16, BF16, 8, 4, ("tokens", 16, 296)), (BF16, E4M3, 8, 4, ("tokens", 8, 444)),
+    (BF16, E4M3, 16, 4, ("tokens", 16, 444)), (BF16, BF16, 16, 5, ("tokens", 16, 296)), (BF16, BF16, 16, 6, ("prompt", 256, 148)), (BF16, E4M3, 2, 96, ("tokens", 16, 444)),
+    (BF16, E4M3, 2, 97, ("prompt", 256, 148)), (BF16, BF16, 2, 2**31 - 1, ("prompt", 256, 148)), (BF16, BF16, 2, 0, ("tokens", 8, 296)),
+    (F32, F32, 2, 1, ("few", 1, 444)), (F32, E4M3, 4, 2, ("few", 1, 444)), (F32, BF16, 6, 2, ("few", 1, 444)), (F32, F32, 6, 3, ("rows", 16, 444)), (BF16, F32, 2, 100, ("rows", 16, 444)),
 ])
 def test_choice_of_kernel(built_library, dtype, kind, heads, max_new, want):
     got = plan(dtype, heads, pages(kind=kind), rows(max_new=max_new))
