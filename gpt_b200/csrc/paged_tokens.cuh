@@ -116,12 +116,10 @@ __device__ __forceinline__ unsigned long long tanh_inner2(unsigned long long x)
     for (int i = 6; i >= 0; --i) p = ptx::fma2(p, u, ptx::both(c[i]));
     return ptx::mul2(p, x);
 }
-// two codes as two halves
-__device__ __forceinline__ uint32_t halves(uint32_t pair)
+// four codes as two pairs of halves
+__device__ __forceinline__ void halves(uint32_t four, uint32_t &first, uint32_t &second)
 {
-    uint32_t h;
-    asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(h) : "r"(pair));
-    return h;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(first), "=r"(second) : "r"(four));
 }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b)
 {
@@ -306,22 +304,23 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 
         // ---- the ring
         // lanes with an even number look up where the tile's first eight keys lie, the others the last eight: those of a page's head lie one behind the other
-        int next_page = -1;
-        const uint8_t *next_rows = nullptr;
-        auto look_up = [&](int i) {
-            next_page = -1;
-            if (i < n_blocks) {
-                const int key = tile_key(i) + 8 * (lane & 1);
-                if (key <= p1 && (key + 7 >= low || key < a.sinks)) next_page = page_of(a.batch, a.pages, place.s, key);
-                next_rows = data + max(next_page, 0) * page_bytes + place.g * head_bytes + (key & mask) * row_bytes;
-            }
+        int next_entry = -1;
+        bool next_wanted = false;
+        auto look_up = [&](int i) {   // the table's entry is not looked at before the tile is fetched, a turn later
+            const int key = tile_key(i) + 8 * (lane & 1);
+            next_wanted = i < n_blocks && key <= p1 && (key + 7 >= low || key < a.sinks);
+            if (next_wanted) next_entry = a.batch.table[static_cast<long long>(place.s) * a.batch.table_pitch + (key >> a.pages.page_shift)];
         };
         look_up(0);
         auto fetch = [&](int i) {
             const int stage = i % S::kStages;
             const uint32_t dst = ring + stage * S::kStage;
-            const int page[2] = {__shfl_sync(0xffffffffu, next_page, 0), __shfl_sync(0xffffffffu, next_page, 1)};
-            const uint8_t *rows8[2] = {shared_pointer(next_rows, 0), shared_pointer(next_rows, 1)};
+            const bool there = next_wanted && next_entry >= 0 && next_entry < a.pages.num_pages;
+            if (next_wanted && !there) report_bad(a.batch.status);
+            const int my_page = there ? next_entry : -1;
+            const uint8_t *my_rows = data + max(my_page, 0) * page_bytes + place.g * head_bytes + ((tile_key(i) + 8 * (lane & 1)) & mask) * row_bytes;
+            const int page[2] = {__shfl_sync(0xffffffffu, my_page, 0), __shfl_sync(0xffffffffu, my_page, 1)};
+            const uint8_t *rows8[2] = {shared_pointer(my_rows, 0), shared_pointer(my_rows, 1)};
             look_up(i + 1);
             if (i < n_blocks) {
                 const int t = tile_key(i);
@@ -425,7 +424,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             const int t = tile_key(it);
             const uint32_t kt = ring + it % S::kStages * S::kStage, vt = kt + 16 * S::kKeyPitch, et = vt + 16 * S::kValuePitch;
             // scores: rows of the product are keys g8 and g8 + 8, columns rows of the tile
-            float x[NT][4] = {};
+            float x[NT][4] = {}, x2[NT][4] = {};   // two sums: a product waits for the one before it in its sum
             float value_e[2] = {};   // exponents of the two keys' values
             if constexpr (CODES) {
                 constexpr int kWords = D16 % 4 == 0 ? 4 : 2;
@@ -436,9 +435,11 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     lds_words<kWords>(v, kt + (g8 + 8) * S::kKeyPitch + t4 * 4 * D16 + 4 * k);
 #pragma unroll
                     for (int i = 0; i < kWords; ++i) {
-                        const uint32_t f[4] = {halves(u[i]), halves(v[i]), halves(u[i] >> 16), halves(v[i] >> 16)};
+                        uint32_t f[4];
+                        halves(u[i], f[0], f[2]);
+                        halves(v[i], f[1], f[3]);
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma<true>(x[n], f, qf[n][k + i][0], qf[n][k + i][1]);
+                        for (int n = 0; n < NT; ++n) mma<true>(i & 1 ? x2[n] : x[n], f, qf[n][k + i][0], qf[n][k + i][1]);
                     }
                 }
                 uint32_t ke[2], ve[2];
@@ -449,8 +450,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     value_e[j] = static_cast<float>(static_cast<int>(ve[j]) - 127);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        x[n][2 * j] *= scale_of(ke[j]);
-                        x[n][2 * j + 1] *= scale_of(ke[j]);
+                        x[n][2 * j] = (x[n][2 * j] + x2[n][2 * j]) * scale_of(ke[j]);
+                        x[n][2 * j + 1] = (x[n][2 * j + 1] + x2[n][2 * j + 1]) * scale_of(ke[j]);
                     }
                 }
             } else {
@@ -459,14 +460,14 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     uint32_t f[4];
                     ldsm4(f, kt + (lane & 15) * S::kKeyPitch + (k * 16 + ((lane >> 4) << 3)) * 2);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) mma<false>(x[n], f, qf[n][k][0], qf[n][k][1]);
+                    for (int n = 0; n < NT; ++n) mma<false>(k & 1 ? x2[n] : x[n], f, qf[n][k][0], qf[n][k][1]);
                 }
             }
             const bool all_seen = t + 15 <= p0 && (a.window == 0 || t > p1 - a.window || t + 15 < a.sinks) && p0 >= 0;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] *= to_score[n][i & 1];
+                for (int i = 0; i < 4; ++i) x[n][i] = (CODES ? x[n][i] : x[n][i] + x2[n][i]) * to_score[n][i & 1];
                 if (a.cap > 0.0f) {   // a polynomial where all of the warp's scores lie within the cap
                     if (__all_sync(0xffffffffu, fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3]))) <= 1.0f)) {
                         unpair(tanh_inner2(pair(x[n][0], x[n][1])), x[n][0], x[n][1]);
@@ -551,9 +552,11 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 for (int r = 0; r < 4; ++r) lds_words<kWords>(c[r], vt + (2 * t4 + (r & 1) + 8 * (r >> 1)) * S::kValuePitch + g8 * 2 * D16);
 #pragma unroll
                 for (int i = 0; i < kWords; ++i) {
-                    const uint32_t lo0 = __byte_perm(c[0][i], c[1][i], 0x5140), lo1 = __byte_perm(c[0][i], c[1][i], 0x7362);
-                    const uint32_t hi0 = __byte_perm(c[2][i], c[3][i], 0x5140), hi1 = __byte_perm(c[2][i], c[3][i], 0x7362);
-                    const uint32_t f0[4] = {halves(lo0), halves(lo0 >> 16), halves(hi0), halves(hi0 >> 16)}, f1[4] = {halves(lo1), halves(lo1 >> 16), halves(hi1), halves(hi1 >> 16)};
+                    uint32_t f0[4], f1[4];
+                    halves(__byte_perm(c[0][i], c[1][i], 0x5140), f0[0], f0[1]);
+                    halves(__byte_perm(c[2][i], c[3][i], 0x5140), f0[2], f0[3]);
+                    halves(__byte_perm(c[0][i], c[1][i], 0x7362), f1[0], f1[1]);
+                    halves(__byte_perm(c[2][i], c[3][i], 0x7362), f1[2], f1[3]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma<true>(O[n][2 * i], f0, weights[n][0], weights[n][1]);
