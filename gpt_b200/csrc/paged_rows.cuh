@@ -168,6 +168,9 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
     Place place;
     const Range range = range_of_block<kTokensThreads>(a, args.cut, place);
     const int dim = a.pages.dim, pieces = dim / 8, mask = (1 << a.pages.page_shift) - 1;
+    // weighted values: four dimensions a lane; heads of up to 64 leave half of the lanes to every second key
+    const bool narrow = dim <= 64;
+    const int lane_d = 4 * (narrow ? lane & 15 : lane), lane_key = narrow ? lane >> 4 : 0, key_step = narrow ? 2 : 1;
     const long long values_at = static_cast<long long>(a.pages.kv_heads) << a.pages.page_shift;   // from a key's row to its value's
     for (long long at = range.begin; at < range.end;) {
         const Part part = part_of(place, range, at, args.cut);
@@ -248,10 +251,10 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
             float4 *mine = reinterpret_cast<float4 *>(weights) + warp * kRowsKeys;
             mine[lane] = w;
             __syncwarp();
-            if (4 * lane < dim) {
+            if (lane_d < dim) {
 #pragma unroll 8
-                for (int j = 0; j < kRowsKeys; ++j) {
-                    const float4 p = mine[j], v = *reinterpret_cast<const float4 *>(values + j * kPitch + 4 * lane);
+                for (int j = lane_key; j < kRowsKeys; j += key_step) {
+                    const float4 p = mine[j], v = *reinterpret_cast<const float4 *>(values + j * kPitch + lane_d);
                     const float *pp = &p.x;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
@@ -274,7 +277,11 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
                 total_ml[4 * warp + i][0] = m[i];
                 total_ml[4 * warp + i][1] = l[i];
             }
-            if (4 * lane < dim) *reinterpret_cast<float4 *>(queries + (4 * warp + i) * kPitch + 4 * lane) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
+            if (narrow) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) O[i][e] += __shfl_xor_sync(0xffffffffu, O[i][e], 16);
+            }
+            if (lane_d < dim && lane_key == 0) *reinterpret_cast<float4 *>(queries + (4 * warp + i) * kPitch + lane_d) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
         }
         __syncthreads();
         finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
