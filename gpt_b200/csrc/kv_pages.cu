@@ -103,21 +103,25 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
 
 // Which kernel attends, and how its grid is made; host logic.
 struct PagedPlan {
-    int kernel;       // 0: nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 few / sixteen rows on FMAs
+    int kernel;       // 0: nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 single / 16 or 32 rows on FMAs
     int tile_rows, per_sm, part_floats;
 };
 enum { PAGED_NONE = 0, PAGED_TOKENS = 1, PAGED_PROMPT = 2, PAGED_FEW = 3, PAGED_ROWS = 4 };
 
-PagedPlan plan_paged(int dtype, int kind, long long max_rows)
+// max_rows: of a head, for a sequence; all_rows: of all heads and sequences
+PagedPlan plan_paged(int dtype, int kind, long long max_rows, long long all_rows)
 {
     const bool codes = kind == GPTB200_KV_E4M3;
     if (dtype == GPTB200_DTYPE_F32 || kind == GPTB200_KV_F32) {
         // a row at a time: 4 sequences of 1024, 12 heads of 64, 2 / 4 / 8 rows a head: 21 / 21 / 28 us, 32 of 4096, 8 heads of 128, 4 / 8 / 16 rows: 396 / 373 / 671 us;
         // sixteen at a time 26 / 27 / 30 us and 394 / 364 / 453 us
         if (max_rows <= 8) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kTokensPart};
-        return {PAGED_ROWS, kvp::kRowsTile, kvp::kRowsPerSm, kvp::kTokensPart};
+        // four or eight rows a warp, in us, 16 sequences of 2048: 10 / 32 rows a head 36 / 48 against 46 / 54, 64 / 128 rows (3016 / 5488 in all) 99 / 169 against 89 / 142;
+        // 2000 rows 909 against 663; but with 2124 in all, 100 a head at most, 32 against 43: too few tiles
+        const int each = max_rows > 32 && all_rows >= 2560 ? 8 : 4;
+        return {PAGED_ROWS, kvp::rows_tile(each), kvp::kRowsPerSm, kvp::rows_part(each)};
     }
-    // 16 sequences of 4096, 8 heads of 128, in us: bf16, 24 / 32 / 48 rows a head: streamed 54 / 67 / 83, prompt 68 / 67 / 63; e4m3, 64 / 96 rows: 111 / 145 against 150 / 148
+    // 16 sequences of 4096, 8 heads of 128, in us: bf16, 32 / 40 / 48 rows a head: streamed 64 / 69 / 78, prompt 67 / 68 / 63; e4m3, 64 / 96 rows: 109 / 142 against 151 / 148
     // (with 2 sequences, 64 rows: 27 against 40 and 31 against 53)
     if (max_rows > (codes ? 96 : 40)) return {PAGED_PROMPT, kvp::kPromptRows, 1, kvp::kPromptPart};
     // tiles of eight or sixteen rows: bf16, 12 / 16 rows: 46 / 55 against 49 / 50; e4m3, 16 / 32 rows: 47 / 72 against 48 / 65
@@ -196,7 +200,8 @@ int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, const PagedPlan &plan)
     kvp::TokensArgs args{a, {}, {plan.tile_rows, kvp::kFewKeys, 1, 5}};
     if (plan.kernel == PAGED_FEW) return run_line(ctx, kvp::paged_few_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::kFewSmem, plan.per_sm, kvp::kFewBlocks, plan.part_floats);
     args.cut.keys = kvp::kRowsKeys;
-    return run_line(ctx, kvp::paged_rows_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::rows_smem(), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
+    return plan.tile_rows == kvp::rows_tile(4) ? run_line(ctx, kvp::paged_rows_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::rows_smem(4), plan.per_sm, kvp::kRowsBlocks, plan.part_floats)
+                                               : run_line(ctx, kvp::paged_rows_kernel<T, KIND, 8>, args, kvp::kTokensThreads, kvp::rows_smem(8), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
 }
 
 template <int NB, bool CODES, bool CAPPED>
@@ -260,7 +265,7 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     OnDevice device;
     CUDA_TRY(ctx, device.enter(ctx->device));
     a.q = q; a.out = out; a.lse = lse; a.q_pitch = q_pitch; a.out_pitch = out_pitch;
-    const PagedPlan plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share);
+    const PagedPlan plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share, 1LL * rows->rows * a.heads);
     if (plan.kernel == PAGED_PROMPT) return attention_prompt(ctx, a, pages->kind);
     if (plan.kernel == PAGED_TOKENS) return attention_tokens(ctx, a, pages->kind, plan.tile_rows == 8);
     if (dtype == GPTB200_DTYPE_BF16) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, a, plan);
@@ -275,7 +280,7 @@ int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb20
     const int rc = check_attention(nullptr, dtype, heads, pages, rows, scale, cap, window, sinks, &a);
     if (rc != GPTB200_OK) return rc;
     PagedPlan plan{};
-    if (rows->sequences > 0 && rows->rows > 0) plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share);
+    if (rows->sequences > 0 && rows->rows > 0) plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share, 1LL * rows->rows * a.heads);
     const int blocks = num_sms * plan.per_sm;
     const int out[4] = {plan.kernel, plan.tile_rows, blocks, static_cast<int>((2LL * blocks * plan.part_floats * sizeof(float)) >> 10)};
     for (int i = 0; i < 4; ++i) plan4[i] = out[i];

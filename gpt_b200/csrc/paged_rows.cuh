@@ -3,8 +3,8 @@
 //
 //   paged_few_kernel    a row at a time (single tokens): half a warp holds a row of 128 (eight dimensions a lane) and takes every second key straight from the pages; eight
 //                       keys per warp are under way at a time.  Bound by the cache's bytes, and by latency where they are few.
-//   paged_rows_kernel   sixteen packed rows against blocks of 32 keys in shared memory: a warp's four rows meet a key per lane, then four dimensions per lane.  Bound by
-//                       shared-memory loads: eight wavefronts for sixteen FMAs a lane in the scores, five in the weighted values.
+//   paged_rows_kernel   16 or 32 packed rows against blocks of 32 keys in shared memory: a warp's four or eight rows meet a key per lane, then four dimensions per lane.  Eight
+//                       (twelve) wavefronts of shared memory for 16 (32) FMAs a lane in the scores, five (six) in the weighted values.
 #pragma once
 
 #include "paged_tokens.cuh"
@@ -13,18 +13,17 @@ namespace gptb200 {
 namespace kvp {
 
 constexpr int kFewKeys = 64, kFewPerSm = 3;
-constexpr int kRowsTile = 16, kRowsKeys = 32, kRowsPerSm = 3;
+constexpr int kRowsKeys = 32, kRowsPerSm = 3;
+__host__ __device__ constexpr int rows_tile(int each) { return kTokensWarps * each; }                  // rows of a tile, `each` per warp
+__host__ __device__ constexpr int rows_part(int each) { return rows_tile(each) * 128 + 2 * rows_tile(each); }   // floats of a part in scratch
 constexpr float kFmaGrowth = 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled
 constexpr float kLog2E = 1.4426950408889634f;
 
 constexpr int kFewBlocks = kFewPerSm * 160, kRowsBlocks = kRowsPerSm * 160;   // of a grid, at most: so many parts' sums have room in shared memory
 constexpr int kFewSmem = kFewBlocks * 8;   // the warps' sums, 132 floats each, have room in it
 static_assert(kFewSmem >= kTokensWarps * 132 * 4);
-__host__ __device__ constexpr int rows_smem()
-{
-    const int work = (kRowsTile + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * 16, sums = kRowsBlocks * kRowsTile * 8;
-    return work > sums ? work : sums;
-}
+__host__ __device__ constexpr int rows_smem(int each) { return (rows_tile(each) + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * each * 4; }
+static_assert(rows_smem(4) / 8 >= kRowsBlocks);
 
 // A score in base 2.
 __device__ __forceinline__ float score2(const Attention &a, float dot)
@@ -40,7 +39,8 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
     using tok::exp2_fast;
     extern __shared__ __align__(16) float rows_shared[];
     __shared__ float warp_ml[kTokensWarps][2], total_ml[1][2];
-    __shared__ int bad_rows, arrived_last;
+    __shared__ unsigned int bad_rows;
+    __shared__ int arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
     grid_dependency_launch();
@@ -145,22 +145,25 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
         for (int e = 0; e < 8; ++e) acc[e] *= to_top;
         if (half == 0) store8(rows_shared + warp * 132 + piece * 8, acc);
         __syncthreads();
-        finish_tile<T, KIND, 1, kTokensWarps>(a, args.parts, place, part, 1, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
+        finish_tile<T, KIND, 1, kTokensWarps>(a, args.parts, place, part, 1, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), kFewBlocks, &bad_rows, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }
 
-template <typename T, int KIND>
+// kRowsEach: rows of a warp, 4 or 8
+template <typename T, int KIND, int kRowsEach>
 __global__ void __launch_bounds__(kTokensThreads, kRowsPerSm)
 paged_rows_kernel(const __grid_constant__ TokensArgs args)
 {
     using tok::exp2_fast;
+    constexpr int kRowsTile = rows_tile(kRowsEach);
     constexpr int kPitch = 132;   // floats: lanes that read a row each touch all banks
     extern __shared__ __align__(16) float rows_shared[];
     __shared__ float total_ml[kRowsTile][2];
     __shared__ long long key_row[2][kRowsKeys];   // in turn: a key's row among its page's, -1: zeros
-    __shared__ int bad_rows, arrived_last;
-    float *queries = rows_shared, *keys = queries + kRowsTile * kPitch, *values = keys + kRowsKeys * kPitch, *weights = values + kRowsKeys * kPitch;   // weights [warp][key][4 rows]
+    __shared__ unsigned int bad_rows;
+    __shared__ int arrived_last;
+    float *queries = rows_shared, *keys = queries + kRowsTile * kPitch, *values = keys + kRowsKeys * kPitch, *weights = values + kRowsKeys * kPitch;   // weights [warp][key][row of the warp]
     const Attention &a = args.a;
     grid_dependency_wait();
     grid_dependency_launch();
@@ -190,13 +193,13 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
         }
         if (warp == 0) look_up(0);
         if (threadIdx.x == 0) bad_rows = 0;
-        float m[4], l[4], O[4][4] = {};
-        int pos[4];
+        float m[kRowsEach], l[kRowsEach], O[kRowsEach][4] = {};
+        int pos[kRowsEach];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kRowsEach; ++i) {
             m[i] = -INFINITY;
             l[i] = 0.0f;
-            pos[i] = 4 * warp + i < rows ? place.q.pos0 + a.shares.divide(packed0 + 4 * warp + i) : -1;
+            pos[i] = kRowsEach * warp + i < rows ? place.q.pos0 + a.shares.divide(packed0 + kRowsEach * warp + i) : -1;
         }
         for (int it = 0; it < part.blocks; ++it) {
             __syncthreads();   // the block before has been read, this one's rows are known
@@ -217,22 +220,21 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
             }
             if (warp == 0 && it + 1 < part.blocks) look_up(it + 1);
             __syncthreads();
-            if (4 * warp >= rows) continue;
+            if (kRowsEach * warp >= rows) continue;
             const int key = block_key(place.blocks, part.from + it, kRowsKeys) + lane;
-            float x[4] = {};
+            float x[kRowsEach] = {};
 #pragma unroll 4
             for (int d = 0; d < dim; d += 4) {
                 const float4 kk = *reinterpret_cast<const float4 *>(keys + lane * kPitch + d);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float4 qq = *reinterpret_cast<const float4 *>(queries + (4 * warp + i) * kPitch + d);
+                for (int i = 0; i < kRowsEach; ++i) {
+                    const float4 qq = *reinterpret_cast<const float4 *>(queries + (kRowsEach * warp + i) * kPitch + d);
                     x[i] = fmaf(qq.x, kk.x, fmaf(qq.y, kk.y, fmaf(qq.z, kk.z, fmaf(qq.w, kk.w, x[i]))));
                 }
             }
-            float4 w;
-            float *wp = &w.x;
+            float w[kRowsEach];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kRowsEach; ++i) {
                 x[i] = visible(a, key, pos[i]) ? score2(a, x[i]) : -INFINITY;
                 if (__any_sync(0xffffffffu, x[i] > m[i] + kFmaGrowth || (m[i] == -INFINITY && x[i] > -INFINITY))) {
                     float top = x[i];
@@ -245,19 +247,25 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) O[i][e] *= f;
                 }
-                wp[i] = exp2_fast(x[i] - (m[i] == -INFINITY ? 0.0f : m[i]));
-                l[i] += wp[i];
+                w[i] = exp2_fast(x[i] - (m[i] == -INFINITY ? 0.0f : m[i]));
+                l[i] += w[i];
             }
-            float4 *mine = reinterpret_cast<float4 *>(weights) + warp * kRowsKeys;
-            mine[lane] = w;
+            float *mine = weights + warp * kRowsKeys * kRowsEach;
+#pragma unroll
+            for (int i = 0; i < kRowsEach; i += 4) *reinterpret_cast<float4 *>(mine + lane * kRowsEach + i) = make_float4(w[i], w[i + 1], w[i + 2], w[i + 3]);
             __syncwarp();
             if (lane_d < dim) {
 #pragma unroll 8
                 for (int j = lane_key; j < kRowsKeys; j += key_step) {
-                    const float4 p = mine[j], v = *reinterpret_cast<const float4 *>(values + j * kPitch + lane_d);
-                    const float *pp = &p.x;
+                    float pp[kRowsEach];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < kRowsEach; i += 4) {
+                        const float4 p = *reinterpret_cast<const float4 *>(mine + j * kRowsEach + i);
+                        pp[i] = p.x; pp[i + 1] = p.y; pp[i + 2] = p.z; pp[i + 3] = p.w;
+                    }
+                    const float4 v = *reinterpret_cast<const float4 *>(values + j * kPitch + lane_d);
+#pragma unroll
+                    for (int i = 0; i < kRowsEach; ++i) {
                         O[i][0] = fmaf(pp[i], v.x, O[i][0]);
                         O[i][1] = fmaf(pp[i], v.y, O[i][1]);
                         O[i][2] = fmaf(pp[i], v.z, O[i][2]);
@@ -270,21 +278,21 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
         __syncthreads();
         // the queries' place takes the sums
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < kRowsEach; ++i) {
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
             if (lane == 0) {
-                total_ml[4 * warp + i][0] = m[i];
-                total_ml[4 * warp + i][1] = l[i];
+                total_ml[kRowsEach * warp + i][0] = m[i];
+                total_ml[kRowsEach * warp + i][1] = l[i];
             }
             if (narrow) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) O[i][e] += __shfl_xor_sync(0xffffffffu, O[i][e], 16);
             }
-            if (lane_d < dim && lane_key == 0) *reinterpret_cast<float4 *>(queries + (4 * warp + i) * kPitch + lane_d) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
+            if (lane_d < dim && lane_key == 0) *reinterpret_cast<float4 *>(queries + (kRowsEach * warp + i) * kPitch + lane_d) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
         }
         __syncthreads();
-        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), &bad_rows, &arrived_last);
+        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), rows_smem(kRowsEach) / 8, &bad_rows, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }

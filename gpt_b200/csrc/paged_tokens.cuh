@@ -44,9 +44,8 @@ struct TokensShape {
     static constexpr int kRing = kTokensWarps * kStages * kStage;
     static constexpr int kMergePitch = kDim + 4;
     static constexpr int kMerge = kTokensWarps * kRows * kMergePitch * 4;
-    static constexpr int kMaxBlocks = kPerSm * 160;                  // of the grid: a tile may be shared by all of them ...
-    static constexpr int kPartSums = kMaxBlocks * kRows * 8;         // ... whose maxima and sums then lie in shared memory
-    static constexpr int kLarger = kRing > kMerge ? kRing : kMerge, kSmem = kRows * kQPitch + (kLarger > kPartSums ? kLarger : kPartSums);
+    static constexpr int kSmem = kRows * kQPitch + (kRing > kMerge ? kRing : kMerge), kMaxBlocks = kPerSm * 160;
+    static_assert((kSmem - kRows * kQPitch) / 8 >= kMaxBlocks);   // of the grid: a tile's parts, at most
 };
 
 namespace tok {
@@ -157,11 +156,12 @@ struct TokensArgs {
 
 // The end of a tile, for a block of kTokensThreads threads that holds its rows' sums in shared memory: merge [SUMS][ROWS][pitch] weighted values (added up here) against
 // total_ml [ROWS] = (maximum in base 2, sum).  A whole tile is stored; else the part goes to scratch, and the block that arrives last puts the parts together.
-// sums: room for (blocks of the grid) x ROWS pairs, which may be `merge` itself.  bad_rows is zero on entry.
+// sums: room for as many pairs, one per block of the grid at least; it may be `merge` itself.  bad_rows is zero on entry.
 template <typename T, int KIND, int ROWS, int SUMS>
 __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &parts, const Place &place, const Part &part, int rows, const float *merge, int pitch,
-                                            float (*total_ml)[2], float2 *sums, int *bad_rows, int *arrived_last)
+                                            float (*total_ml)[2], float2 *sums, int room, unsigned int *bad_rows, int *arrived_last)
 {
+    constexpr int kSlot = (ROWS > kTokensMaxRows ? ROWS : kTokensMaxRows) * 128;   // a part in scratch: values, then maxima and sums
     constexpr float kLn2 = 0.69314718055994531f;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.pages.dim, pieces = dim / 8, packed0 = place.tile * ROWS;
     auto finish = [&](int r, int c, float (&v)[8], float top, float sum) {   // piece c of row r
@@ -174,7 +174,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
             v[e] *= inv;
             fine = fine && fabsf(v[e]) <= FLT_MAX;
         }
-        if (!fine) atomicOr(bad_rows, 1 << r);
+        if (!fine) atomicOr(bad_rows, 1u << r);
         store8(static_cast<T *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
         if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
     };
@@ -193,7 +193,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
             finish(r, c, v, total_ml[r][0], total_ml[r][1]);
         } else {
             store8(own + r * dim + c * 8, v);
-            if (c == 0) *reinterpret_cast<float2 *>(own + kTokensMaxRows * 128 + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
+            if (c == 0) *reinterpret_cast<float2 *>(own + kSlot + 2 * r) = make_float2(total_ml[r][0], total_ml[r][1]);
         }
     }
     if (!part.whole) {
@@ -210,45 +210,51 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
         if (*arrived_last) {
             // the parts' maxima and sums first, all of them under way at once; a part's factor takes the place of its maximum
             auto slot = [&](int b) { return parts.base + (2LL * b + (b == b0)) * parts.floats; };
-            for (int i = threadIdx.x; i < count * rows; i += kTokensThreads) sums[i] = __ldcg(reinterpret_cast<const float2 *>(slot(b0 + i / rows) + kTokensMaxRows * 128 + 2 * (i % rows)));
-            __syncthreads();
-            for (int r = warp; r < rows; r += kTokensWarps) {
-                float top = -INFINITY, sum = 0.0f;
-                for (int i = lane; i < count; i += 32) top = fmaxf(top, sums[i * rows + r].x);
+            const int most = min(rows, room / count);   // rows at a time
+            for (int r0 = 0; r0 < rows; r0 += most) {
+                const int n_rows = min(most, rows - r0);
+                __syncthreads();
+                for (int i = threadIdx.x; i < count * n_rows; i += kTokensThreads) sums[i] = __ldcg(reinterpret_cast<const float2 *>(slot(b0 + i / n_rows) + kSlot + 2 * (r0 + i % n_rows)));
+                __syncthreads();
+                for (int r = warp; r < n_rows; r += kTokensWarps) {
+                    float top = -INFINITY, sum = 0.0f;
+                    for (int i = lane; i < count; i += 32) top = fmaxf(top, sums[i * n_rows + r].x);
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                for (int i = lane; i < count; i += 32) {
-                    float2 &v = sums[i * rows + r];
-                    v.x = tok::share_of(v.x, top);
-                    sum = fmaf(v.y, v.x, sum);
-                }
+                    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                    for (int i = lane; i < count; i += 32) {
+                        float2 &v = sums[i * n_rows + r];
+                        v.x = tok::share_of(v.x, top);
+                        sum = fmaf(v.y, v.x, sum);
+                    }
 #pragma unroll
-                for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) {
-                    total_ml[r][0] = top;
-                    total_ml[r][1] = sum;
+                    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                    if (lane == 0) {
+                        total_ml[r0 + r][0] = top;
+                        total_ml[r0 + r][1] = sum;
+                    }
                 }
-            }
-            __syncthreads();
-            for (int i = threadIdx.x; i < rows * pieces; i += kTokensThreads) {
-                const int r = i / pieces, c = i % pieces;
-                float v[8] = {};
+                __syncthreads();
+                for (int i = threadIdx.x; i < n_rows * pieces; i += kTokensThreads) {
+                    const int r = i / pieces, c = i % pieces;
+                    float v[8] = {};
 #pragma unroll 8
-                for (int n = 0; n < count; ++n) {
-                    const float *from = slot(b0 + n) + r * dim + c * 8;
-                    const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + 4));
-                    const float f = sums[n * rows + r].x;
-                    v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
-                    v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
+                    for (int n = 0; n < count; ++n) {
+                        const float *from = slot(b0 + n) + (r0 + r) * dim + c * 8;
+                        const float4 u0 = __ldcg(reinterpret_cast<const float4 *>(from)), u1 = __ldcg(reinterpret_cast<const float4 *>(from + 4));
+                        const float f = sums[n * n_rows + r].x;
+                        v[0] = fmaf(u0.x, f, v[0]); v[1] = fmaf(u0.y, f, v[1]); v[2] = fmaf(u0.z, f, v[2]); v[3] = fmaf(u0.w, f, v[3]);
+                        v[4] = fmaf(u1.x, f, v[4]); v[5] = fmaf(u1.y, f, v[5]); v[6] = fmaf(u1.z, f, v[6]); v[7] = fmaf(u1.w, f, v[7]);
+                    }
+                    finish(r0 + r, c, v, total_ml[r0 + r][0], total_ml[r0 + r][1]);
                 }
-                finish(r, c, v, total_ml[r][0], total_ml[r][1]);
             }
         }
     }
     __syncthreads();
     // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is formed once more
     // from its own keys alone.
-    for (int rest = *bad_rows, n = 0; rest; rest &= rest - 1, ++n) {
+    int n = 0;
+    for (unsigned int rest = *bad_rows; rest; rest &= rest - 1, ++n) {
         if (n % kTokensWarps != warp) continue;
         const int packed = packed0 + __ffs(rest) - 1, token = a.shares.divide(packed);
         attention_row<T, KIND>(a, place.s, place.q.pos0 + token, place.q.row0 + token, place.g * a.share + packed - token * a.share, lane);
@@ -268,7 +274,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     constexpr float kLog2e = 1.4426950408889634f;
     extern __shared__ __align__(16) uint8_t tokens_smem[];
     __shared__ float merge_ml[kTokensWarps][kRows][2], total_ml[kRows][2], row_power[kRows];
-    __shared__ int bad_rows, arrived_last;
+    __shared__ unsigned int bad_rows;
+    __shared__ int arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
     grid_dependency_launch();
@@ -617,7 +624,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 }
             }
         __syncthreads();
-        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), &bad_rows, &arrived_last);
+        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), (S::kSmem - kRows * S::kQPitch) / 8, &bad_rows, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }

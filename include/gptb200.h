@@ -317,7 +317,7 @@ int gptb200_kv_pages_read(gptb200_ctx *ctx, void *k, long long k_pitch, void *v,
 int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, float *lse, const void *q, long long q_pitch, int dtype, int heads,
                             const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks);
 /* The checks of a call of gptb200_attention_paged but those of q and out, and how it runs on a GPU with num_sms SMs (host logic only; no address is read).
- * plan4 = {kernel (0 nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 few / sixteen rows on fp32 FMAs), query rows of a tile (rows of a group's heads
+ * plan4 = {kernel (0 nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 single / 16 or 32 rows on fp32 FMAs), query rows of a tile (rows of a group's heads
  * and tokens side by side), blocks of the grid, scratch KiB}. */
 int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks,
                                  int *plan4);

@@ -87,3 +87,9 @@ def test_null_arguments(built_library):
     assert lib.gptb200_plan_attention_paged(0, 0, 4, p, r, 1.0, 0.0, 0, 0, out) == 1
     assert lib.gptb200_attention_paged(None, 0x1000, 256, None, 0x2000, 256, 0, 4, p, r, 1.0, 0.0, 0, 0) == 1
     assert lib.gptb200_kv_pages_write(None, p, r, 0x1000, 128, 0x2000, 128, 0) == 1 and lib.gptb200_kv_pages_read(None, 0x1000, 128, 0x2000, 128, 0, p, r) == 1
+
+
+@pytest.mark.parametrize("heads,max_new,count,want", [(32, 2, 4096, 16), (32, 3, 79, 16), (32, 3, 80, 32), (8, 40, 319, 16), (8, 40, 320, 32)])
+def test_rows_of_a_tile_on_fmas(built_library, heads, max_new, count, want):
+    got = plan(F32, heads, pages(kind=F32), rows(max_new=max_new, count=count))
+    assert (got["kernel"], got["tile_rows"]) == ("rows", want)

@@ -456,3 +456,34 @@ def test_a_served_batch(backend, dtype, kind, heads, dim, window, sinks):
     backend.synchronize()
     for which, got in ((0, k), (1, v)):
         assert torch.equal(got.double().cpu(), torch.cat([history[s][which] for s in order]).reshape(sum(counts), -1).to(torch.float32).double())
+
+
+@pytest.mark.parametrize("dtype,kind", [("f32", "f32"), ("f32", "e4m3"), ("bf16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("lengths,counts,kv_heads,share,dim,page,cap,window,sinks", [
+    ([700, 90, 3], [333, 90, 1], 2, 4, 128, 16, 0.0, 50, 5),
+    ([513, 60], [513, 1], 1, 8, 80, 64, 40.0, 0, 0),
+    ([6000], [20], 1, 8, 64, 32, 0.0, 0, 0),           # a tile's parts lie all over the grid
+    ([40, 41, 31], [33, 9, 31], 1, 8, 8, 8, 0.0, 0, 0),
+])
+def test_wide_tiles_on_fmas(backend, lengths, counts, kv_heads, share, dim, page, cap, window, sinks, dtype, kind):
+    """Calls of many rows of all heads, though most of them may lie behind the last sequence."""
+    import gpt_b200
+    c = Cache(kind, lengths, counts, kv_heads, dim, page, seed=dim, extra_rows=520, poison=True)
+    c.cuda(max_new=max(counts))
+    heads, scale = kv_heads * share, dim ** -0.5
+    assert gpt_b200.plan_attention_paged(148, {"bf16": 0, "f32": 1}[dtype], heads, c.pages, c.batch, scale, cap, window, sinks)["tile_rows"] == 32
+    q, _ = rows_in(c.rows, heads * dim, dtype, 8, 5, scale=2.0)
+    out, sums = attend(backend, c, q, heads, dtype, scale, cap, window, sinks, extra=8)
+    backend.synchronize()
+    check(c, q, out, sums, heads, dtype, scale, cap, window, sinks)
+    # a value that is not finite, seen by the last row of a sequence alone
+    last, c.values = int(c.table_cpu[0, (lengths[0] - 1) // page]), c.values.clone()
+    data = c.data.float()
+    data[last, 1, :, (lengths[0] - 1) % page, 5] = float("nan")
+    c.data.copy_(data.to(c.data.dtype))
+    c.values[last, 1, :, (lengths[0] - 1) % page, 5] = float("nan")
+    out, sums = attend(backend, c, q, heads, dtype, scale, cap, window, sinks, extra=8)
+    backend.synchronize()
+    want, got = c.attention(q, heads, scale, cap, window, sinks)[0], out.double().cpu()
+    end = sum(counts)
+    assert torch.equal(torch.isnan(got[:end]), torch.isnan(want[:end])) and torch.isnan(want[counts[0] - 1]).any() and not torch.isnan(want[:counts[0] - 1]).any()
