@@ -9,9 +9,12 @@
 // instructions do here; what counts is bytes in flight and instructions per byte, hence the rings (40 to 100 KB per block) and no barrier inside the loop.
 //
 // Codes (e4m3) go through registers once, to fp16, which holds every code exactly; their powers of two never touch the products:
-//   scores   q of a row is divided by a power of two (its largest value's), so that fp16 holds it as bf16 did; the row's and the key's powers multiply the score
-//   values   weight j enters the second product as 2^(x_j + e_j - R), x_j the score in base 2, e_j the value's exponent, R their running maximum: at most 1, rounded
-//            to eleven bits where bf16 weights have eight.  The sum of weights runs against the scores' own maximum, in fp32.
+//   scores   q of a row is brought to [2^15, 2^16) at its largest by a power of two, so that fp16 holds all eight bits of a bf16 element down to 2^-32 of the largest
+//            (and part of them down to 2^-40); the row's and the key's powers multiply the score
+//   values   weight j enters the second product as 2^(x_j + e_j - R + 11), x_j the score in base 2, e_j the value's exponent, R their running maximum within 2^4: at most
+//            2^15.  The sum of weights runs against the scores' own maximum, in fp32.
+// Weights enter the products in two terms, so that their rounding stays below that of an fp32 sum's order: sixteen bits of bf16, which has fp32's exponents, or
+// twenty-two of fp16, whose second term ends at 2^-35 of the row's largest: what a key adds is off by 2^-22 of itself and 2^-36 of the largest weight times power.
 // The products' inner dimension may be permuted on both sides, and so may the output's columns: a lane takes neighbouring codes with one load, pairs two keys'
 // codes with a byte permutation, and no transposition is needed.
 #pragma once
@@ -126,6 +129,7 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b)
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(h) : "f"(b), "f"(a));
     return h;
 }
+__device__ __forceinline__ float2 unpack_half2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2 *>(&v)); }
 // an 8 x 8 matrix of sixteen-bit values, a row per four lanes, transposed
 __device__ __forceinline__ uint32_t transposed(uint32_t v)
 {
@@ -269,7 +273,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     using namespace tok;
     using S = TokensShape<D16, CODES, NT>;
     constexpr int kRows = S::kRows;
-    constexpr float kGrowth = CODES ? 8.0f : 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled: fp16 weights end at 2^16
+    constexpr float kGrowth = CODES ? 4.0f : 32.0f;   // of a row's maximum, base 2, before what has been added up is scaled
+    constexpr float kLift = CODES ? 11.0f : 0.0f;     // fp16 weights end at 2^16: the largest is 2^(kLift + kGrowth)
     constexpr int kind = CODES ? KIND_E4M3 : KIND_BF16;
     constexpr float kLog2e = 1.4426950408889634f;
     extern __shared__ __align__(16) uint8_t tokens_smem[];
@@ -384,7 +389,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-                const int e2 = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -100), 100);
+                const int e2 = max(static_cast<int>(__float_as_uint(most) >> 23) - 127, -111) - 15;   // infinite or zero: whatever, the row stays so
                 const float by = power_of_two(-e2);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) w[i] = pack_half2(v[2 * i] * by, v[2 * i + 1] * by);
@@ -456,10 +461,9 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(ve[j]) : "r"(et + 16 + g8 + 8 * j));
                     value_e[j] = static_cast<float>(static_cast<int>(ve[j]) - 127);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) {
-                        x[n][2 * j] = (x[n][2 * j] + x2[n][2 * j]) * scale_of(ke[j]);
-                        x[n][2 * j + 1] = (x[n][2 * j + 1] + x2[n][2 * j + 1]) * scale_of(ke[j]);
-                    }
+                    for (int n = 0; n < NT; ++n)   // the row's power first: a large query times a large key's power is beyond fp32 where the score is not
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) x[n][2 * j + e] = (x[n][2 * j + e] + x2[n][2 * j + e]) * to_score[n][e] * scale_of(ke[j]);
                 }
             } else {
 #pragma unroll
@@ -474,7 +478,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[n][i] = (CODES ? x[n][i] : x[n][i] + x2[n][i]) * to_score[n][i & 1];
+                for (int i = 0; i < 4; ++i)
+                    if (!CODES) x[n][i] = (x[n][i] + x2[n][i]) * to_score[n][i & 1];
                 if (a.cap > 0.0f) {   // a polynomial where all of the warp's scores lie within the cap
                     if (__all_sync(0xffffffffu, fmaxf(fmaxf(fabsf(x[n][0]), fabsf(x[n][1])), fmaxf(fabsf(x[n][2]), fabsf(x[n][3]))) <= 1.0f)) {
                         unpair(tanh_inner2(pair(x[n][0], x[n][1])), x[n][0], x[n][1]);
@@ -528,7 +533,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     }
             }
             // weights: from rows of keys to the B operand's columns of rows of the tile by one transposition of 8 x 8 each
-            uint32_t weights[NT][2], weights_rest[NT][2];   // bf16: a second term each, so that the products carry sixteen bits of a weight
+            uint32_t weights[NT][2], weights_rest[NT][2];   // two terms each
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 float w[4];
@@ -538,12 +543,15 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     const float against = m[n][e] == -INFINITY ? 0.0f : m[n][e];   // nothing seen yet: every weight is 2^-inf = 0
                     const float p = exp2_fast(x[n][i] - against);
                     l[n][e] += p;
-                    w[i] = CODES ? exp2_fast(x[n][i] + value_e[i >> 1] - (ref[n][e] == -INFINITY ? 0.0f : ref[n][e])) : p;
+                    w[i] = CODES ? exp2_fast(x[n][i] + value_e[i >> 1] - (ref[n][e] == -INFINITY ? 0.0f : ref[n][e] - kLift)) : p;
                 }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     if constexpr (CODES) {
-                        weights[n][j] = transposed(pack_half2(w[2 * j], w[2 * j + 1]));
+                        const uint32_t first = pack_half2(w[2 * j], w[2 * j + 1]);
+                        const float2 held = unpack_half2(first);
+                        weights[n][j] = transposed(first);
+                        weights_rest[n][j] = transposed(pack_half2(w[2 * j] - held.x, w[2 * j + 1] - held.y));
                     } else {
                         const uint32_t first = ptx::pack_bf16x2(w[2 * j], w[2 * j + 1]);
                         weights[n][j] = transposed(first);
@@ -568,6 +576,8 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     for (int n = 0; n < NT; ++n) {
                         mma<true>(O[n][2 * i], f0, weights[n][0], weights[n][1]);
                         mma<true>(O[n][2 * i + 1], f1, weights[n][0], weights[n][1]);
+                        mma<true>(O[n][2 * i], f0, weights_rest[n][0], weights_rest[n][1]);
+                        mma<true>(O[n][2 * i + 1], f1, weights_rest[n][0], weights_rest[n][1]);
                     }
                 }
             } else {
@@ -615,7 +625,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     total_ml[r][0] = top;
                     total_ml[r][1] = sum;
                 }
-                const float f = share_of(CODES ? ref[n][e] : m[n][e], top);
+                const float f = share_of(CODES ? ref[n][e] - kLift : m[n][e], top);
                 float *to = merge + (warp * kRows + r) * S::kMergePitch;
 #pragma unroll
                 for (int u = 0; u < D16; ++u) {

@@ -295,8 +295,11 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
  *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
  *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they share no
- *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold;
- *           the order of sums, and so the last bits of a row, depend on the lengths of all sequences of the call.
+ *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.  Weights multiply values as fp32 where queries or pages are
+ *           fp32; else (gptb200_plan_attention_paged says which) in two 16-bit terms for few rows, off by 2^-16 of themselves at most, and rounded to bf16 once for prompts, off
+ *           by 2^-8 of themselves, where the sum that divides is that of the rounded ones.  Few rows over codes: a key whose weight times its value's power of two is below
+ *           2^-36 of the row's largest adds nothing to out, nor does an element of q below 2^-40 of its head's largest to a score.
+ *           The order of sums, and so the last bits of a row, depend on the lengths of all sequences of the call.
  *   All addresses are 16-byte aligned, pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
  *   other. */
 typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;
