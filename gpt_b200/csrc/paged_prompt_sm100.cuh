@@ -485,9 +485,10 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         if (b >= 0) ptx::mma_commit(v_empty(vs));
                         if (more) ptx::mma_commit(k_empty(ks));
                         if (b + 2 == seg.blocks) ptx::mma_commit(q_empty);   // the last scores
-                        if (!more) {
-                            ptx::mma_commit(o_full(0));
-                            ptx::mma_commit(o_full(1));
+                        if (!more) {   // a half without products has nothing to wait for: its phases are those that its warps have weights for, so that none passes unseen
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                if (begun[h]) ptx::mma_commit(o_full(h));
                         }
                     }
                     __syncwarp();
@@ -548,7 +549,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         const int r = quarter * 32 + lane;   // row within the half
         auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, DEV_TIMEOUT_EPILOGUE)); };
         bool ok = true;
-        int turns = 0;
+        int turns = 0, outputs = 0;   // blocks with scores of this half so far, tiles with outputs of it
         for (int tile = 0;; ++tile) {
             if (!pro::all_of(4 + h, 128, wait(seg_full(tile), segment_phase(tile)))) break;
             const Segment &seg = segment(tile);
@@ -687,7 +688,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 to[i] = rr < seg.rows ? static_cast<__nv_bfloat16 *>(a.out) + (seg.row0 + tk) * a.out_pitch + (seg.g * a.share + pr - tk * a.share) * dim + 8 * piece : nullptr;
             }
             const float by_whole = 1.0f / sum_rounded;
-            if (ok) ok = wait(o_full(h), tile & 1);
+            if (ok && begun) ok = wait(o_full(h), outputs++ & 1);
             ptx::tc_fence_after();
             if (!pro::all_of(4 + h, 128, ok)) break;
             if (h * 128 < seg.rows) {
