@@ -654,6 +654,18 @@ struct Parts {
     int floats;
 };
 
+// Eight elements of a pool of a kind.
+struct RawCodes8 {
+    uint2 w;
+    __device__ __forceinline__ void load(const uint8_t *p) { w = *reinterpret_cast<const uint2 *>(p); }
+    __device__ __forceinline__ void zero() { w = make_uint2(0u, 0u); }
+    __device__ __forceinline__ void get(float (&v)[8]) const { codes8(v, w, 1.0f); }
+};
+template <int KIND> struct Held8;
+template <> struct Held8<KIND_BF16> { using Raw = Raw8<__nv_bfloat16>; using Element = __nv_bfloat16; };
+template <> struct Held8<KIND_F32> { using Raw = Raw8<float>; using Element = float; };
+template <> struct Held8<KIND_E4M3> { using Raw = RawCodes8; using Element = uint8_t; };
+
 template <int KIND>
 __device__ __forceinline__ void load8_held(float (&v)[8], const Pages &p, int page, int which, int head, int token, int piece)
 {
@@ -666,56 +678,270 @@ __device__ __forceinline__ void load8_held(float (&v)[8], const Pages &p, int pa
         load8(v, static_cast<const float *>(p.data) + at * p.dim + piece * 8);
 }
 
-// One query row of one head, by a whole warp, from the definition: only keys that the row sees are read.  Sixteen lanes hold a head (eight elements each), so that
-// the warp's halves take every second key; a running maximum and sum per half, put together at the end.
-template <typename T, int KIND>
-__device__ void attention_row(const Attention &a, int s, int position, int row, int head, int lane)
+// Keys `from` to `to` of a sequence's head in groups of eight, which lie side by side in a page: one per turn and half of a warp, by a team's warps in turn.  `take` gets the group's
+// place in the pool (rows of keys or values; -1: the table names no page) and its first key; its page was looked up a turn before.  take: false ends it, for the whole warp.
+template <typename Take>
+__device__ __forceinline__ void over_groups(const Attention &a, int s, int g, int which, int from, int to, int rank, int warps, Take take)
 {
-    const int piece = lane & 15, half = lane >> 4, pieces = a.pages.dim / 8, g = head / a.share;
-    const bool active = piece < pieces;
-    float q[8] = {}, acc[8] = {}, m = -INFINITY, l = 0.0f;
-    if (active) load8(q, static_cast<const T *>(a.q) + row * a.q_pitch + head * a.pages.dim + piece * 8);
-    const int from = a.window ? max(0, position - a.window + 1) : 0, sinks = a.window ? min(a.sinks, from) : 0;
-    const int keys = position < 0 ? 0 : sinks + position - from + 1;
-    for (int i = 0; i < keys; i += 2) {   // the halves stay together: shuffles are the whole warp's
-        const int n = i + half, key = n < sinks ? n : from + n - sinks;
-        const bool on = n < keys;
-        float k[8] = {}, v[8] = {};
-        bool there = false;
-        if (on) {
-            const int page = page_of(a.batch, a.pages, s, key), token = key & ((1 << a.pages.page_shift) - 1);
-            there = page >= 0;
-            if (there && active) {
-                load8_held<KIND>(k, a.pages, page, 0, g, token, piece);
-                load8_held<KIND>(v, a.pages, page, 1, g, token, piece);
-            }
-        }
-        float x = 0.0f;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x = fmaf(q[e], k[e], x);
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        if (on && there) {
-            x *= a.scale;
-            if (a.cap > 0.0f) x = a.cap * tanhf(x / a.cap);
-            const float now = fmaxf(m, x), keep = m == -INFINITY ? 0.0f : expf(m - now), w = x == -INFINITY ? 0.0f : expf(x - now);
-            m = now;
-            l = fmaf(l, keep, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) acc[e] = fmaf(acc[e], keep, w * v[e]);
-        }
+    if (from > to) return;
+    const int half = (threadIdx.x & 31) >> 4, mask = (1 << a.pages.page_shift) - 1;
+    auto look_up = [&](int key0) { return key0 <= to && key0 + 7 >= from ? page_of(a.batch, a.pages, s, key0) : -1; };
+    int key0 = (from & ~7) + 8 * (2 * rank + half), page = look_up(key0);
+    for (; key0 - 8 * half <= to; key0 += 16 * warps) {   // the halves stay together: shuffles are the whole warp's
+        const long long at = page >= 0 ? a.pages.place(page, which, g, key0 & mask) : -1;
+        page = look_up(key0 + 16 * warps);
+        if (!take(at, key0)) return;
     }
-    const float other = __shfl_xor_sync(0xffffffffu, m, 16), top = fmaxf(m, other), f = m == -INFINITY ? 1.0f : expf(m - top);   // a half that saw nothing holds zeros
+}
+
+// One query row of one head, by a team of WARPS warps that `sync` brings together, from the definition: only keys that the row sees are read.  Sixteen lanes hold a head
+// (eight elements each), so that the halves of a warp take a group of eight keys each (fp32: in two steps); a running maximum and sum per half, put together at the end, the warps'
+// in `room` (kTeamRoom floats each).
+constexpr int kTeamRoom = 132;
+template <typename T, int KIND, int WARPS, typename Sync>
+__device__ void attention_row(const Attention &a, int s, int position, int row, int head, int rank, int lane, float *room, Sync sync)
+{
+    constexpr int kAhead = KIND == KIND_F32 ? 4 : 8;
+    using Raw = typename Held8<KIND>::Raw;
+    const int piece = lane & 15, half = lane >> 4, dim = a.pages.dim, g = head / a.share;
+    const bool active = piece < dim / 8;
+    float q[8] = {}, acc[8] = {}, m = -INFINITY, l = 0.0f;
+    if (active) load8(q, static_cast<const T *>(a.q) + row * a.q_pitch + head * dim + piece * 8);
+    const auto *data = static_cast<const typename Held8<KIND>::Element *>(a.pages.data) + piece * 8;
+    const long long value_rows = static_cast<long long>(a.pages.kv_heads) << a.pages.page_shift;   // from a key's row to its value's
+    auto over = [&](int from, int to) {
+        over_groups(a, s, g, 0, from, to, rank, WARPS, [&](long long at, int key0) {
+#pragma unroll
+            for (int u0 = 0; u0 < 8; u0 += kAhead) {
+                Raw k[kAhead], v[kAhead];
+                float k_scale[kAhead], v_scale[kAhead], x[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int key = key0 + u0 + u;
+                    const bool there = at >= 0 && key >= from && key <= to;
+                    k[u].zero();
+                    v[u].zero();
+                    k_scale[u] = v_scale[u] = 1.0f;
+                    x[u] = there ? 0.0f : -INFINITY;
+                    if (there && active) {
+                        k[u].load(data + (at + u0 + u) * dim);
+                        v[u].load(data + (at + u0 + u + value_rows) * dim);
+                        if (KIND == KIND_E4M3) {
+                            k_scale[u] = scale_of(a.pages.scales[at + u0 + u]);
+                            v_scale[u] = scale_of(a.pages.scales[at + u0 + u + value_rows]);
+                        }
+                    }
+                }
+                float dot[kAhead], now = m;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    float e8[8];
+                    k[u].get(e8);
+                    dot[u] = 0.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dot[u] = fmaf(q[e], KIND == KIND_E4M3 ? e8[e] * k_scale[u] : e8[e], dot[u]);
+                }
+#pragma unroll
+                for (int o = 8; o > 0; o >>= 1)
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], o);
+                if (a.cap > 0.0f) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) dot[u] = a.cap * tanhf(dot[u] * a.scale / a.cap);
+                } else {
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) dot[u] *= a.scale;
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    if (x[u] == 0.0f) x[u] = dot[u];
+                    now = fmaxf(now, x[u]);
+                }
+                const float keep = m == -INFINITY ? 0.0f : expf(m - now);
+                m = now;
+                l *= keep;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) acc[e] *= keep;
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const float w = x[u] == -INFINITY ? 0.0f : expf(x[u] - now);
+                    float e8[8];
+                    v[u].get(e8);
+                    l += w;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) acc[e] = fmaf(w, KIND == KIND_E4M3 ? e8[e] * v_scale[u] : e8[e], acc[e]);
+                }
+            }
+            return true;
+        });
+    };
+    const int low = a.window ? max(0, position - a.window + 1) : 0;
+    over(0, min(a.sinks, low) - 1);
+    over(low, position);
+    auto share_of = [](float of, float top) { return of == -INFINITY ? 1.0f : expf(of - top); };   // what saw nothing holds zeros (or NaN, which stay)
+    const float both = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16)), f = share_of(m, both);
     l *= f;
     l += __shfl_xor_sync(0xffffffffu, l, 16);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         acc[e] *= f;
         acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 16);
-        acc[e] = keys > 0 ? acc[e] / l : 0.0f;
     }
-    if (active && half == 0) store8(static_cast<T *>(a.out) + row * a.out_pitch + head * a.pages.dim + piece * 8, acc);
-    if (a.lse && lane == 0) a.lse[static_cast<long long>(row) * a.heads + head] = keys > 0 ? top + logf(l) : -INFINITY;
+    if (half == 0) {
+        store8(room + rank * kTeamRoom + piece * 8, acc);
+        if (piece == 0) *reinterpret_cast<float2 *>(room + rank * kTeamRoom + 128) = make_float2(both, l);
+    }
+    sync();
+    if (rank == 0 && half == 0) {
+        float top = -INFINITY, sum = 0.0f, out[8] = {};
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, room[w * kTeamRoom + 128]);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float by = share_of(room[w * kTeamRoom + 128], top);
+            float part[8];
+            load8(part, room + w * kTeamRoom + piece * 8);
+            sum = fmaf(room[w * kTeamRoom + 129], by, sum);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) out[e] = fmaf(part[e], by, out[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = position >= 0 ? out[e] / sum : 0.0f;
+        if (active) store8(static_cast<T *>(a.out) + row * a.out_pitch + head * dim + piece * 8, out);
+        if (a.lse && piece == 0) a.lse[static_cast<long long>(row) * a.heads + head] = position >= 0 ? top + logf(sum) : -INFINITY;
+    }
+    sync();
+}
+
+// ---- rows whose output is not finite though the sum of their weights is
+//
+// Either the row sees a value that makes it so, or the tile's product multiplied one that the row does not see by zero, which is NaN, or sums against an old maximum left
+// fp32's range.  In the first case the result stands: an element that is NaN where the row sees a NaN or infinities of both signs there, one that is infinite where it sees that
+// infinity.  All rows of a tile see nearly the same keys, so a team of warps goes over the values that all of these rows see once, and stops as soon as every element is accounted
+// for; each row then looks at the few others that it sees.  Rows that remain are formed again from their own keys alone.
+
+constexpr uint32_t kSeenNan = 0xffu, kSeenInfinities = 0xffff00u;   // a bit per element: NaN, plus infinity, minus infinity
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(const Raw8<T> &raw) { return raw.largest() >= 0x7f800000u; }
+template <typename T>
+__device__ __noinline__ uint32_t kinds_of(Raw8<T> raw)   // out of line: what a tile runs through once has to be fetched each time (917 -> 1014 us with twice the code)
+{
+    uint32_t kinds = 0;
+    float v[8];
+    raw.get(v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) kinds |= (v[e] != v[e] ? 1u : v[e] > FLT_MAX ? 0x100u : v[e] < -FLT_MAX ? 0x10000u : 0u) << e;
+    return kinds;
+}
+__device__ __forceinline__ bool not_finite(const RawCodes8 &raw) { return ((((raw.w.x & 0x7f7f7f7fu) + 0x01010101u) | ((raw.w.y & 0x7f7f7f7fu) + 0x01010101u)) & 0x80808080u) != 0; }
+__device__ __forceinline__ uint32_t kinds_of(RawCodes8 raw)   // the format's NaN: all bits but the sign
+{
+    const uint32_t x = ((raw.w.x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u, y = ((raw.w.y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+    return ((x * 0x00204081u) >> 28) | (((y * 0x00204081u) >> 28) << 4);   // a word's four bits side by side
+}
+// Elements that are not finite for which nothing that was seen accounts.
+__device__ __forceinline__ uint32_t open_kinds(uint32_t are, uint32_t seen) { return (are & ~(seen | ((seen >> 8) & (seen >> 16))) & kSeenNan) | (are & ~seen & kSeenInfinities); }
+
+struct UnsureRows {   // in shared memory
+    unsigned int rows[4], again[4];     // a bit per row; those that are formed again
+    unsigned int are[16], seen[16];     // kinds by eights of dimensions: among these rows' outputs, among the values that all of them see
+};
+
+// Kinds among the values of keys `from` to `to`, which all rows in question see, by a team's warps in turn; true: every element is accounted for.
+template <int KIND>
+__device__ inline bool look_through(const Attention &a, int s, int g, int from, int to, int rank, int warps, uint32_t are, uint32_t &seen, unsigned int *shared)
+{
+    const int lane = threadIdx.x & 31, piece = lane & 15, dim = a.pages.dim;
+    const bool active = piece < dim / 8;
+    const auto *data = static_cast<const typename Held8<KIND>::Element *>(a.pages.data) + piece * 8;
+    bool all = __all_sync(0xffffffffu, open_kinds(are, seen) == 0);
+    if (all) return true;
+    over_groups(a, s, g, 1, from, to, rank, warps, [&](long long at, int key0) {
+        typename Held8<KIND>::Raw v[8];
+        bool any = false;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            v[u].zero();
+            if (at >= 0 && active && key0 + u >= from && key0 + u <= to) v[u].load(data + (at + u) * dim);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) any = any || not_finite(v[u]);
+        if (any) {
+#pragma unroll
+            for (int u = 0; u < 8; ++u) seen |= kinds_of(v[u]);
+        }
+        seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
+        if (shared) {
+            if (lane < 16 && seen & ~*reinterpret_cast<volatile unsigned int *>(shared + piece)) atomicOr(shared + piece, seen);
+            __syncwarp();
+            seen |= *reinterpret_cast<volatile unsigned int *>(shared + piece);
+        }
+        all = __all_sync(0xffffffffu, open_kinds(are, seen) == 0);
+        return !all;
+    });
+    return all;
+}
+
+// The rows of u.rows (row r: packed row packed0 + r), by a team of WARPS warps that `sync` brings together; the outputs have been stored, and u.rows is known to all.
+// room: kTeamRoom floats per warp.
+template <typename T, int KIND, int WARPS, typename Sync>
+__device__ __noinline__ void settle_rows(const Attention &a, int s, int g, int row0, int pos0, int packed0, UnsureRows &u, int rank, float *room, Sync sync)
+{
+    const int lane = threadIdx.x & 31, piece = lane & 15, half = lane >> 4, dim = a.pages.dim;
+    const bool active = piece < dim / 8;
+    int first = 128, last = -1;
+    for (int w = 0; w < 4; ++w)
+        if (const unsigned int rows = u.rows[w]) {
+            first = min(first, 32 * w + __ffs(rows) - 1);
+            last = 32 * w + 31 - __clz(rows);
+        }
+    auto is_in = [&](int r) { return (u.rows[r >> 5] >> (r & 31) & 1) != 0; };
+    auto token_of = [&](int r) { return a.shares.divide(packed0 + r); };
+    auto head_of = [&](int r) { return g * a.share + packed0 + r - token_of(r) * a.share; };
+    auto stored = [&](int r, Raw8<T> &raw) {
+        raw.zero();
+        if (active && r <= last && is_in(r)) raw.load(static_cast<const T *>(a.out) + (row0 + token_of(r)) * a.out_pitch + head_of(r) * dim + piece * 8);
+    };
+    if (rank == 0 && half == 0) u.are[piece] = u.seen[piece] = u.again[piece & 3] = 0u;
+    sync();
+    uint32_t are = 0;
+    for (int r = first + 2 * rank + half; r <= last; r += 16 * WARPS) {   // the same rounds for both halves or one more, without shuffles
+        Raw8<T> raw[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) stored(r + 2 * WARPS * i, raw[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) are |= kinds_of(raw[i]);
+    }
+    if (are) atomicOr(u.are + piece, are);
+    sync();
+    const int p0 = pos0 + token_of(first), p1 = pos0 + token_of(last), low = a.window ? max(0, p1 - a.window + 1) : 0;
+    uint32_t seen = 0;
+    are = u.are[piece];
+    if (!look_through<KIND>(a, s, g, 0, min(min(a.sinks, low) - 1, p0), rank, WARPS, are, seen, u.seen)) look_through<KIND>(a, s, g, low, p0, rank, WARPS, are, seen, u.seen);
+    sync();
+    const uint32_t by_all = u.seen[piece];
+    if (__all_sync(0xffffffffu, open_kinds(are, by_all) == 0)) last = -1;   // the same in all warps: what accounts for all rows' elements does so for each row's
+    for (int r = first, n = 0; r <= last; ++r) {
+        if (!is_in(r) || n++ % WARPS != rank) continue;
+        const int token = token_of(r), position = pos0 + token, from = a.window ? max(0, position - a.window + 1) : 0;
+        Raw8<T> raw;
+        stored(r, raw);
+        are = kinds_of(raw);
+        seen = by_all;
+        // what this row sees and the others may not: behind the first of them, in front of the last one's window
+        if (look_through<KIND>(a, s, g, max(p0 + 1, from), position, 0, 1, are, seen, nullptr) || look_through<KIND>(a, s, g, p0 + 1, min(a.sinks, from) - 1, 0, 1, are, seen, nullptr) ||
+            look_through<KIND>(a, s, g, from, min(low - 1, p0), 0, 1, are, seen, nullptr))
+            continue;
+        if (lane == 0) atomicOr(u.again + (r >> 5), 1u << (r & 31));
+    }
+    sync();
+    for (int w = 0; w < 4; ++w)
+        for (unsigned int rest = u.again[w]; rest; rest &= rest - 1) {
+            const int r = 32 * w + __ffs(rest) - 1, token = token_of(r);
+            attention_row<T, KIND, WARPS>(a, s, pos0 + token, row0 + token, head_of(r), rank, lane, room, sync);
+        }
+    sync();   // what the next tile writes has been read
 }
 
 }  // namespace kvp

@@ -92,6 +92,32 @@ __device__ __forceinline__ bool all_of(int barrier, int threads, bool mine)
     return ok != 0;
 }
 
+struct HalfSync {   // the four softmax warps of a half
+    int barrier;
+    __device__ __forceinline__ void operator()() const { asm volatile("barrier.cta.sync %0, 128;" ::"r"(barrier) : "memory"); }
+};
+
+// bounded_wait whose time does not run while softmax warps look at rows once more: that ends by itself, however long the row.
+__device__ __forceinline__ bool patient_wait(uint32_t bar, uint32_t parity, volatile uint32_t *abort_flag, const volatile unsigned int *working, int *status, int code)
+{
+    if (ptx::mbar_try_wait(bar, parity)) return true;
+    long long t0 = clock64();
+    uint32_t spins = 0;
+    while (true) {
+        if (ptx::mbar_try_wait(bar, parity)) return true;
+        if ((++spins & 31u) == 0) {
+            if (*abort_flag) return false;
+            if (*working) {
+                t0 = clock64();
+            } else if (clock64() - t0 > kWaitTimeoutCycles) {
+                *abort_flag = 1u;
+                atomicCAS(status, 0, code);
+                return false;
+            }
+        }
+    }
+}
+
 // Bits 0 .. n - 1 of a word.
 __device__ __forceinline__ uint32_t bits_below(int n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; }
 
@@ -163,6 +189,8 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
     __shared__ long long row_at[2][2][kPromptKeys];   // keys / values, in turn: element of a key's row, -1: zeros
     __shared__ int row_e[2][2][kPromptKeys];          // codes: exponent
     __shared__ int arrived_last[2];
+    __shared__ UnsureRows unsure[2];
+    __shared__ unsigned int working;   // halves that look at rows once more, which may take longer than any wait's limit
     __shared__ Segment segments[kPromptSegments];
     const Attention &a = args.a;
     const uint32_t base = (ptx::smem_u32(prompt_smem) + 1023u) & ~1023u;
@@ -206,6 +234,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         ptx::mbar_init(q_empty, 1);
         ptx::mbar_init(drain, 1);
         *abort_flag = 0u;
+        working = 0u;
         ptx::fence_mbar_init();
     }
     if (warp == 4) {
@@ -263,7 +292,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         };
         // the two warps learn together whether there is another tile
         auto another = [&] {
-            const bool ok = bounded_wait(seg_full(tile), segment_phase(tile), abort_flag, status, DEV_TIMEOUT_PRODUCER);
+            const bool ok = pro::patient_wait(seg_full(tile), segment_phase(tile), abort_flag, &working, status, DEV_TIMEOUT_PRODUCER);
             return pro::all_of(2 + which, 64, ok) && segment(tile).blocks > 0;
         };
         bool more = another();
@@ -274,7 +303,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             const int packed0 = segment(tile).packed0, rows = segment(tile).rows, q_turn = tile & 1;
             const __nv_bfloat16 *q = static_cast<const __nv_bfloat16 *>(a.q) + segment(tile).row0 * a.q_pitch + segment(tile).g * a.share * dim;
             const uint32_t full = which ? v_full(stage) : k_full(stage);
-            bool ok = bounded_wait(which ? v_empty(stage) : k_empty(stage), ((n / S::kStages) & 1) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);
+            bool ok = pro::patient_wait(which ? v_empty(stage) : k_empty(stage), ((n / S::kStages) & 1) ^ 1, abort_flag, &working, status, DEV_TIMEOUT_PRODUCER);
             if (!pro::all_of(2 + which, 64, ok)) break;
             const uint32_t dst = ring + stage * S::kTile;
             if constexpr (!CODES) {
@@ -402,7 +431,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 ptx::mbar_arrive(full);
             }
             if (first) {   // queries, when the tile before has no more use for its own: all four warps, a row's pieces of eight side by side
-                ok = bounded_wait(q_empty, q_turn ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER);   // run out: the warps leave together at the next block
+                ok = pro::patient_wait(q_empty, q_turn ^ 1, abort_flag, &working, status, DEV_TIMEOUT_PRODUCER);   // run out: the warps leave together at the next block
 #pragma unroll 4
                 for (int i = threadIdx.x; ok && i < kPromptRows * 8 * NB; i += 128) {
                     const int r = i / (8 * NB), c = i % (8 * NB), packed = packed0 + r, token = a.shares.divide(packed);
@@ -424,7 +453,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             const uint32_t idesc_o = ptx::make_idesc_bf16(128, 16 * steps, false, true);
             const ptx::SmemDesc dq = ptx::smem_desc_words(q_base, 16, 1024, ptx::kLayoutSw128), dk = ptx::smem_desc_words(k_base, 16, 1024, ptx::kLayoutSw128),
                                 dv = ptx::smem_desc_words(v_base, kPromptBlock, 1024, ptx::kLayoutSw128);
-            auto wait = [&](uint32_t b, uint32_t parity, int code) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, code)); };
+            auto wait = [&](uint32_t b, uint32_t parity, int code) { return __all_sync(0xffffffffu, pro::patient_wait(b, parity, abort_flag, &working, status, code)); };
             bool ok = true;
             int n = 0, turns[2] = {0, 0};
             for (int tile = 0; ok; ++tile) {
@@ -499,7 +528,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             }
             if (issuer) ptx::mma_commit(drain);
             __syncwarp();
-            bounded_wait(drain, 0u, abort_flag, status, DEV_TIMEOUT_DRAIN);
+            pro::patient_wait(drain, 0u, abort_flag, &working, status, DEV_TIMEOUT_DRAIN);
         } else if (warp == 5) {
             int n = 0;
             bool go = range.begin < range.end;
@@ -532,7 +561,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 } else {
                     ended = 1;   // the last entry: no blocks
                 }
-                if (!__all_sync(0xffffffffu, bounded_wait(seg_empty(n), segment_phase(n) ^ 1, abort_flag, status, DEV_TIMEOUT_PRODUCER))) break;
+                if (!__all_sync(0xffffffffu, pro::patient_wait(seg_empty(n), segment_phase(n) ^ 1, abort_flag, &working, status, DEV_TIMEOUT_PRODUCER))) break;
                 if (lane == 0) {
                     segments[n % kPromptSegments] = seg;
                     ptx::mbar_arrive(seg_full(n));
@@ -547,7 +576,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
         const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t s_addr = tmem + lanes + 128 * h, o_addr = tmem + lanes + 256 + 128 * h;
         const int r = quarter * 32 + lane;   // row within the half
-        auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, bounded_wait(b, parity, abort_flag, status, DEV_TIMEOUT_EPILOGUE)); };
+        auto wait = [&](uint32_t b, uint32_t parity) { return __all_sync(0xffffffffu, pro::patient_wait(b, parity, abort_flag, &working, status, DEV_TIMEOUT_EPILOGUE)); };
         bool ok = true;
         int turns = 0, outputs = 0;   // blocks with scores of this half so far, tiles with outputs of it
         for (int tile = 0;; ++tile) {
@@ -717,6 +746,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                     if (SUMS && there) a.lse[row * a.heads + head] = sees ? top * kLn2 + logf(total) : -INFINITY;
                 };
                 bool done = seg.whole;
+                float divisor = sum_rounded;
                 if (seg.whole) {
                     for (int c = 0; c < 16 * steps; c += 32) {
                         uint32_t o[32];
@@ -762,6 +792,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                             total_rounded = fmaf(ml.z, f, total_rounded);
                         }
                         const float by = 1.0f / total_rounded;
+                        divisor = total_rounded;
                         for (int c = 0; c < 16 * steps; c += 32) {
                             float v[32] = {};
                             for (int b = b0; b <= b1; ++b) {
@@ -779,12 +810,13 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                         store_sum(top, total);
                     }
                 }
-                // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is
-                // formed once more from its own keys alone.
-                __syncwarp();
-                for (uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && check != 0.0f); bad; bad &= bad - 1) {
-                    const int p = seg.packed0 + h * 128 + quarter * 32 + __ffs(bad) - 1;
-                    attention_row<__nv_bfloat16, kind>(a, seg.s, seg.pos0 + a.shares.divide(p), seg.row0 + a.shares.divide(p), seg.g * a.share + p - a.shares.divide(p) * a.share, lane);
+                const uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && check != 0.0f && divisor > 0.0f && divisor <= FLT_MAX);
+                if (lane == 0) unsure[h].rows[quarter] = bad;
+                if (!pro::all_of(4 + h, 128, bad == 0)) {
+                    if (r == 0) atomicAdd(&working, 1u);
+                    settle_rows<__nv_bfloat16, kind, 4>(a, seg.s, seg.g, seg.row0, seg.pos0, seg.packed0 + h * 128, unsure[h], quarter, reinterpret_cast<float *>(gen + (staging - base) + 4 * h * 2048),
+                                                        pro::HalfSync{4 + h});
+                    if (r == 0) atomicSub(&working, 1u);
                 }
             }
             ptx::tc_fence_before();   // the accumulator has been read: the next tile's products may write it (they wait for its weights)

@@ -21,7 +21,7 @@ constexpr float kLog2E = 1.4426950408889634f;
 
 constexpr int kFewBlocks = kFewPerSm * 160, kRowsBlocks = kRowsPerSm * 160;   // of a grid, at most: so many parts' sums have room in shared memory
 constexpr int kFewSmem = kFewBlocks * 8;   // the warps' sums, 132 floats each, have room in it
-static_assert(kFewSmem >= kTokensWarps * 132 * 4);
+static_assert(kFewSmem >= kTokensWarps * 132 * 4 && kTeamRoom <= 132);
 __host__ __device__ constexpr int rows_smem(int each) { return (rows_tile(each) + 2 * kRowsKeys) * 132 * 4 + kTokensWarps * kRowsKeys * each * 4; }
 static_assert(rows_smem(4) / 8 >= kRowsBlocks);
 
@@ -39,7 +39,7 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
     using tok::exp2_fast;
     extern __shared__ __align__(16) float rows_shared[];
     __shared__ float warp_ml[kTokensWarps][2], total_ml[1][2];
-    __shared__ unsigned int bad_rows;
+    __shared__ UnsureRows unsure;
     __shared__ int arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
@@ -67,7 +67,7 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
             }
         };
         look_up(0);
-        if (threadIdx.x == 0) bad_rows = 0;
+        if (threadIdx.x < 4) unsure.rows[threadIdx.x] = 0u;
         for (int it = 0; it < part.blocks; ++it) {
             const int t = first_key(it), page[2] = {pages[0], pages[1]};
             look_up(it + 1);
@@ -145,7 +145,7 @@ paged_few_kernel(const __grid_constant__ TokensArgs args)
         for (int e = 0; e < 8; ++e) acc[e] *= to_top;
         if (half == 0) store8(rows_shared + warp * 132 + piece * 8, acc);
         __syncthreads();
-        finish_tile<T, KIND, 1, kTokensWarps>(a, args.parts, place, part, 1, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), kFewBlocks, &bad_rows, &arrived_last);
+        finish_tile<T, KIND, 1, kTokensWarps>(a, args.parts, place, part, 1, rows_shared, 132, total_ml, reinterpret_cast<float2 *>(rows_shared), kFewBlocks, unsure, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }
@@ -161,7 +161,7 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
     extern __shared__ __align__(16) float rows_shared[];
     __shared__ float total_ml[kRowsTile][2];
     __shared__ long long key_row[2][kRowsKeys];   // in turn: a key's row among its page's, -1: zeros
-    __shared__ unsigned int bad_rows;
+    __shared__ UnsureRows unsure;
     __shared__ int arrived_last;
     float *queries = rows_shared, *keys = queries + kRowsTile * kPitch, *values = keys + kRowsKeys * kPitch, *weights = values + kRowsKeys * kPitch;   // weights [warp][key][row of the warp]
     const Attention &a = args.a;
@@ -192,7 +192,7 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
             store8(queries + r * kPitch + c * 8, v);
         }
         if (warp == 0) look_up(0);
-        if (threadIdx.x == 0) bad_rows = 0;
+        if (threadIdx.x < 4) unsure.rows[threadIdx.x] = 0u;
         float m[kRowsEach], l[kRowsEach], O[kRowsEach][4] = {};
         int pos[kRowsEach];
 #pragma unroll
@@ -292,7 +292,7 @@ paged_rows_kernel(const __grid_constant__ TokensArgs args)
             if (lane_d < dim && lane_key == 0) *reinterpret_cast<float4 *>(queries + (kRowsEach * warp + i) * kPitch + lane_d) = make_float4(O[i][0], O[i][1], O[i][2], O[i][3]);
         }
         __syncthreads();
-        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), rows_smem(kRowsEach) / 8, &bad_rows, &arrived_last);
+        finish_tile<T, KIND, kRowsTile, 1>(a, args.parts, place, part, rows, queries, kPitch, total_ml, reinterpret_cast<float2 *>(rows_shared), rows_smem(kRowsEach) / 8, unsure, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }

@@ -48,7 +48,7 @@ struct TokensShape {
     static constexpr int kMergePitch = kDim + 4;
     static constexpr int kMerge = kTokensWarps * kRows * kMergePitch * 4;
     static constexpr int kSmem = kRows * kQPitch + (kRing > kMerge ? kRing : kMerge), kMaxBlocks = kPerSm * 160;
-    static_assert((kSmem - kRows * kQPitch) / 8 >= kMaxBlocks);   // of the grid: a tile's parts, at most
+    static_assert((kSmem - kRows * kQPitch) / 8 >= kMaxBlocks && kSmem - kRows * kQPitch >= kTokensWarps * kTeamRoom * 4);   // of the grid: a tile's parts, at most
 };
 
 namespace tok {
@@ -158,12 +158,16 @@ struct TokensArgs {
     Cut cut;
 };
 
+struct BlockSync {
+    __device__ __forceinline__ void operator()() const { __syncthreads(); }
+};
+
 // The end of a tile, for a block of kTokensThreads threads that holds its rows' sums in shared memory: merge [SUMS][ROWS][pitch] weighted values (added up here) against
 // total_ml [ROWS] = (maximum in base 2, sum).  A whole tile is stored; else the part goes to scratch, and the block that arrives last puts the parts together.
-// sums: room for as many pairs, one per block of the grid at least; it may be `merge` itself.  bad_rows is zero on entry.
+// sums: room for as many pairs, one per block of the grid and kTeamRoom / 2 per warp at least; it may be `merge` itself.  unsure.rows is zero on entry.
 template <typename T, int KIND, int ROWS, int SUMS>
 __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &parts, const Place &place, const Part &part, int rows, const float *merge, int pitch,
-                                            float (*total_ml)[2], float2 *sums, int room, unsigned int *bad_rows, int *arrived_last)
+                                            float (*total_ml)[2], float2 *sums, int room, UnsureRows &unsure, int *arrived_last)
 {
     constexpr int kSlot = (ROWS > kTokensMaxRows ? ROWS : kTokensMaxRows) * 128;   // a part in scratch: values, then maxima and sums
     constexpr float kLn2 = 0.69314718055994531f;
@@ -178,7 +182,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
             v[e] *= inv;
             fine = fine && fabsf(v[e]) <= FLT_MAX;
         }
-        if (!fine) atomicOr(bad_rows, 1u << r);
+        if (!fine && sum > 0.0f && sum <= FLT_MAX) atomicOr(unsure.rows, 1u << r);   // with any other sum the row is NaN by definition
         store8(static_cast<T *>(a.out) + row * a.out_pitch + head * dim + c * 8, v);
         if (a.lse && c == 0) a.lse[static_cast<long long>(row) * a.heads + head] = sees ? top * kLn2 + logf(sum) : -INFINITY;
     };
@@ -255,14 +259,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
         }
     }
     __syncthreads();
-    // A row that is not finite: a value that it does not see, but another row of its tile does, may be the reason (0 * inf in the product), so it is formed once more
-    // from its own keys alone.
-    int n = 0;
-    for (unsigned int rest = *bad_rows; rest; rest &= rest - 1, ++n) {
-        if (n % kTokensWarps != warp) continue;
-        const int packed = packed0 + __ffs(rest) - 1, token = a.shares.divide(packed);
-        attention_row<T, KIND>(a, place.s, place.q.pos0 + token, place.q.row0 + token, place.g * a.share + packed - token * a.share, lane);
-    }
+    if (unsure.rows[0]) settle_rows<T, KIND, kTokensWarps>(a, place.s, place.g, place.q.row0, place.q.pos0, packed0, unsure, warp, reinterpret_cast<float *>(sums), BlockSync());
     __syncthreads();   // what the next tile writes again has been read
 }
 
@@ -279,7 +276,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
     constexpr float kLog2e = 1.4426950408889634f;
     extern __shared__ __align__(16) uint8_t tokens_smem[];
     __shared__ float merge_ml[kTokensWarps][kRows][2], total_ml[kRows][2], row_power[kRows];
-    __shared__ unsigned int bad_rows;
+    __shared__ UnsureRows unsure;
     __shared__ int arrived_last;
     const Attention &a = args.a;
     grid_dependency_wait();
@@ -400,7 +397,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             }
             if (c < 2 * D16) ptx::sts128(q_tile + r * S::kQPitch + c * 16, w[0], w[1], w[2], w[3]);
         }
-        if (threadIdx.x == 0) bad_rows = 0;
+        if (threadIdx.x < 4) unsure.rows[threadIdx.x] = 0u;
         __syncthreads();
         // queries as B operands: columns are rows of the tile
         uint32_t qf[NT][D16][2];
@@ -634,7 +631,7 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                 }
             }
         __syncthreads();
-        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), (S::kSmem - kRows * S::kQPitch) / 8, &bad_rows, &arrived_last);
+        finish_tile<__nv_bfloat16, kind, kRows, kTokensWarps>(a, args.parts, place, part, rows, merge, S::kMergePitch, total_ml, reinterpret_cast<float2 *>(merge), (S::kSmem - kRows * S::kQPitch) / 8, unsure, &arrived_last);
         if (!advance(a, range, place, at, args.cut)) break;
     }
 }

@@ -63,3 +63,173 @@ def test_rows_formed_again_beside_tiles_of_one_half(backend, kind, bad_rows):
     check_wide(c, q, out, sums, share, "bf16", 0.125)
     got = out.double().cpu()
     assert torch.isnan(got[64 - bad_rows:64, 5::64]).all() and torch.isfinite(got[:64 - bad_rows]).all() and torch.isfinite(got[64:]).all()
+
+
+def kinds(x):
+    """0 finite, 1 NaN, 2 infinite, 3 minus infinite."""
+    return torch.where(torch.isnan(x), 1, torch.where(torch.isposinf(x), 2, torch.where(torch.isneginf(x), 3, 0)))
+
+
+def kinds_by_definition(c, heads, window, sinks):
+    """[rows, heads, dim] of the outputs, from the values that each row sees (all scores finite): every weight is positive."""
+    want = torch.zeros(c.rows, heads, c.dim, dtype=torch.int64)
+    for s, n in enumerate(c.counts):
+        length, r0 = c.lengths[s], int(c.starts_cpu[s])
+        v = c.sequence(s)[1]
+        key = torch.arange(length)
+        for i in range(n):
+            at = length - n + i
+            seen = (key <= at) & ((at - key < window) | (key < sinks) if window else key >= 0)
+            x = v[:, seen]
+            nan, high, low = torch.isnan(x).any(1), torch.isposinf(x).any(1), torch.isneginf(x).any(1)
+            kind = torch.where(nan | (high & low), 1, torch.where(high, 2, torch.where(low, 3, 0)))
+            want[r0 + i] = kind.repeat_interleave(heads // c.kv_heads, 0)
+    return want.reshape(c.rows, -1)
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "bf16"), ("bf16", "e4m3"), ("f32", "f32"), ("f32", "e4m3"), ("bf16", "f32")])
+@pytest.mark.parametrize("counts", [[1, 1, 1], [3, 2, 1], [40, 1, 33], [200, 100, 7]])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+def test_kinds_of_what_is_not_finite(backend, dtype, kind, counts, window, sinks):
+    """NaN and infinities at first, old, new and last tokens of a batch: an output is of the kind that the values its row sees make it, and all others are right."""
+    inf, nan = float("inf"), float("nan")
+    lengths, dim, heads = [400, 300, 40], 64, 4
+    c = Cache(kind, lengths, counts, 2, dim, 16, seed=3)
+    spots = [(0, 0, 0, inf), (0, 3, 1, -inf), (0, 200, 2, nan), (0, 399, 3, nan), (0, 390, 4, inf), (0, 392, 4, -inf), (0, 398, 6, inf), (1, 1, 7, nan), (1, 4, 63, -inf), (1, 299, 62, inf), (1, 270, 9, inf),
+             (1, 230, 9, -inf), (1, 231, 10, inf), (0, 321, 11, nan), (0, 320, 11, inf)]
+    for s, position, element, value in spots:
+        put(c, kind, s, position, value, heads=position % 2, element=element)
+    c.cuda()
+    q, _ = rows_in(c.rows, heads * dim, dtype, 0, 8)
+    out, sums = attend(backend, c, q, heads, dtype, 0.125, 0.0, window, sinks)
+    backend.synchronize()
+    got = out.double().cpu()
+    assert torch.equal(kinds(got), kinds_by_definition(c, heads, window, sinks))
+    # without them, where rows are finite: the same
+    for s, position, element, value in spots:
+        put(c, kind, s, position, 0.0, heads=position % 2, element=element)
+    c.values[torch.isnan(c.values)] = 0.0
+    want, lse, spread, slack = c.attention(q, heads, 0.125, 0.0, window, sinks)
+    bound = spread * (2.0 ** -7 + 2 * (dim + 8) * 2.0 ** -23 * slack + 2.0 ** -17) + want.abs() * (2.0 ** -8 if dtype == "bf16" else 2.0 ** -24)
+    fine = torch.isfinite(got)
+    assert ((got - want).abs() <= bound + 1e-30)[fine].all()
+    assert ((sums[:c.rows].double().cpu() - lse).abs() <= 2 * (dim + 8) * 2.0 ** -23 * slack.reshape(c.rows, heads, -1)[:, :, 0] + 2.0 ** -17 * (1 + lse.abs())).all()
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32")])
+@pytest.mark.parametrize("count,share", [(1, 1), (1, 8), (2, 8), (40, 2), (300, 1)])
+def test_sums_that_would_leave_the_range(backend, dtype, kind, count, share):
+    """Weights stand against a first score that later ones exceed by a factor of e^19, and values near the type's largest are multiplied by them: the outputs are in range."""
+    length, dim = 300 + count, 64
+    c = Cache(kind, [length], [count], 1, dim, 16, seed=3)
+    for position in range(length):
+        page, token = int(c.table_cpu[0, position // 16]), position % 16
+        row = torch.zeros(2, dim)
+        row[0, 0] = 0.0 if position == 0 else 19.0 if position in (20, 170) else -40.0
+        row[1] = 2.0 ** 125 if position in (20, 170) else 1.0
+        c.data_cpu[page, :, 0, token] = row.to(c.TYPES[kind])
+        c.values[page, :, 0, token] = row.double()
+    c.cuda()
+    q = torch.zeros(count, share * dim, dtype=torch.bfloat16 if dtype == "bf16" else torch.float32, device="cuda")
+    q[:, ::dim] = 1.0
+    out, sums = attend(backend, c, q, share, dtype, 1.0)
+    backend.synchronize()
+    check(c, q, out, sums, share, dtype, 1.0)
+
+
+def least_ms(call, turns=8):
+    """The shortest of some calls' times."""
+    begin, end, got = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True), []
+    for _ in range(turns):
+        begin.record()
+        call()
+        end.record()
+        end.synchronize()
+        got.append(begin.elapsed_time(end))
+    return min(got)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("which,position,value", [(1, 0, float("nan")), (0, 0, float("nan")), (1, 0, float("inf")), (1, 8191, float("nan"))])
+def test_a_poisoned_prompt_beside_a_healthy_one(backend, kind, which, position, value):
+    """What a row sees makes it NaN or infinite: it is not formed again for that, the other sequence is as it was, and the call takes no more than twice the time."""
+    heads, dim, lengths = 32, 128, [8192, 2000]
+    c = Cache(kind, lengths, lengths, 8, dim, 64, seed=3).cuda()
+    q, _ = rows_in(c.rows, heads * dim, "bf16", 0, 8)
+    out = torch.empty_like(q)
+    call = lambda: backend.attention_paged(out, out.stride(0), None, q, q.stride(0), 0, heads, c.pages, c.batch, dim ** -0.5)   # noqa: E731
+    healthy = least_ms(call)
+    clean = out.clone()
+    page, token = int(c.table_cpu[0, position // 64]), position % 64
+    value = float("nan") if kind == "e4m3" else value
+    if kind == "e4m3":
+        c.data.view(torch.uint8)[page, which, :, token, 5] = 0x7f
+    else:
+        c.data[page, which, :, token, 5] = value
+    poisoned = least_ms(call)
+    backend.synchronize()
+    assert torch.equal(out[8192:], clean[8192:])
+    mine, before = out[:8192].reshape(8192, heads, dim), clean[:8192].reshape(8192, heads, dim)
+    if which == 0:
+        assert torch.isnan(mine[position:]).all() and torch.equal(mine[:position], before[:position])
+    else:
+        sees = mine[position:, :, 5]
+        assert torch.isnan(sees).all() if value != value else (sees == value).all()
+        if position == 0:
+            keep = [d for d in range(dim) if d != 5]
+            assert torch.equal(mine[:, :, keep], before[:, :, keep])
+        else:       # rows of the last tiles that do not see it were formed again, in fp32: off by the weights' rounding
+            keep = torch.ones_like(mine, dtype=torch.bool)
+            keep[position:, :, 5] = False
+            assert torch.isfinite(mine[keep]).all() and ((mine - before).abs()[keep] <= 2.0 ** -7 * before.abs()[keep] + 2.0 ** -6).all()
+    print(f"{kind} {which} {position} {value}: healthy {healthy * 1e3:.0f} us, poisoned {poisoned * 1e3:.0f} us")
+    if position == 0:
+        assert poisoned <= 2.0 * healthy, (poisoned, healthy)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("position,value", [(0, float("nan")), (30000, float("nan")), (30000, float("inf"))])
+def test_poisoned_tokens_beside_healthy_ones(backend, kind, position, value):
+    heads, dim, lengths = 16, 128, [40000, 50000, 7, 20000]
+    c = Cache(kind, lengths, [1] * 4, 4, dim, 64, seed=3).cuda()
+    q, _ = rows_in(c.rows, heads * dim, "bf16", 0, 8)
+    out = torch.empty_like(q)
+    call = lambda: backend.attention_paged(out, out.stride(0), None, q, q.stride(0), 0, heads, c.pages, c.batch, dim ** -0.5)   # noqa: E731
+    healthy = least_ms(call)
+    clean = out.clone()
+    page, token = int(c.table_cpu[0, position // 64]), position % 64
+    value = float("nan") if kind == "e4m3" else value
+    if kind == "e4m3":
+        c.data.view(torch.uint8)[page, 1, :, token, 5] = 0x7f
+    else:
+        c.data[page, 1, :, token, 5] = value
+    poisoned = least_ms(call)
+    backend.synchronize()
+    assert torch.equal(out[1:], clean[1:])
+    sees = out[0].reshape(heads, dim)[:, 5]
+    assert torch.isnan(sees).all() if value != value else (sees == value).all()
+    keep = [d for d in range(dim) if d != 5]
+    off = (out[0].reshape(heads, dim)[:, keep].float() - clean[0].reshape(heads, dim)[:, keep].float()).abs()
+    assert (off <= 2.0 ** -7 * clean[0].reshape(heads, dim)[:, keep].float().abs() + 2.0 ** -12).all()
+    print(f"{kind} {position} {value}: healthy {healthy * 1e3:.0f} us, poisoned {poisoned * 1e3:.0f} us")
+
+
+def test_rows_formed_again_for_longer_than_a_wait_may_take(backend):
+    """The last of 64 new tokens behind 400 000 others holds a NaN that the 63 before it do not see: all of theirs are formed again, which takes a second or so, while the other warps wait."""
+    length, count, share, dim = 400000, 64, 4, 64
+    c = Cache("bf16", [length, 50], [count, 20], 1, dim, 64, seed=3)
+    want, _, spread, slack = c.attention(rows_in(count + 20, share * dim, "bf16", 0, 8)[0], share, 0.125)
+    page, token = int(c.table_cpu[0, (length - 1) // 64]), (length - 1) % 64
+    c.data_cpu[page, 1, :, token, 5] = float("nan")
+    c.cuda()
+    q, _ = rows_in(c.rows, share * dim, "bf16", 0, 8)
+    out = torch.empty_like(q)
+    took = least_ms(lambda: backend.attention_paged(out, out.stride(0), None, q, q.stride(0), 0, share, c.pages, c.batch, 0.125), 1)
+    backend.synchronize()
+    print(f"{took:.0f} ms")
+    got = out.double().cpu()
+    assert torch.isnan(got[count - 1, 5::64]).all()
+    bound = spread * (2.0 ** -7 + 2 * (dim + 8) * 2.0 ** -23 * slack + 2.0 ** -17) + want.abs() * 2.0 ** -8
+    keep = torch.ones_like(got, dtype=torch.bool)
+    keep[count - 1, 5::64] = False
+    assert ((got - want).abs() <= bound)[keep].all()
