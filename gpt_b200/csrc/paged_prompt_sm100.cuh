@@ -276,7 +276,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
             if (boxes) {
                 if (t * args.box_rows < kPromptKeys) {
                     const int key = key0 + t * args.box_rows, page = page_of(a.batch, a.pages, seg.s, key);
-                    row_at[which][turn][t * args.box_rows] = a.pages.place(max(page, 0), which, seg.g, key & mask);
+                    row_at[which][turn][t * args.box_rows] = page >= 0 ? a.pages.place(page, which, seg.g, key & mask) : -args.box_rows;   // no page: a box in front of the pool, zeros
                 }
                 return;
             }

@@ -233,3 +233,32 @@ def test_rows_formed_again_for_longer_than_a_wait_may_take(backend):
     keep = torch.ones_like(got, dtype=torch.bool)
     keep[count - 1, 5::64] = False
     assert ((got - want).abs() <= bound)[keep].all()
+
+
+@pytest.mark.parametrize("dtype,kind", [("bf16", "bf16"), ("bf16", "e4m3"), ("f32", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("count", [1, 40, 300])
+@pytest.mark.parametrize("page", [16, 64, 256])
+@pytest.mark.parametrize("entry", [-1, -2**31, 2**31 - 1, "past"])
+def test_a_page_that_is_none_brings_in_no_other(backend, dtype, kind, count, page, entry):
+    """An entry of the table that names no page of the pool: nothing of the pool's pages that the sequence does not own takes part, whatever they hold."""
+    import gpt_b200
+    lengths, dim = [1200, 700], 64
+    seed = next(s for s in range(100) if not {0} & set(Cache(kind, lengths, [count] * 2, 2, 8, page, seed=s).used))
+    c = Cache(kind, lengths, [count] * 2, 2, dim, page, seed=seed)
+    foreign = [p for p in range(c.num_pages) if p not in c.used]
+    assert 0 in foreign
+    c.cuda()
+    c.table[0, 1] = c.num_pages if entry == "past" else entry
+    q, _ = rows_in(c.rows, 4 * dim, dtype, 0, 8)
+    got = []
+    for fill in (0.0, float("nan")):
+        data = c.data.float()
+        data[foreign] = fill
+        c.data.copy_(data.to(c.data.dtype))
+        out, sums = attend(backend, c, q, 4, dtype, 0.125)
+        with pytest.raises(gpt_b200.GptB200Error) as e:
+            backend.synchronize()
+        assert e.value.status == 1
+        got.append((out.clone(), sums.clone()))
+    for a, b in zip(*got):
+        assert torch.isfinite(b[:c.rows].float()).all() and torch.equal(a, b)
