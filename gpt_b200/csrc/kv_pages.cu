@@ -86,8 +86,9 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
     a.columns = std::min(all_columns, kvp::kRowThreads);
     const int side = kvp::kRowThreads / a.columns, threads = (side * a.columns + 31) / 32 * 32;
     a.rows_per_block = std::max(1, std::min({kvp::kRowMax, kvp::row_turns(WRITE) * side, rows->rows / (2 * ctx->num_sms)}));
-    const int blocks = (rows->rows + a.rows_per_block - 1) / a.rows_per_block;
-    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(blocks), dim3(threads), 0, a); };
+    a.row_blocks = static_cast<unsigned int>((1LL * rows->rows + a.rows_per_block - 1) / a.rows_per_block);
+    const unsigned int checkers = static_cast<unsigned int>((1LL * rows->sequences + kvp::kCheckedStarts - 1) / kvp::kCheckedStarts);
+    auto launch = [&](auto kernel) { return launch_chained(ctx, kernel, dim3(a.row_blocks + checkers), dim3(threads), 0, a); };
     auto launch_kind = [&](auto type) {
         using T = decltype(type);
         switch (pages->kind) {

@@ -152,6 +152,7 @@ __device__ __forceinline__ int exponent_for(float most)
 // codes by instructions (a row's largest value, a conversion per pair), which is why the largest value of bf16 rows is found two at a time on their bits.
 constexpr int kRowThreads = 256;
 constexpr int kRowMax = 64;    // rows per block, at most
+constexpr int kCheckedStarts = 1024;   // sequences whose starts a block checks
 // Pieces under way per thread, blocks per SM, rows per thread.  Writing (24 400 rows of 8 heads of 128 from bf16 to codes): 39.5 us with four blocks of four pieces each, 5.1 TB/s;
 // 56 us with rows looked up by a warp each and two blocks.  Reading (16 600 rows of 4 heads back): 25.5 us with eight blocks and one piece, 4.3 TB/s; 33 us with
 // four pieces each.
@@ -167,6 +168,7 @@ struct RowsArgs {
     int lanes_log2;      // lanes per head
     int columns;         // threads that share a row: all its pieces, or the block
     int rows_per_block;
+    unsigned int row_blocks;   // blocks that have rows; those behind them check starts
 };
 
 // Eight elements as they lie in memory.
@@ -222,7 +224,16 @@ kv_rows_kernel(const RowsArgs a)
     __shared__ int where[kRowMax][2];   // page (-1: none) and token within it
     grid_dependency_wait();
     grid_dependency_launch();
-    const int first = blockIdx.x * a.rows_per_block, rows = min(a.rows_per_block, a.batch.rows - first);
+    const int first = blockIdx.x * a.rows_per_block, rows = min(a.rows_per_block, a.batch.rows - first);   // of a block that has some
+    // Starts out of order may leave sequences that no row leads to: blocks behind the rows' look at all of them.
+    if (blockIdx.x >= a.row_blocks) {
+        const long long from = static_cast<long long>(blockIdx.x - a.row_blocks) * kCheckedStarts;
+        for (long long s = from + threadIdx.x; s < min(from + kCheckedStarts, static_cast<long long>(a.batch.sequences)); s += blockDim.x) {
+            const int begin = a.batch.row_starts[s], end = a.batch.row_starts[s + 1];
+            if (begin < 0 || end < begin || end > a.batch.rows) report_bad(a.batch.status);
+        }
+        return;
+    }
     const int per = 1 << a.lanes_log2, heads = a.pages.kv_heads, dim = a.pages.dim, all_columns = 2 * heads << a.lanes_log2;
     const int row0 = threadIdx.x / a.columns, column0 = threadIdx.x - row0 * a.columns, step = blockDim.x / a.columns;
     // a thread per row: the loads of a look-up depend on one another, so the rows' chains run side by side

@@ -262,3 +262,29 @@ def test_a_page_that_is_none_brings_in_no_other(backend, dtype, kind, count, pag
         got.append((out.clone(), sums.clone()))
     for a, b in zip(*got):
         assert torch.isfinite(b[:c.rows].float()).all() and torch.equal(a, b)
+
+
+STARTS = [[0, 10, 5, 8], [0, 5, 3, 3], [-3, 2, 4, 8], [0, 4, 8, 13], [8, 8, 4, 2], [0, 2**31 - 1, 5, 8], [12, 0, 0, 0], [0, 0, -1, 0]]
+
+
+@pytest.mark.parametrize("starts", STARTS)
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+def test_starts_out_of_order_are_reported(backend, starts, kind):
+    """By every call, whichever rows they leave to no sequence."""
+    import gpt_b200
+    c = Cache(kind, [20, 30, 40], [4, 4, 4], 2, 64, 16, seed=2).cuda()
+    c.starts.copy_(torch.tensor(starts, dtype=torch.int32))
+    x, _ = rows_in(c.rows, 128, "bf16", 0, 8)
+    q, _ = rows_in(c.rows, 256, "bf16", 0, 8)
+    out = torch.empty_like(q)
+    k, v = torch.empty_like(x), torch.empty_like(x)
+    for call in (lambda: backend.kv_pages_write(c.pages, c.batch, x, 128, x, 128, 0), lambda: backend.kv_pages_read(k, 128, v, 128, 0, c.pages, c.batch),
+                 lambda: backend.attention_paged(out, 256, None, q, 256, 0, 4, c.pages, c.batch, 0.125)):
+        call()
+        with pytest.raises(gpt_b200.GptB200Error) as e:
+            backend.synchronize()
+        assert e.value.status == 1
+        backend.synchronize()      # once
+    c.starts.copy_(c.starts_cpu)
+    backend.kv_pages_write(c.pages, c.batch, x, 128, x, 128, 0)
+    backend.synchronize()
