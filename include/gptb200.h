@@ -290,7 +290,8 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *           memory: that part of the results is undefined and the next gptb200_ctx_synchronize returns GPTB200_ERR_INVALID_ARG.
  *   kv_pages_write   k and v [rows][kv_heads * dim] in dtype (gptb200_dtype), pitches in elements, into their places.  e4m3: the power of two of a token's head is the
  *           smallest whose 448-fold reaches its largest finite value (between 2^-117 and 2^119: beyond, values saturate or vanish), codes are
- *           rounded to nearest even; infinities and NaN become NaN.  A place that two rows of a call share holds either.
+ *           rounded to nearest even; infinities and NaN become NaN.  What a place that two rows of a call share holds is undefined:
+ *           pieces of both, codes of one beside the power of two of the other.
  *   kv_pages_read    the same rows' values out of the pages: k and v are written.  With row counts equal to the lengths, whole sequences.
  *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
  *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
