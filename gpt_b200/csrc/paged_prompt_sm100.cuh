@@ -130,8 +130,14 @@ __device__ __forceinline__ float rcp_fast(float x)
 using tok::pair;
 using tok::tanh_inner2;
 using tok::unpair;
-// cap * tanh(x), x the score over the cap: cap - 2 cap / (1 + exp(2 x))
-__device__ __forceinline__ float capped(float x, float cap) { return fmaf(-2.0f * cap, rcp_fast(1.0f + tok::exp2_fast(x * 2.8853900817779268f)), cap); }
+// tanh(x) of two values of any size: 1 - 2 / (1 + exp(2 x)), which is off by a share of 1, not of x, so that the polynomial stands up to 1
+__device__ __forceinline__ unsigned long long tanh2(float x, float y)
+{
+    auto beyond = [](float v) { return fmaf(-2.0f, rcp_fast(1.0f + tok::exp2_fast(v * 2.8853900817779268f)), 1.0f); };
+    float u, v;
+    unpair(tanh_inner2(pair(x, y)), u, v);
+    return pair(fabsf(x) <= 1.0f ? u : beyond(x), fabsf(y) <= 1.0f ? v : beyond(y));
+}
 // Eight codes as bf16 values times a power of two.  A code's bits in a bf16's place (exponent and mantissa side by side) stand for code * 2^-120, subnormal
 // ones among them; one product by 2^(120 + e) puts them right, exactly, for e up to 7 (values up to 57344).
 __device__ __forceinline__ uint32_t bf16_mul(uint32_t a, uint32_t b)
@@ -625,7 +631,12 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                             pro::tmem_ld_32x16(s_addr + 16 * c, y);
                             ptx::tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) y[i] = __float_as_uint(pro::capped(__uint_as_float(y[i]) * args.cap_arg, args.cap_log2));
+                            for (int i = 0; i < 16; i += 2) {
+                                float u, v;
+                                pro::unpair(ptx::mul2(pro::tanh2(__uint_as_float(y[i]) * args.cap_arg, __uint_as_float(y[i + 1]) * args.cap_arg), ptx::both(args.cap_log2)), u, v);
+                                y[i] = __float_as_uint(u);
+                                y[i + 1] = __float_as_uint(v);
+                            }
                             pro::tmem_st_32x16(s_addr + 16 * c, y);
                         }
                         pro::tmem_st_wait();

@@ -181,3 +181,18 @@ def test_queries_and_keys_of_any_size(backend, kind, power):
     out, sums = attend(backend, c, q, share, "bf16", dim ** -0.5)
     backend.synchronize()
     check(c, q, out, sums, share, "bf16", dim ** -0.5)
+
+
+@pytest.mark.parametrize("dtype,kind", KINDS)
+@pytest.mark.parametrize("count,share", [(4, 2), (64, 1), (300, 4)])
+@pytest.mark.parametrize("cap", [20.0, 2.0 ** 10, 2.0 ** 17])
+def test_scores_far_below_the_cap_beside_those_beyond_it(backend, dtype, kind, count, share, cap):
+    """Every third row's scores are many times the cap; the others' are ordinary ones, and as exact as without those."""
+    length, dim, g = count + 200, 64, torch.Generator().manual_seed(5)
+    c = held(kind, torch.randn(length, 1, dim, generator=g, dtype=torch.float64), torch.randn(length, 1, dim, generator=g, dtype=torch.float64), counts=(count,))
+    x = torch.randn(count, share * dim, generator=g)
+    x[::3] *= 8.0 * cap
+    q = x.to(TYPES[dtype]).cuda()
+    out, sums = attend(backend, c, q, share, dtype, dim ** -0.5, cap)
+    backend.synchronize()
+    check(c, q, out, sums, share, dtype, dim ** -0.5, cap)
