@@ -11,6 +11,8 @@ using namespace gptb200;
 
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // The device that is current at the call stays so.
@@ -137,6 +139,9 @@ int check_attention(gptb200_ctx *ctx, int dtype, int heads, const gptb200_kv_pag
     if (heads <= 0 || heads % pages->kv_heads) return fail(ctx, GPTB200_ERR_INVALID_ARG, "%d heads are not a multiple of the cache's %d", heads, pages->kv_heads);
     if (!(scale > 0.0f) || !std::isfinite(scale) || !(cap >= 0.0f) || !std::isfinite(cap) || window < 0 || sinks < 0)
         return fail(ctx, GPTB200_ERR_INVALID_ARG, "scale %g, cap %g, window %d, first tokens %d", scale, cap, window, sinks);
+    // the kernels' factors: scores in base 2, scores over the cap
+    if (!std::isfinite(scale * kLog2e) || (cap > 0.0f && (!std::isfinite(cap * kLog2e) || !std::isnormal(scale / cap))))
+        return fail(ctx, GPTB200_ERR_INVALID_ARG, "scale %g and cap %g, or their quotient, leave the range of fp32", scale, cap);
     if (1LL * heads * pages->dim > INT_MAX / 64 || 1LL * rows->rows * heads > INT_MAX - 256)
         return fail(ctx, GPTB200_ERR_TOO_LARGE, "%d rows of %lld elements", rows->rows, 1LL * heads * pages->dim);
     a->heads = heads;
@@ -221,7 +226,6 @@ int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args, bool codes)
 
 int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
 {
-    constexpr float kLog2e = 1.4426950408889634f;
     const bool codes = kind == GPTB200_KV_E4M3;
     kvp::PromptArgs args{};
     args.a = a;

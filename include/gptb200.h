@@ -294,7 +294,8 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *           pieces of both, codes of one beside the power of two of the other.
  *   kv_pages_read    the same rows' values out of the pages: k and v are written.  With row counts equal to the lengths, whole sequences.
  *   attention_paged  out[row][h] = sum_j p_j v_j over the keys j that the row at position t sees: j <= t and, where window > 0, also t - j < window or j < sinks.
- *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap).  Query head h reads key / value head h / (heads / kv_heads).
+ *           p = softmax(f(scale * q . k_j)), f(x) = x or, where cap > 0, cap * tanh(x / cap);
+ *           scale and cap times log2(e) are finite in fp32, scale / cap is a normal number.  Query head h reads key / value head h / (heads / kv_heads).
  *           lse (may be NULL): fp32 [rows][heads], the logarithm of the sum of exp(f(scale * q . k_j)).  q and out [rows][heads * dim] in dtype; they share no
  *           element.  Scores, sums and outputs are formed in fp32 from the values that the pages hold.  Weights multiply values as fp32 where queries or pages are
  *           fp32; else (gptb200_plan_attention_paged says which) in two 16-bit terms for few rows, off by 2^-16 of themselves at most, and rounded to bf16 once for prompts, off
