@@ -249,20 +249,59 @@ def _ptr(t: Any) -> int | None:
     return int(t.data_ptr())
 
 
+def _pinned(t: Any) -> bool:
+    """Page-locked host memory, which kernels read as well."""
+    try:
+        return bool(t.is_pinned())
+    except RuntimeError:   # torch finds no device
+        return False
+
+
+def _check_tensor(name: str, t: Any, dtypes: tuple, elements: int, itemsize: int, rows: bool = False) -> None:
+    """Raises where a torch tensor is not `elements` elements (of `itemsize` bytes) of one of the types side by side in device memory; addresses are taken as they are.
+    rows: the last dimension alone has to be contiguous, and the elements are those up to the last row's first."""
+    if t is None or isinstance(t, int) or not hasattr(t, "untyped_storage"):
+        return
+    kind = str(t.dtype).removeprefix("torch.")
+    if kind not in dtypes:
+        raise ValueError(f"{name} is a tensor of {kind}, not of {' or '.join(dtypes)}")
+    if not (t.is_cuda or _pinned(t)):
+        raise ValueError(f"{name} is not in device memory")
+    if not (t.is_contiguous() or (rows and t.dim() > 0 and t.stride(-1) == 1)):
+        raise ValueError(f"{name} is not contiguous")
+    held = t.untyped_storage().nbytes() - t.storage_offset() * t.element_size() if rows else t.numel() * t.element_size()
+    if held < elements * itemsize:
+        raise ValueError(f"{name} holds {held} bytes where {elements * itemsize} are described")
+
+
+_KV_TYPES = {KV_BF16: (("bfloat16", "uint8"), 2), KV_F32: (("float32", "uint8"), 4), KV_E4M3: (("float8_e4m3fn", "uint8", "int8"), 1)}   # of a pool's tensor, or its bytes
+
+
 class KvPages:
     """A layer's pool of a paged cache of keys and values (gptb200_kv_pages in include/gptb200.h): data [num_pages][2][kv_heads][page_tokens][dim], for
-    KV_E4M3 scales [num_pages][2][kv_heads][page_tokens].  Keeps what it is given alive; calls take it as often as they like."""
+    KV_E4M3 scales [num_pages][2][kv_heads][page_tokens].  Keeps what it is given alive; calls take it as often as they like.  Raises ValueError where a tensor's type, size,
+    layout or place is not the one described."""
 
     def __init__(self, data, scales, kind: int, num_pages: int, page_tokens: int, kv_heads: int, dim: int):
+        if kind in _KV_TYPES:
+            types, itemsize = _KV_TYPES[kind]
+            _check_tensor("data", data, types, num_pages * 2 * kv_heads * page_tokens * dim, itemsize)
+            if kind == KV_E4M3:
+                _check_tensor("scales", scales, ("uint8", "int8"), num_pages * 2 * kv_heads * page_tokens, 1)
         self._tensors = (data, scales)
         self.struct = _KvPages(_ptr(data), _ptr(scales), kind, num_pages, page_tokens, kv_heads, dim)
 
 
 class KvRows:
     """The new rows of a call on a paged cache (gptb200_kv_rows in include/gptb200.h): int32 device arrays row_starts [sequences + 1], lengths [sequences] and
-    page_table [sequences][table_pitch], the tensors' rows and the most new rows of a sequence.  Keeps the arrays alive; their contents may change between calls."""
+    page_table [sequences][table_pitch], the tensors' rows and the most new rows of a sequence.  Keeps the arrays alive; their contents may change between calls.  Raises
+    ValueError where a tensor's type, size, layout or place is not the one described."""
 
     def __init__(self, row_starts, lengths, page_table, sequences: int, table_pitch: int, rows: int, max_new: int):
+        if sequences > 0:
+            _check_tensor("row_starts", row_starts, ("int32",), sequences + 1, 4)
+            _check_tensor("lengths", lengths, ("int32",), sequences, 4)
+            _check_tensor("page_table", page_table, ("int32",), (sequences - 1) * table_pitch + 1 if table_pitch > 0 else 0, 4, rows=True)
         self._tensors = (row_starts, lengths, page_table)
         self.struct = _KvRows(_ptr(row_starts), _ptr(lengths), _ptr(page_table), sequences, table_pitch, rows, max_new)
 
