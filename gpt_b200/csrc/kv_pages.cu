@@ -15,6 +15,8 @@ constexpr float kLog2e = 1.4426950408889634f;
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
+bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
 // The device that is current at the call stays so.
 struct OnDevice {
     int before = -1;
@@ -48,6 +50,7 @@ int check_pages(gptb200_ctx *ctx, const gptb200_kv_pages *p, const gptb200_kv_ro
         if (!p->data || !aligned16(p->data) || (p->kind == GPTB200_KV_E4M3 && (!p->scales || !aligned16(p->scales))))
             return fail(ctx, GPTB200_ERR_INVALID_ARG, "pages: no memory, or not aligned to 16 bytes");
         if (!b->row_starts || !b->lengths || (!b->page_table && b->table_pitch > 0)) return fail(ctx, GPTB200_ERR_INVALID_ARG, "rows: no starts, lengths or page table");
+        if (!aligned4(b->row_starts) || !aligned4(b->lengths) || !aligned4(b->page_table)) return fail(ctx, GPTB200_ERR_INVALID_ARG, "rows: an array of int32 is not aligned to 4 bytes");
     }
     int shift = 0;
     while ((1 << shift) < p->page_tokens) ++shift;
@@ -266,6 +269,7 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     if (rows->sequences == 0 || rows->rows == 0) return GPTB200_OK;
     const long long width = 1LL * heads * pages->dim;
     if ((rc = check_rows(ctx, "q", q, q_pitch, width, dtype)) != GPTB200_OK || (rc = check_rows(ctx, "out", out, out_pitch, width, dtype)) != GPTB200_OK) return rc;
+    if (!aligned4(lse)) return fail(ctx, GPTB200_ERR_INVALID_ARG, "lse is not aligned to 4 bytes");
     if (out == q) return fail(ctx, GPTB200_ERR_INVALID_ARG, "out is q");
     OnDevice device;
     CUDA_TRY(ctx, device.enter(ctx->device));

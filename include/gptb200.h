@@ -302,7 +302,7 @@ int gptb200_advance_position(gptb200_ctx *ctx, int *pos_dev);
  *           by 2^-8 of themselves, where the sum that divides is that of the rounded ones.  Few rows over codes: a key whose weight times its value's power of two is below
  *           2^-36 of the row's largest adds nothing to out, nor does an element of q below 2^-40 of its head's largest to a score.
  *           The order of sums, and so the last bits of a row, depend on the lengths of all sequences of the call.
- *   All addresses are 16-byte aligned, pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
+ *   Addresses of the pool and of k, v, q and out are 16-byte aligned (the int32 arrays' and lse's 4-byte aligned), pitches multiples of 16 bytes.  Scratch is the context's: calls of one context, captured ones too, run one after the
  *   other. */
 typedef enum gptb200_dtype { GPTB200_DTYPE_BF16 = 0, GPTB200_DTYPE_F32 = 1 } gptb200_dtype;
 typedef enum gptb200_kv_kind { GPTB200_KV_BF16 = 0, GPTB200_KV_F32 = 1, GPTB200_KV_E4M3 = 2 } gptb200_kv_kind;

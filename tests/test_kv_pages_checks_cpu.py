@@ -100,3 +100,14 @@ def test_pools_with_gaps_short_scales_or_on_the_host():
         pool(scales=device(5, 2, 3, 16, dtype=torch.float32))
     with pytest.raises(ValueError, match="device memory"):
         pool(data=torch.zeros(5, 2, 3, 16, 64, dtype=torch.uint8))
+
+
+@pytest.mark.parametrize("name", ["starts", "lengths", "table"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_arrays_at_odd_addresses(built_library, name, off):
+    """A load of four bytes from there would fault."""
+    import gpt_b200
+    with pytest.raises(gpt_b200.GptB200Error) as e:
+        plan(r=rows(**{name: 0x3000 + off}))
+    assert e.value.status == 1
+    assert plan(r=rows(**{name: 0x3004}))["kernel"] == "tokens"

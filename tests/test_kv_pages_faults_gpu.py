@@ -288,3 +288,17 @@ def test_starts_out_of_order_are_reported(backend, starts, kind):
     c.starts.copy_(c.starts_cpu)
     backend.kv_pages_write(c.pages, c.batch, x, 128, x, 128, 0)
     backend.synchronize()
+
+
+def test_sums_at_an_odd_address_are_refused(backend):
+    import gpt_b200
+    c = Cache("bf16", [20], [2], 2, 64, 16).cuda()
+    q, out = torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda"), torch.zeros(2, 256, dtype=torch.bfloat16, device="cuda")
+    sums = torch.zeros(16, device="cuda")
+    n = backend.launch_count()
+    for off in (1, 2, 3):
+        with pytest.raises(gpt_b200.GptB200Error) as e:
+            backend.attention_paged(out, 256, sums.data_ptr() + off, q, 256, 0, 4, c.pages, c.batch, 0.1)
+        assert e.value.status == 1 and backend.launch_count() == n
+    backend.attention_paged(out, 256, sums.data_ptr() + 4, q, 256, 0, 4, c.pages, c.batch, 0.1)
+    backend.synchronize()
