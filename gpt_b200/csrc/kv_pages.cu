@@ -110,7 +110,11 @@ int run_rows(gptb200_ctx *ctx, void *k, long long k_pitch, void *v, long long v_
 // Which kernel attends, and how its grid is made; host logic.
 struct PagedPlan {
     int kernel;       // 0: nothing to do, 1 few rows on mma.sync, 2 prompts on tcgen05, 3 / 4 single / 16 or 32 rows on FMAs
-    int tile_rows, per_sm, part_floats;
+    int tile_rows, per_sm, most_blocks, part_floats;
+
+    // of the grid: per_sm on every SM, as far as the kernel has room for the parts of a tile
+    int blocks(int sms) const { return static_cast<int>(std::min<long long>(1LL * sms * per_sm, most_blocks)); }
+    size_t scratch(int sms) const { return size_t(2) * blocks(sms) * part_floats * sizeof(float); }
 };
 enum { PAGED_NONE = 0, PAGED_TOKENS = 1, PAGED_PROMPT = 2, PAGED_FEW = 3, PAGED_ROWS = 4 };
 
@@ -121,17 +125,17 @@ PagedPlan plan_paged(int dtype, int kind, long long max_rows, long long all_rows
     if (dtype == GPTB200_DTYPE_F32 || kind == GPTB200_KV_F32) {
         // a row at a time: 4 sequences of 1024, 12 heads of 64, 2 / 4 / 8 rows a head: 21 / 21 / 28 us, 32 of 4096, 8 heads of 128, 4 / 8 / 16 rows: 396 / 373 / 671 us;
         // sixteen at a time 26 / 27 / 30 us and 394 / 364 / 453 us
-        if (max_rows <= 8) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kTokensPart};
+        if (max_rows <= 8) return {PAGED_FEW, 1, kvp::kFewPerSm, kvp::kFewBlocks, kvp::kTokensPart};
         // four or eight rows a warp, in us, 16 sequences of 2048: 10 / 32 rows a head 36 / 48 against 46 / 54, 64 / 128 rows (3016 / 5488 in all) 99 / 169 against 89 / 142;
         // 2000 rows 909 against 663; but with 2124 in all, 100 a head at most, 32 against 43: too few tiles
         const int each = max_rows > 32 && all_rows >= 2560 ? 8 : 4;
-        return {PAGED_ROWS, kvp::rows_tile(each), kvp::kRowsPerSm, kvp::rows_part(each)};
+        return {PAGED_ROWS, kvp::rows_tile(each), kvp::kRowsPerSm, kvp::kRowsBlocks, kvp::rows_part(each)};
     }
     // 16 sequences of 4096, 8 heads of 128, in us: bf16, 32 / 40 / 48 rows a head: streamed 64 / 69 / 78, prompt 67 / 68 / 63; e4m3, 64 / 96 rows: 109 / 142 against 151 / 148
     // (with 2 sequences, 64 rows: 27 against 40 and 31 against 53)
-    if (max_rows > (codes ? 96 : 40)) return {PAGED_PROMPT, kvp::kPromptRows, 1, kvp::kPromptPart};
+    if (max_rows > (codes ? 96 : 40)) return {PAGED_PROMPT, kvp::kPromptRows, 1, kPagedTickets / 2, kvp::kPromptPart};
     // tiles of eight or sixteen rows: bf16, 12 / 16 rows: 46 / 55 against 49 / 50; e4m3, 16 / 32 rows: 47 / 72 against 48 / 65
-    return {PAGED_TOKENS, max_rows <= (codes ? 16 : 12) ? 8 : 16, codes ? 3 : 2, kvp::kTokensPart};
+    return {PAGED_TOKENS, max_rows <= (codes ? 16 : 12) ? 8 : 16, kvp::tokens_per_sm(codes), kvp::tokens_blocks(codes), kvp::kTokensPart};
 }
 
 int check_attention(gptb200_ctx *ctx, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks, kvp::Attention *a)
@@ -157,9 +161,11 @@ int check_attention(gptb200_ctx *ctx, int dtype, int heads, const gptb200_kv_pag
     return GPTB200_OK;
 }
 
-// A kernel that cuts the line of work into equal ranges: `per_sm` blocks on every SM, a part of a tile in scratch for either end of a range.
+static_assert(kvp::kFewBlocks <= kPagedTickets && kvp::kRowsBlocks <= kPagedTickets && kvp::tokens_blocks(true) <= kPagedTickets && kvp::tokens_blocks(false) <= kPagedTickets);
+
+// A kernel that cuts the line of work into equal ranges, a part of a tile in scratch for either end of a range.
 template <typename Args>
-int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, int smem, int per_sm, int most_blocks, int part_floats)
+int run_line(gptb200_ctx *ctx, const PagedPlan &plan, void (*kernel)(Args), Args &args, int threads, int smem)
 {
     const void *key = reinterpret_cast<const void *>(kernel);
     if (!ctx->configured.count(key)) {
@@ -167,72 +173,70 @@ int run_line(gptb200_ctx *ctx, void (*kernel)(Args), Args &args, int threads, in
         ctx->configured.insert(key);
     }
     const int sms = ctx->max_sms > 0 ? std::min(ctx->max_sms, ctx->num_sms) : ctx->num_sms;
-    const int blocks = std::min(sms * per_sm, most_blocks);
-    const int rc = ensure_workspace(ctx, size_t(2) * blocks * part_floats * sizeof(float));
+    const int rc = ensure_workspace(ctx, plan.scratch(sms));
     if (rc != GPTB200_OK) return rc;
-    args.parts = {ctx->ws, ctx->d_paged_tickets, part_floats};
-    CUDA_TRY(ctx, launch_chained(ctx, kernel, dim3(blocks), dim3(threads), smem, args));
+    args.parts = {ctx->ws, ctx->d_paged_tickets, plan.part_floats};
+    args.cut.tile_rows = plan.tile_rows;
+    CUDA_TRY(ctx, launch_chained(ctx, kernel, dim3(plan.blocks(sms)), dim3(threads), smem, args));
     ctx->launches++;
     return GPTB200_OK;
 }
 
 template <int D16, bool CODES, int NT>
-int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args)
+int run_tokens(gptb200_ctx *ctx, const PagedPlan &plan, kvp::TokensArgs &args)
 {
-    using S = kvp::TokensShape<D16, CODES, NT>;
-    args.cut.tile_rows = S::kRows;
-    return run_line(ctx, kvp::paged_tokens_kernel<D16, CODES, NT>, args, kvp::kTokensThreads, S::kSmem, S::kPerSm, std::min(S::kMaxBlocks, kPagedTickets), kvp::kTokensPart);
+    return run_line(ctx, plan, kvp::paged_tokens_kernel<D16, CODES, NT>, args, kvp::kTokensThreads, kvp::TokensShape<D16, CODES, NT>::kSmem);
 }
 
 template <int D16>
-int run_tokens(gptb200_ctx *ctx, kvp::TokensArgs &args, bool codes, bool few)
+int run_tokens(gptb200_ctx *ctx, const PagedPlan &plan, kvp::TokensArgs &args, bool codes)
 {
-    if (codes) return few ? run_tokens<D16, true, 1>(ctx, args) : run_tokens<D16, true, 2>(ctx, args);
-    return few ? run_tokens<D16, false, 1>(ctx, args) : run_tokens<D16, false, 2>(ctx, args);
+    if (codes) return plan.tile_rows == 8 ? run_tokens<D16, true, 1>(ctx, plan, args) : run_tokens<D16, true, 2>(ctx, plan, args);
+    return plan.tile_rows == 8 ? run_tokens<D16, false, 1>(ctx, plan, args) : run_tokens<D16, false, 2>(ctx, plan, args);
 }
 
-int attention_tokens(gptb200_ctx *ctx, const kvp::Attention &a, int kind, bool few)
+int attention_tokens(gptb200_ctx *ctx, const PagedPlan &plan, const kvp::Attention &a, int kind)
 {
     kvp::TokensArgs args{a, {}, {0, kvp::kTokensKeys, 1, 5}};
     const bool codes = kind == GPTB200_KV_E4M3;
     switch ((a.pages.dim + 31) / 32) {
-        case 1: return run_tokens<2>(ctx, args, codes, few);
-        case 2: return run_tokens<4>(ctx, args, codes, few);
-        case 3: return run_tokens<6>(ctx, args, codes, few);
-        default: return run_tokens<8>(ctx, args, codes, few);
+        case 1: return run_tokens<2>(ctx, plan, args, codes);
+        case 2: return run_tokens<4>(ctx, plan, args, codes);
+        case 3: return run_tokens<6>(ctx, plan, args, codes);
+        default: return run_tokens<8>(ctx, plan, args, codes);
     }
 }
 
 template <typename T, int KIND>
-int run_fma(gptb200_ctx *ctx, const kvp::Attention &a, const PagedPlan &plan)
+int run_fma(gptb200_ctx *ctx, const PagedPlan &plan, const kvp::Attention &a)
 {
-    kvp::TokensArgs args{a, {}, {plan.tile_rows, kvp::kFewKeys, 1, 5}};
-    if (plan.kernel == PAGED_FEW) return run_line(ctx, kvp::paged_few_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::kFewSmem, plan.per_sm, kvp::kFewBlocks, plan.part_floats);
+    kvp::TokensArgs args{a, {}, {0, kvp::kFewKeys, 1, 5}};
+    if (plan.kernel == PAGED_FEW) return run_line(ctx, plan, kvp::paged_few_kernel<T, KIND>, args, kvp::kTokensThreads, kvp::kFewSmem);
     args.cut.keys = kvp::kRowsKeys;
-    return plan.tile_rows == kvp::rows_tile(4) ? run_line(ctx, kvp::paged_rows_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::rows_smem(4), plan.per_sm, kvp::kRowsBlocks, plan.part_floats)
-                                               : run_line(ctx, kvp::paged_rows_kernel<T, KIND, 8>, args, kvp::kTokensThreads, kvp::rows_smem(8), plan.per_sm, kvp::kRowsBlocks, plan.part_floats);
+    return plan.tile_rows == kvp::rows_tile(4) ? run_line(ctx, plan, kvp::paged_rows_kernel<T, KIND, 4>, args, kvp::kTokensThreads, kvp::rows_smem(4))
+                                               : run_line(ctx, plan, kvp::paged_rows_kernel<T, KIND, 8>, args, kvp::kTokensThreads, kvp::rows_smem(8));
 }
 
 template <int NB, bool CODES, bool CAPPED>
-int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args)
+int run_prompt(gptb200_ctx *ctx, const PagedPlan &plan, kvp::PromptArgs &args)
 {
-    return run_line(ctx, args.a.lse ? kvp::paged_prompt_kernel<NB, CODES, CAPPED, true> : kvp::paged_prompt_kernel<NB, CODES, CAPPED, false>, args, kvp::kPromptThreads,
-                    kvp::PromptShape<NB>::kSmem, 1, kPagedTickets / 2, kvp::kPromptPart);
+    return run_line(ctx, plan, args.a.lse ? kvp::paged_prompt_kernel<NB, CODES, CAPPED, true> : kvp::paged_prompt_kernel<NB, CODES, CAPPED, false>, args, kvp::kPromptThreads,
+                    kvp::PromptShape<NB>::kSmem);
 }
 
 template <int NB>
-int run_prompt(gptb200_ctx *ctx, kvp::PromptArgs &args, bool codes)
+int run_prompt(gptb200_ctx *ctx, const PagedPlan &plan, kvp::PromptArgs &args, bool codes)
 {
-    if (args.a.cap > 0.0f) return codes ? run_prompt<NB, true, true>(ctx, args) : run_prompt<NB, false, true>(ctx, args);
-    return codes ? run_prompt<NB, true, false>(ctx, args) : run_prompt<NB, false, false>(ctx, args);
+    if (args.a.cap > 0.0f) return codes ? run_prompt<NB, true, true>(ctx, plan, args) : run_prompt<NB, false, true>(ctx, plan, args);
+    return codes ? run_prompt<NB, true, false>(ctx, plan, args) : run_prompt<NB, false, false>(ctx, plan, args);
 }
 
-int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
+int attention_prompt(gptb200_ctx *ctx, const PagedPlan &plan, const kvp::Attention &a, int kind)
 {
     const bool codes = kind == GPTB200_KV_E4M3;
     kvp::PromptArgs args{};
     args.a = a;
-    args.cut = {kvp::kPromptRows, kvp::kPromptKeys, 2, 4};
+    args.cut = {0, kvp::kPromptKeys, 2, 4};
     args.scale_log2 = a.scale * kLog2e;
     args.cap_log2 = a.cap * kLog2e;
     args.cap_arg = a.cap > 0.0f ? a.scale / a.cap : 0.0f;
@@ -242,7 +246,7 @@ int attention_prompt(gptb200_ctx *ctx, const kvp::Attention &a, int kind)
         const int rc = bf16_operand_map(ctx, &args.map, a.pages.data, rows, a.pages.dim, a.pages.dim, args.box_rows);
         if (rc != GPTB200_OK) return rc;
     }
-    return a.pages.dim <= 64 ? run_prompt<1>(ctx, args, codes) : run_prompt<2>(ctx, args, codes);
+    return a.pages.dim <= 64 ? run_prompt<1>(ctx, plan, args, codes) : run_prompt<2>(ctx, plan, args, codes);
 }
 
 }  // namespace
@@ -275,11 +279,11 @@ int gptb200_attention_paged(gptb200_ctx *ctx, void *out, long long out_pitch, fl
     CUDA_TRY(ctx, device.enter(ctx->device));
     a.q = q; a.out = out; a.lse = lse; a.q_pitch = q_pitch; a.out_pitch = out_pitch;
     const PagedPlan plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share, 1LL * rows->rows * a.heads);
-    if (plan.kernel == PAGED_PROMPT) return attention_prompt(ctx, a, pages->kind);
-    if (plan.kernel == PAGED_TOKENS) return attention_tokens(ctx, a, pages->kind, plan.tile_rows == 8);
-    if (dtype == GPTB200_DTYPE_BF16) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, a, plan);
-    return pages->kind == GPTB200_KV_E4M3 ? run_fma<float, kvp::KIND_E4M3>(ctx, a, plan)
-           : pages->kind == GPTB200_KV_F32 ? run_fma<float, kvp::KIND_F32>(ctx, a, plan) : run_fma<float, kvp::KIND_BF16>(ctx, a, plan);
+    if (plan.kernel == PAGED_PROMPT) return attention_prompt(ctx, plan, a, pages->kind);
+    if (plan.kernel == PAGED_TOKENS) return attention_tokens(ctx, plan, a, pages->kind);
+    if (dtype == GPTB200_DTYPE_BF16) return run_fma<__nv_bfloat16, kvp::KIND_F32>(ctx, plan, a);
+    return pages->kind == GPTB200_KV_E4M3 ? run_fma<float, kvp::KIND_E4M3>(ctx, plan, a)
+           : pages->kind == GPTB200_KV_F32 ? run_fma<float, kvp::KIND_F32>(ctx, plan, a) : run_fma<float, kvp::KIND_BF16>(ctx, plan, a);
 }
 
 int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb200_kv_pages *pages, const gptb200_kv_rows *rows, float scale, float cap, int window, int sinks, int *plan4)
@@ -290,8 +294,7 @@ int gptb200_plan_attention_paged(int num_sms, int dtype, int heads, const gptb20
     if (rc != GPTB200_OK) return rc;
     PagedPlan plan{};
     if (rows->sequences > 0 && rows->rows > 0) plan = plan_paged(dtype, pages->kind, 1LL * rows->max_new * a.share, 1LL * rows->rows * a.heads);
-    const int blocks = num_sms * plan.per_sm;
-    const int out[4] = {plan.kernel, plan.tile_rows, blocks, static_cast<int>((2LL * blocks * plan.part_floats * sizeof(float)) >> 10)};
+    const int out[4] = {plan.kernel, plan.tile_rows, plan.blocks(num_sms), static_cast<int>(plan.scratch(num_sms) >> 10)};
     for (int i = 0; i < 4; ++i) plan4[i] = out[i];
     return GPTB200_OK;
 }

@@ -30,6 +30,9 @@ constexpr int kTokensWarps = 4, kTokensThreads = kTokensWarps * 32;
 constexpr int kTokensMaxRows = 16, kTokensKeys = 64;
 constexpr int kTokensPart = kTokensMaxRows * 128 + 2 * kTokensMaxRows;   // floats of a part in scratch
 
+__host__ __device__ constexpr int tokens_per_sm(bool codes) { return codes ? 3 : 2; }              // blocks on an SM
+__host__ __device__ constexpr int tokens_blocks(bool codes) { return tokens_per_sm(codes) * 160; }   // of a grid, at most: so many parts' sums have room in shared memory
+
 // D16: dimensions in steps of 16 (zeros behind the head's own)
 template <int D16, bool CODES, int NT>
 struct TokensShape {
@@ -40,15 +43,14 @@ struct TokensShape {
     static constexpr int kKeyPitch = CODES ? (D16 == 8 ? 144 : 16 * D16) : 2 * kDim + 16;
     static constexpr int kValuePitch = CODES ? (D16 == 8 ? 144 : D16 == 6 ? 112 : D16 == 4 ? 80 : 48) : 2 * kDim + 16;
     static constexpr int kStage = 16 * (kKeyPitch + kValuePitch) + (CODES ? 32 : 0);
-        static constexpr int kStages = NT == 1 && !CODES ? 2 : 3;
+    static constexpr int kStages = NT == 1 && !CODES ? 2 : 3;
     static constexpr int kRows = 8 * NT;
-    static constexpr int kPerSm = CODES ? 3 : 2;   // blocks on an SM
     static constexpr int kQPitch = 2 * kDim + 16;
     static constexpr int kRing = kTokensWarps * kStages * kStage;
     static constexpr int kMergePitch = kDim + 4;
     static constexpr int kMerge = kTokensWarps * kRows * kMergePitch * 4;
-    static constexpr int kSmem = kRows * kQPitch + (kRing > kMerge ? kRing : kMerge), kMaxBlocks = kPerSm * 160;
-    static_assert((kSmem - kRows * kQPitch) / 8 >= kMaxBlocks && kSmem - kRows * kQPitch >= kTokensWarps * kTeamRoom * 4);   // of the grid: a tile's parts, at most
+    static constexpr int kSmem = kRows * kQPitch + (kRing > kMerge ? kRing : kMerge);
+    static_assert((kSmem - kRows * kQPitch) / 8 >= tokens_blocks(CODES) && kSmem - kRows * kQPitch >= kTokensWarps * kTeamRoom * 4);   // of the grid: a tile's parts, at most
 };
 
 namespace tok {
@@ -264,7 +266,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
 }
 
 template <int D16, bool CODES, int NT>
-__global__ void __launch_bounds__(kTokensThreads, TokensShape<D16, CODES, NT>::kPerSm)
+__global__ void __launch_bounds__(kTokensThreads, tokens_per_sm(CODES))
 paged_tokens_kernel(const __grid_constant__ TokensArgs args)
 {
     using namespace tok;

@@ -111,3 +111,16 @@ def test_arrays_at_odd_addresses(built_library, name, off):
         plan(r=rows(**{name: 0x3000 + off}))
     assert e.value.status == 1
     assert plan(r=rows(**{name: 0x3004}))["kernel"] == "tokens"
+
+
+@pytest.mark.parametrize("dtype,kind,max_new,kernel,per_sm,most,part", [
+    (BF16, BF16, 1, "tokens", 2, 320, 16 * 130), (BF16, E4M3, 1, "tokens", 3, 480, 16 * 130), (BF16, BF16, 100, "prompt", 1, 512, 256 * 132), (F32, F32, 1, "few", 3, 480, 16 * 130),
+    (F32, F32, 100, "rows", 3, 480, 16 * 130),
+])
+@pytest.mark.parametrize("sms", [1, 7, 148, 160, 200, 2000, 2**31 - 1])
+def test_plan_on_any_number_of_sms(built_library, dtype, kind, max_new, kernel, per_sm, most, part, sms):
+    """The grid that a call launches, and the scratch for two parts per block: no more blocks than parts of a tile have room for."""
+    import gpt_b200
+    got = gpt_b200.plan_attention_paged(sms, dtype, 4, pages(kind=kind), rows(max_new=max_new), 0.125)
+    blocks = min(sms * per_sm, most)
+    assert got["kernel"] == kernel and got["blocks"] == blocks and got["scratch_kib"] == 2 * blocks * part * 4 >> 10
