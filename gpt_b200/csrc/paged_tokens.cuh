@@ -416,14 +416,16 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
             }
         // a lane's rows: 2 t4 and 2 t4 + 1 of every eight
         int pos[NT][2];
-        float to_score[NT][2], m[NT][2], ref[NT][2], l[NT][2] = {};   // m: what the sums stand against, ref: what the weighted values stand against (codes; else m)
+        float small[NT][2], to_score[NT][2], m[NT][2], ref[NT][2], l[NT][2] = {};   // m: what the sums stand against, ref: what the weighted values stand against (codes; else m)
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = 8 * n + 2 * t4 + e;
                 pos[n][e] = r < rows ? place.q.pos0 + a.shares.divide(packed0 + r) : -1;
-                to_score[n][e] = (a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e) * (CODES ? row_power[r] : 1.0f);   // over the cap, or in base 2
+                const float power = CODES ? row_power[r] : 1.0f;
+                small[n][e] = fminf(power, 1.0f);
+                to_score[n][e] = (a.cap > 0.0f ? a.scale / a.cap : a.scale * kLog2e) * fmaxf(power, 1.0f);   // over the cap, or in base 2
                 m[n][e] = ref[n][e] = -INFINITY;
             }
         const float cap_log2 = a.cap * kLog2e;
@@ -460,9 +462,9 @@ paged_tokens_kernel(const __grid_constant__ TokensArgs args)
                     asm volatile("ld.shared.u8 %0, [%1];" : "=r"(ve[j]) : "r"(et + 16 + g8 + 8 * j));
                     value_e[j] = static_cast<float>(static_cast<int>(ve[j]) - 127);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)   // the row's power first: a large query times a large key's power is beyond fp32 where the score is not
+                    for (int n = 0; n < NT; ++n)   // a small row's power in front of the key's, a large one's behind it: what lies between stays within fp32 where the score does
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) x[n][2 * j + e] = (x[n][2 * j + e] + x2[n][2 * j + e]) * to_score[n][e] * scale_of(ke[j]);
+                        for (int e = 0; e < 2; ++e) x[n][2 * j + e] = (x[n][2 * j + e] + x2[n][2 * j + e]) * small[n][e] * scale_of(ke[j]) * to_score[n][e];
                 }
             } else {
 #pragma unroll

@@ -196,3 +196,16 @@ def test_scores_far_below_the_cap_beside_those_beyond_it(backend, dtype, kind, c
     out, sums = attend(backend, c, q, share, dtype, dim ** -0.5, cap)
     backend.synchronize()
     check(c, q, out, sums, share, dtype, dim ** -0.5, cap)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "e4m3"])
+@pytest.mark.parametrize("query,key", [(2.0 ** 125, 2.0 ** -115), (2.0 ** 120, 2.0 ** -118), (2.0 ** -118, 2.0 ** 115), (2.0 ** -110, 2.0 ** 119)])
+def test_queries_and_keys_at_the_ends_of_the_range(backend, kind, query, key):
+    """Scores of ordinary size: the scale takes what the two leave."""
+    length, dim, share, g = 100, 64, 8, torch.Generator().manual_seed(4)
+    scale = 2.0 ** -3 / (query * key)
+    c = held(kind, torch.randn(length, 1, dim, generator=g, dtype=torch.float64) * key, torch.randn(length, 1, dim, generator=g, dtype=torch.float64))
+    q = (torch.randn(1, share * dim, generator=g).clamp(-1.9, 1.9) * query).to(torch.bfloat16).cuda()
+    out, sums = attend(backend, c, q, share, "bf16", scale)
+    backend.synchronize()
+    check(c, q, out, sums, share, "bf16", scale)
