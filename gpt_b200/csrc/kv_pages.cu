@@ -132,7 +132,7 @@ PagedPlan plan_paged(int dtype, int kind, long long max_rows, long long all_rows
         return {PAGED_ROWS, kvp::rows_tile(each), kvp::kRowsPerSm, kvp::kRowsBlocks, kvp::rows_part(each)};
     }
     // 16 sequences of 4096, 8 heads of 128, in us: bf16, 32 / 40 / 48 rows a head: streamed 64 / 69 / 78, prompt 67 / 68 / 63; e4m3, 64 / 96 rows: 109 / 142 against 151 / 148
-    // (with 2 sequences, 64 rows: 27 against 40 and 31 against 53)
+    // (by rows alone, whatever there is to do: with 2 sequences, 64 rows, the streamed kernel takes 27 against 40 and 31 against 53)
     if (max_rows > (codes ? 96 : 40)) return {PAGED_PROMPT, kvp::kPromptRows, 1, kPagedTickets / 2, kvp::kPromptPart};
     // tiles of eight or sixteen rows: bf16, 12 / 16 rows: 46 / 55 against 49 / 50; e4m3, 16 / 32 rows: 47 / 72 against 48 / 65
     return {PAGED_TOKENS, max_rows <= (codes ? 16 : 12) ? 8 : 16, kvp::tokens_per_sm(codes), kvp::tokens_blocks(codes), kvp::kTokensPart};

@@ -153,8 +153,8 @@ __device__ __forceinline__ int exponent_for(float most)
 constexpr int kRowThreads = 256;
 constexpr int kRowMax = 64;    // rows per block, at most
 constexpr int kCheckedStarts = 1024;   // sequences whose starts a block checks
-// Pieces under way per thread, blocks per SM, rows per thread.  Writing (24 400 rows of 8 heads of 128 from bf16 to codes): 39.5 us with four blocks of four pieces each, 5.1 TB/s;
-// 56 us with rows looked up by a warp each and two blocks.  Reading (16 600 rows of 4 heads back): 25.5 us with eight blocks and one piece, 4.3 TB/s; 33 us with
+// Pieces under way per thread, blocks per SM, rows per thread.  Writing (24 400 rows of 8 heads of 128 from bf16 to codes): 40 us with four blocks of four pieces each, 5.0 TB/s;
+// 56 us with rows looked up by a warp each and two blocks.  Reading (16 600 rows of 4 heads back): 22.7 us with eight blocks and one piece, 4.8 TB/s; 33 us with
 // four pieces each.
 __host__ __device__ constexpr int row_batch(bool write) { return write ? 4 : 1; }
 __host__ __device__ constexpr int row_blocks(bool write) { return write ? 4 : 8; }
@@ -836,7 +836,7 @@ constexpr uint32_t kSeenNan = 0xffu, kSeenInfinities = 0xffff00u;   // a bit per
 template <typename T>
 __device__ __forceinline__ bool not_finite(const Raw8<T> &raw) { return raw.largest() >= 0x7f800000u; }
 template <typename T>
-__device__ __noinline__ uint32_t kinds_of(Raw8<T> raw)   // out of line: what a tile runs through once has to be fetched each time (917 -> 1014 us with twice the code)
+__device__ __noinline__ uint32_t kinds_of(Raw8<T> raw)   // out of line: code that a tile runs through once has to be fetched each time (a prompt of 8192 with a NaN 920 us, 1010 with twice the code)
 {
     uint32_t kinds = 0;
     float v[8];

@@ -16,7 +16,8 @@
 //   warp 4           issues the products, one elected lane
 //   warp 5           walks along the line and hands the others each tile's part of the range through a ring in shared memory
 //   warps 8-11       softmax and output of half 0;  warps 12-15: half 1
-// Keys and values that no row of the tile sees are zeros in shared memory, whatever the pages hold there.  Every wait is bounded.
+// Keys and values that no row of the tile sees are zeros in shared memory, whatever the pages hold there.  Every wait is bounded; its time stands still while a half looks at rows
+// that are not finite (settle_rows), which ends by itself.
 #pragma once
 
 #include "paged_tokens.cuh"
