@@ -829,7 +829,9 @@ __device__ void attention_row(const Attention &a, int s, int position, int row, 
 // Either the row sees a value that makes it so, or the tile's product multiplied one that the row does not see by zero, which is NaN, or sums against an old maximum left
 // fp32's range.  In the first case the result stands: an element that is NaN where the row sees a NaN or infinities of both signs there, one that is infinite where it sees that
 // infinity.  All rows of a tile see nearly the same keys, so a team of warps goes over the values that all of these rows see once, and stops as soon as every element is accounted
-// for; each row then looks at the few others that it sees.  Rows that remain are formed again from their own keys alone.
+// for; each row then looks at the few others that it sees.  A NaN where the row sees one infinity alone becomes that infinity: every weight is positive, though the product may have
+// met one that fp32 does not hold, or a negative second term.  (But a key that is not finite has weight 0, or the weights had no sum; 0 times an infinity is NaN.)  Rows with an element
+// that none of this explains are formed again from their own keys alone.
 
 constexpr uint32_t kSeenNan = 0xffu, kSeenInfinities = 0xffff00u;   // a bit per element: NaN, plus infinity, minus infinity
 
@@ -859,15 +861,15 @@ struct UnsureRows {   // in shared memory
     unsigned int are[16], seen[16];     // kinds by eights of dimensions: among these rows' outputs, among the values that all of them see
 };
 
-// Kinds among the values of keys `from` to `to`, which all rows in question see, by a team's warps in turn; true: every element is accounted for.
+// `seen` and the kinds among the values of keys `from` to `to`, which all rows in question see, by a team's warps in turn, or as many of them as account for every element.
 template <int KIND>
-__device__ inline bool look_through(const Attention &a, int s, int g, int from, int to, int rank, int warps, uint32_t are, uint32_t &seen, unsigned int *shared)
+__device__ __noinline__ uint32_t look_through(const Attention &a, int s, int g, int from, int to, int rank, int warps, uint32_t are, uint32_t seen, unsigned int *shared)
 {
     const int lane = threadIdx.x & 31, piece = lane & 15, dim = a.pages.dim;
     const bool active = piece < dim / 8;
     const auto *data = static_cast<const typename Held8<KIND>::Element *>(a.pages.data) + piece * 8;
-    bool all = __all_sync(0xffffffffu, open_kinds(are, seen) == 0);
-    if (all) return true;
+    const long long to_key = static_cast<long long>(a.pages.kv_heads) << a.pages.page_shift;   // rows from a key's to its value's
+    if (__all_sync(0xffffffffu, open_kinds(are, seen) == 0)) return seen;
     over_groups(a, s, g, 1, from, to, rank, warps, [&](long long at, int key0) {
         typename Held8<KIND>::Raw v[8];
         bool any = false;
@@ -878,9 +880,18 @@ __device__ inline bool look_through(const Attention &a, int s, int g, int from, 
         }
 #pragma unroll
         for (int u = 0; u < 8; ++u) any = any || not_finite(v[u]);
-        if (any) {
+        if (__any_sync(0xffffffffu, any)) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) seen |= kinds_of(v[u]);
+            for (int u = 0; u < 8; ++u) {
+                uint32_t kinds = kinds_of(v[u]);
+                if (__any_sync(0xffffffffu, kinds & kSeenInfinities)) {
+                    typename Held8<KIND>::Raw k;
+                    k.zero();
+                    if (at >= 0 && active && key0 + u >= from && key0 + u <= to) k.load(data + (at + u - to_key) * dim);
+                    if ((__ballot_sync(0xffffffffu, not_finite(k)) >> (lane & 16)) & 0xffffu) kinds = (kinds | kinds >> 8 | kinds >> 16) & kSeenNan;
+                }
+                seen |= kinds;
+            }
         }
         seen |= __shfl_xor_sync(0xffffffffu, seen, 16);
         if (shared) {
@@ -888,10 +899,9 @@ __device__ inline bool look_through(const Attention &a, int s, int g, int from, 
             __syncwarp();
             seen |= *reinterpret_cast<volatile unsigned int *>(shared + piece);
         }
-        all = __all_sync(0xffffffffu, open_kinds(are, seen) == 0);
-        return !all;
+        return __all_sync(0xffffffffu, open_kinds(are, seen) == 0) == 0;
     });
-    return all;
+    return seen;
 }
 
 // The rows of u.rows (row r: packed row packed0 + r), by a team of WARPS warps that `sync` brings together; the outputs have been stored, and u.rows is known to all.
@@ -912,7 +922,7 @@ __device__ __noinline__ void settle_rows(const Attention &a, int s, int g, int r
     auto head_of = [&](int r) { return g * a.share + packed0 + r - token_of(r) * a.share; };
     auto stored = [&](int r, Raw8<T> &raw) {
         raw.zero();
-        if (active && r <= last && is_in(r)) raw.load(static_cast<const T *>(a.out) + (row0 + token_of(r)) * a.out_pitch + head_of(r) * dim + piece * 8);
+        if (active && r < 128 && is_in(r)) raw.load(static_cast<const T *>(a.out) + (row0 + token_of(r)) * a.out_pitch + head_of(r) * dim + piece * 8);
     };
     if (rank == 0 && half == 0) u.are[piece] = u.seen[piece] = u.again[piece & 3] = 0u;
     sync();
@@ -927,30 +937,40 @@ __device__ __noinline__ void settle_rows(const Attention &a, int s, int g, int r
     if (are) atomicOr(u.are + piece, are);
     sync();
     const int p0 = pos0 + token_of(first), p1 = pos0 + token_of(last), low = a.window ? max(0, p1 - a.window + 1) : 0;
-    uint32_t seen = 0;
     are = u.are[piece];
-    if (!look_through<KIND>(a, s, g, 0, min(min(a.sinks, low) - 1, p0), rank, WARPS, are, seen, u.seen)) look_through<KIND>(a, s, g, low, p0, rank, WARPS, are, seen, u.seen);
+    uint32_t seen = look_through<KIND>(a, s, g, 0, min(min(a.sinks, low) - 1, p0), rank, WARPS, are, 0, u.seen);
+    look_through<KIND>(a, s, g, low, p0, rank, WARPS, are, seen, u.seen);
     sync();
     const uint32_t by_all = u.seen[piece];
     if (__all_sync(0xffffffffu, open_kinds(are, by_all) == 0)) last = -1;   // the same in all warps: what accounts for all rows' elements does so for each row's
-    for (int r = first, n = 0; r <= last; ++r) {
-        if (!is_in(r) || n++ % WARPS != rank) continue;
+    // by one warp; false: an element is left that nothing explains
+    auto explained = [&](int r) {
         const int token = token_of(r), position = pos0 + token, from = a.window ? max(0, position - a.window + 1) : 0;
         Raw8<T> raw;
         stored(r, raw);
         are = kinds_of(raw);
-        seen = by_all;
         // what this row sees and the others may not: behind the first of them, in front of the last one's window
-        if (look_through<KIND>(a, s, g, max(p0 + 1, from), position, 0, 1, are, seen, nullptr) || look_through<KIND>(a, s, g, p0 + 1, min(a.sinks, from) - 1, 0, 1, are, seen, nullptr) ||
-            look_through<KIND>(a, s, g, from, min(low - 1, p0), 0, 1, are, seen, nullptr))
-            continue;
-        if (lane == 0) atomicOr(u.again + (r >> 5), 1u << (r & 31));
-    }
+        seen = look_through<KIND>(a, s, g, max(p0 + 1, from), position, 0, 1, are, by_all, nullptr);
+        seen = look_through<KIND>(a, s, g, p0 + 1, min(a.sinks, from) - 1, 0, 1, are, seen, nullptr);
+        seen = look_through<KIND>(a, s, g, from, min(low - 1, p0), 0, 1, are, seen, nullptr);
+        if (__all_sync(0xffffffffu, open_kinds(are, seen) == 0)) return true;
+        const uint32_t open = open_kinds(are, seen), elements = open | open >> 8 | open >> 16;
+        float v[8];
+        raw.get(v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e)   // not both: that accounts for a NaN, and an infinity has not met the other one
+            if (elements >> e & 1 && seen >> e & 0x10100u) v[e] = seen >> e & 0x100u ? INFINITY : -INFINITY;
+        if (active && half == 0) store8(static_cast<T *>(a.out) + (row0 + token) * a.out_pitch + head_of(r) * dim + piece * 8, v);
+        return __all_sync(0xffffffffu, (elements & ~(seen >> 8 | seen >> 16) & kSeenNan) == 0) != 0;
+    };
+    for (int r = first, n = 0; r <= last; ++r)
+        if (is_in(r) && n++ % WARPS == rank && !explained(r) && lane == 0) atomicOr(u.again + (r >> 5), 1u << (r & 31));
     sync();
     for (int w = 0; w < 4; ++w)
         for (unsigned int rest = u.again[w]; rest; rest &= rest - 1) {
             const int r = 32 * w + __ffs(rest) - 1, token = token_of(r);
             attention_row<T, KIND, WARPS>(a, s, pos0 + token, row0 + token, head_of(r), rank, lane, room, sync);
+            if (rank == 0) explained(r);   // its sums may have met infinities, too
         }
     sync();   // what the next tile writes has been read
 }

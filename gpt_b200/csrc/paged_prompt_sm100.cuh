@@ -824,7 +824,7 @@ paged_prompt_kernel(const __grid_constant__ PromptArgs args)
                 }
                 const uint32_t bad = __ballot_sync(0xffffffffu, done && there && sees && check != 0.0f && divisor > 0.0f && divisor <= FLT_MAX);
                 if (lane == 0) unsure[h].rows[quarter] = bad;
-                if (!pro::all_of(4 + h, 128, bad == 0)) {
+                if (__builtin_expect(!pro::all_of(4 + h, 128, bad == 0), 0)) {
                     if (r == 0) atomicAdd(&working, 1u);
                     settle_rows<__nv_bfloat16, kind, 4>(a, seg.s, seg.g, seg.row0, seg.pos0, seg.packed0 + h * 128, unsure[h], quarter, reinterpret_cast<float *>(gen + (staging - base) + 4 * h * 2048),
                                                         pro::HalfSync{4 + h});

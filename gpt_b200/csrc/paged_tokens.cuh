@@ -261,7 +261,7 @@ __device__ __forceinline__ void finish_tile(const Attention &a, const Parts &par
         }
     }
     __syncthreads();
-    if (unsure.rows[0]) settle_rows<T, KIND, kTokensWarps>(a, place.s, place.g, place.q.row0, place.q.pos0, packed0, unsure, warp, reinterpret_cast<float *>(sums), BlockSync());
+    if (__builtin_expect(unsure.rows[0] != 0u, 0)) settle_rows<T, KIND, kTokensWarps>(a, place.s, place.g, place.q.row0, place.q.pos0, packed0, unsure, warp, reinterpret_cast<float *>(sums), BlockSync());
     __syncthreads();   // what the next tile writes again has been read
 }
 
