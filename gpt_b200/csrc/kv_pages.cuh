@@ -830,7 +830,7 @@ __device__ void attention_row(const Attention &a, int s, int position, int row, 
 // fp32's range.  In the first case the result stands: an element that is NaN where the row sees a NaN or infinities of both signs there, one that is infinite where it sees that
 // infinity.  All rows of a tile see nearly the same keys, so a team of warps goes over the values that all of these rows see once, and stops as soon as every element is accounted
 // for; each row then looks at the few others that it sees.  A NaN where the row sees one infinity alone becomes that infinity: every weight is positive, though the product may have
-// met one that fp32 does not hold, or a negative second term.  (But a key that is not finite has weight 0, or the weights had no sum; 0 times an infinity is NaN.)  Rows with an element
+// met one that fp32 does not hold, or a negative second term.  (But without a cap a key that is not finite has weight 0, or the weights had no sum; 0 times an infinity is NaN.)  Rows with an element
 // that none of this explains are formed again from their own keys alone.
 
 constexpr uint32_t kSeenNan = 0xffu, kSeenInfinities = 0xffff00u;   // a bit per element: NaN, plus infinity, minus infinity
@@ -884,7 +884,7 @@ __device__ __noinline__ uint32_t look_through(const Attention &a, int s, int g, 
 #pragma unroll
             for (int u = 0; u < 8; ++u) {
                 uint32_t kinds = kinds_of(v[u]);
-                if (__any_sync(0xffffffffu, kinds & kSeenInfinities)) {
+                if (a.cap == 0.0f && __any_sync(0xffffffffu, kinds & kSeenInfinities)) {
                     typename Held8<KIND>::Raw k;
                     k.zero();
                     if (at >= 0 && active && key0 + u >= from && key0 + u <= to) k.load(data + (at + u - to_key) * dim);

@@ -306,14 +306,16 @@ def test_sums_at_an_odd_address_are_refused(backend):
 
 @pytest.mark.parametrize("dtype,kind", [("bf16", "bf16"), ("f32", "f32"), ("bf16", "f32"), ("f32", "bf16")])
 @pytest.mark.parametrize("count,share", [(1, 1), (1, 16), (3, 8), (40, 2), (300, 1)])
-@pytest.mark.parametrize("below", [20.0, 95.0, 300.0])
-def test_infinite_values_with_next_to_no_weight(backend, dtype, kind, count, share, below):
-    """A weight of e^-300 is positive, whatever fp32 makes of it: an infinite value makes the output infinite.  Behind a key that is minus infinite the weight is none, and the product NaN."""
+@pytest.mark.parametrize("below,cap", [(20.0, 0.0), (95.0, 0.0), (300.0, 0.0), (20.0, 30.0), (300.0, 400.0)])
+def test_infinite_values_with_next_to_no_weight(backend, dtype, kind, count, share, below, cap):
+    """A weight of e^-300 is positive, whatever fp32 makes of it: an infinite value makes the output infinite.  Behind a key that is minus infinite the weight is none, and the product NaN,
+    but where a cap bounds the score."""
     inf, length, dim = float("inf"), 500 + count, 64
     c = Cache(kind, [length, 30], [count, 3], 1, dim, 16, seed=3)
     for s in (0, 1):
         for position in range(c.lengths[s]):
             put(c, kind, s, position, 0.0, which=0, element=slice(0, 1))
+    put(c, kind, 0, length - count // 2 - 1, float("nan"), element=12)       # some rows do not see it
     for position, key, values in ((7, -below, {3: inf, 4: -inf, 5: inf}), (9, -below, {5: -inf, 6: inf}), (11, -inf, {8: inf, 9: -inf}), (300, -below, {10: inf}), (length - 1, 0.0, {11: inf})):
         put(c, kind, 0, position, key, which=0, element=0)
         for element, value in values.items():
@@ -322,12 +324,15 @@ def test_infinite_values_with_next_to_no_weight(backend, dtype, kind, count, sha
     q = 0.1 * torch.randn(count + 3, share, dim, generator=torch.Generator().manual_seed(2))
     q[:, :, 0] = 1.0
     q = q.reshape(count + 3, -1).to(torch.bfloat16 if dtype == "bf16" else torch.float32).cuda()
-    out, sums = attend(backend, c, q, share, dtype, 1.0)
+    out, sums = attend(backend, c, q, share, dtype, 1.0, cap)
     backend.synchronize()
     got = kinds(out.double().cpu().reshape(count + 3, share, dim))
     want = torch.zeros_like(got)
     want[:count, :, [3, 6, 10]] = 2
     want[:count, :, 4] = 3
-    want[:count, :, [5, 8, 9]] = 1
+    want[:count, :, 5] = 1
+    want[:count, :, 8] = 2 if cap else 1
+    want[:count, :, 9] = 3 if cap else 1
     want[count - 1, :, 11] = 2
+    want[count - count // 2 - 1:count, :, 12] = 1
     assert torch.equal(got, want)
